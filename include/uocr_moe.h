@@ -131,6 +131,46 @@ UOCR_API int uocr_paged_decode_attention(const float* q, const float* k_new, con
                                 const uint32_t* write_index, const uint32_t* attend_len, float scale,
                                 float* out, void* workspace, size_t workspace_bytes, uocr_stream_t stream);
 
+/* Attention of a chunk of new tokens over the page pool, stored by the same call: what
+ * paged_decode_attention (decoder.py:425-437) is for one row per request, for any number of them.
+ * q, k_new, v_new, out and the pool are of one type (UOCR_DTYPE_F32 or UOCR_DTYPE_BF16). New row t lies
+ * at q + t * q_ld elements ([heads][128], heads a multiple of kv_heads; query head h reads KV head
+ * h / (heads / kv_heads)), k_new + t * k_ld and v_new + t * v_ld ([kv_heads][128]); out is [T][heads][128]
+ * and overlaps no input. Request b's new rows are [row_offsets[b], row_offsets[b + 1]) (device int32
+ * [B + 1], ascending, within T; an empty request has none); its i-th one is logical row
+ * p = start[b] + i, stored at row p % 128 of page lut[b * lut_cols + p / 128], and attends the logical
+ * rows r <= p, all of them (window 0) or those with r > p - window or r < prefix[b] (window >= 1; prefix
+ * null: 0). Rows below start[b] are read from the pool (page ids past the pool read its last page), the
+ * new rows from k_new and v_new; new rows beyond the lookup table or with a page id past the pool are
+ * attended but not stored. Rows of out in no request are left as they were. What a row does not see
+ * does not reach it, whatever it holds (NaN and infinities included).
+ * Sums and softmax in fp32. The workspace (uocr_paged_chunk_workspace_bytes() bytes on the current
+ * device, 256-byte aligned, no initial contents) belongs to the call until it has finished. The
+ * result is deterministic (a fixed split and order on one kind of GPU). */
+UOCR_API size_t uocr_paged_chunk_workspace_bytes(void);
+UOCR_API int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, int64_t k_ld, const void* v_new,
+                               int64_t v_ld, int64_t T, int64_t heads, int64_t kv_heads, int64_t head_dim, int dtype,
+                               void* kv_pool, int64_t pages, int64_t layers, int64_t layer, const uint32_t* lut,
+                               int64_t lut_cols, const int32_t* row_offsets, const int32_t* start, int64_t B,
+                               float scale, int64_t window, const int32_t* prefix, void* out, void* workspace,
+                               size_t workspace_bytes, uocr_stream_t stream);
+
+/* Pages of a pool [pages][2][layers][128 rows][row_bytes] copied, in every layer, k and v: page dst[i] takes
+ * the first rows[i] rows (rows null: all 128) of page src[i], i < n. The rest of dst[i] stays. The dst
+ * pages are distinct and no src page is among them; an entry with a page id outside the pool is
+ * skipped. row_bytes a multiple of 16 (heads x 128 x the element size). No counterpart in the reference. */
+UOCR_API int uocr_copy_pages(void* kv_pool, int64_t pages, int64_t layers, int64_t row_bytes, const int32_t* src,
+                    const int32_t* dst, const int32_t* rows, int64_t n, uocr_stream_t stream);
+/* Rows of B requests compacted, in every layer, k and v: logical row i of request b in dst_lut
+ * [B][dst_cols] takes its logical row keep[b * max_keep + i] in src_lut [B][src_cols], for
+ * i < min(keep_len[b], max_keep). keep[b] ascends strictly, so that dst_lut may hold the same pages at
+ * the same places as src_lut (in place); other pages of dst_lut occur in no request's src_lut. A row that
+ * lies beyond its table, or whose page id is outside the pool, is skipped. No counterpart in the
+ * reference. */
+UOCR_API int uocr_compact_rows(void* kv_pool, int64_t pages, int64_t layers, int64_t row_bytes, const int32_t* src_lut,
+                      int64_t src_cols, const int32_t* dst_lut, int64_t dst_cols, const int32_t* keep,
+                      int64_t max_keep, const int32_t* keep_len, int64_t B, uocr_stream_t stream);
+
 /* RoPE on the decode step's fused q|k|v projection output qkv [B][3 x heads x head_dim] (q, then k,
  * then v, each heads x head_dim): q = x_q cos + rotate_half(x_q) sin, k likewise, v copied, into
  * q, k, v [B][heads][head_dim]; cos, sin [B][head_dim] are the rotary table's rows at each row's

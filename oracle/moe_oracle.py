@@ -530,3 +530,50 @@ def paged_decode_attention_ref(q, k_new, v_new, pool, layer, lut, write_index, a
         p /= p.sum(axis=1, keepdims=True)
         out[b] = np.einsum("hr,rhd->hd", p, V)
     return out, pool
+
+
+def chunk_visible(p, rows, window, prefix):
+    """Which of logical rows 0 .. rows - 1 the token at logical row ``p`` sees (bool [rows])."""
+    r = np.arange(rows)
+    seen = r <= p
+    if window:
+        seen &= (r > p - window) | (r < prefix)
+    return seen
+
+
+def paged_chunk_attention_ref(q, k_new, v_new, pool, layer, lut, row_offsets, start, scale, window=0, prefix=None,
+                              out=None):
+    """float64 restatement of the chunk attention: request b's new rows (row_offsets[b] .. row_offsets[b + 1])
+    stored from logical row start[b] on, then each attended over the rows it sees, and those alone.
+    All arrays fp32 or fp64. Returns (out fp64 [T, heads, dim], the magnitudes that its error scales
+    with: sum of p |v| [T, heads, dim] and max over the visible rows of scale * sum |q k| [T, heads], the
+    pool after the store). Rows in no request keep ``out``'s."""
+    pool = np.array(pool, copy=True)
+    T, heads, dim = q.shape
+    kv_heads = k_new.shape[1]
+    got = np.zeros(q.shape, np.float64) if out is None else np.array(out, np.float64)
+    mag, smag = np.zeros(q.shape), np.zeros((T, heads))
+    for b in range(len(start)):
+        lo, hi, s0 = int(row_offsets[b]), int(row_offsets[b + 1]), int(start[b])
+        if hi <= lo:
+            continue
+        n = s0 + hi - lo
+        place = lambda r: (int(lut[b, r // 128]), r % 128)  # noqa: E731
+        for i in range(hi - lo):
+            page, slot = place(s0 + i)
+            pool[page, 0, layer, slot] = k_new[lo + i]
+            pool[page, 1, layer, slot] = v_new[lo + i]
+        K = np.stack([pool[place(r)[0], 0, layer, place(r)[1]] for r in range(n)]).astype(np.float64)
+        V = np.stack([pool[place(r)[0], 1, layer, place(r)[1]] for r in range(n)]).astype(np.float64)
+        for i in range(hi - lo):
+            seen = chunk_visible(s0 + i, n, window, 0 if prefix is None else int(prefix[b]))
+            for h in range(heads):
+                hk = h // (heads // kv_heads)
+                x, kk, vv = q[lo + i, h].astype(np.float64), K[seen, hk], V[seen, hk]
+                s = kk @ x * scale
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                got[lo + i, h] = p @ vv
+                mag[lo + i, h] = p @ np.abs(vv)
+                smag[lo + i, h] = (np.abs(kk) @ np.abs(x)).max() * abs(scale)
+    return got, mag, smag, pool

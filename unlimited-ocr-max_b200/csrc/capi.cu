@@ -310,6 +310,93 @@ int uocr_paged_decode_attention(const float* q, const float* k_new, const float*
                        "paged_decode_attention: launch");
 }
 
+size_t uocr_paged_chunk_workspace_bytes(void) { return uocr::chunk_workspace_bytes(current_sms()); }
+
+int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, int64_t k_ld, const void* v_new,
+                               int64_t v_ld, int64_t T, int64_t heads, int64_t kv_heads, int64_t head_dim, int dtype,
+                               void* kv_pool, int64_t pages, int64_t layers, int64_t layer, const uint32_t* lut,
+                               int64_t lut_cols, const int32_t* row_offsets, const int32_t* start, int64_t B,
+                               float scale, int64_t window, const int32_t* prefix, void* out, void* workspace,
+                               size_t workspace_bytes, uocr_stream_t stream) {
+    if (head_dim != 128)
+        return fail(UOCR_EUNSUPPORTED, "paged_chunk_attention: head_dim %lld (this build: 128)", (long long)head_dim);
+    if (dtype != UOCR_DTYPE_F32 && dtype != UOCR_DTYPE_BF16)
+        return fail(UOCR_EINVAL, "paged_chunk_attention: dtype %d is neither fp32 nor bf16", dtype);
+    if (heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 1024)
+        return fail(UOCR_EINVAL, "paged_chunk_attention: %lld heads over %lld KV heads (a multiple, at most 1024)",
+                    (long long)heads, (long long)kv_heads);
+    // rows and pairs are counted in 32 bits: T x the heads of a group, and the tables' rows, stay below 2^30
+    if (T < 0 || T * (heads / kv_heads) > (int64_t(1) << 30) || B < 0 || B > (1 << 20))
+        return fail(UOCR_EINVAL, "paged_chunk_attention: bad T %lld or B %lld", (long long)T, (long long)B);
+    if (pages < 1 || pages > INT32_MAX || layers < 1 || layers > INT32_MAX || layer < 0 || layer >= layers ||
+        lut_cols < 1 || lut_cols > (1 << 22))
+        return fail(UOCR_EINVAL, "paged_chunk_attention: bad pool (pages %lld, layers %lld, layer %lld, lut_cols %lld)",
+                    (long long)pages, (long long)layers, (long long)layer, (long long)lut_cols);
+    if (window < 0 || window > INT32_MAX)
+        return fail(UOCR_EINVAL, "paged_chunk_attention: window %lld (0: none, else at least 1)", (long long)window);
+    const int64_t unit = dtype == UOCR_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
+    if (q_ld < heads * 128 || k_ld < kv_heads * 128 || v_ld < kv_heads * 128 || q_ld % unit || k_ld % unit || v_ld % unit)
+        return fail(UOCR_EINVAL, "paged_chunk_attention: row strides %lld, %lld, %lld (at least a row, multiples of 16 bytes)",
+                    (long long)q_ld, (long long)k_ld, (long long)v_ld);
+    if (!(scale == scale) || scale - scale != 0.f)
+        return fail(UOCR_EINVAL, "paged_chunk_attention: the scale is not finite");
+    if (B == 0 || T == 0) return ok();
+    const size_t need = uocr_paged_chunk_workspace_bytes();
+    if (!q || !k_new || !v_new || !kv_pool || !lut || !row_offsets || !start || !out || (need && !workspace))
+        return fail(UOCR_EINVAL, "paged_chunk_attention: null pointer");
+    if (!a16(q) || !a16(k_new) || !a16(v_new) || !a16(kv_pool) || !a16(out))
+        return fail(UOCR_EINVAL, "paged_chunk_attention: q, k_new, v_new, the pool and out must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(workspace) & 255)
+        return fail(UOCR_EINVAL, "paged_chunk_attention: workspace must be 256-byte aligned");
+    if (workspace_bytes < need)
+        return fail(UOCR_EINVAL, "paged_chunk_attention: workspace of %zu bytes, need %zu", workspace_bytes, need);
+    uocr::ChunkArgs a{};
+    a.q = q; a.k = k_new; a.v = v_new; a.q_ld = q_ld; a.k_ld = k_ld; a.v_ld = v_ld;
+    a.out = out; a.pool = kv_pool; a.lut = lut; a.offsets = row_offsets; a.start = start;
+    a.prefix = window ? prefix : nullptr;
+    a.T = (int)T; a.B = (int)B; a.heads = (int)heads; a.kv_heads = (int)kv_heads; a.pages = (int)pages;
+    a.layers = (int)layers; a.layer = (int)layer; a.lut_cols = (int)lut_cols; a.window = (int)window;
+    a.bf16 = dtype == UOCR_DTYPE_BF16; a.scale = scale;
+    return cuda_status(uocr::launch_chunk_attention(a, workspace, current_sms(), S(stream)),
+                       "paged_chunk_attention: launch");
+}
+
+static int check_pages(const char* who, int64_t pages, int64_t layers, int64_t row_bytes) {
+    if (pages < 1 || pages > INT32_MAX || layers < 1 || layers > 32767 || row_bytes < 16 || row_bytes % 16 ||
+        row_bytes > (1 << 23))
+        return fail(UOCR_EINVAL, "%s: bad pool (pages %lld, layers %lld, row_bytes %lld)", who, (long long)pages,
+                    (long long)layers, (long long)row_bytes);
+    return UOCR_OK;
+}
+
+int uocr_copy_pages(void* kv_pool, int64_t pages, int64_t layers, int64_t row_bytes, const int32_t* src,
+                    const int32_t* dst, const int32_t* rows, int64_t n, uocr_stream_t stream) {
+    if (int rc = check_pages("copy_pages", pages, layers, row_bytes)) return rc;
+    if (n < 0 || n > INT32_MAX) return fail(UOCR_EINVAL, "copy_pages: bad n %lld", (long long)n);
+    if (n == 0) return ok();
+    if (!kv_pool || !src || !dst) return fail(UOCR_EINVAL, "copy_pages: null pointer");
+    if (!a16(kv_pool)) return fail(UOCR_EINVAL, "copy_pages: the pool must be 16-byte aligned");
+    return cuda_status(uocr::launch_copy_pages(kv_pool, (int)pages, (int)layers, (int)row_bytes, src, dst, rows, (int)n,
+                                               S(stream)),
+                       "copy_pages: launch");
+}
+
+int uocr_compact_rows(void* kv_pool, int64_t pages, int64_t layers, int64_t row_bytes, const int32_t* src_lut,
+                      int64_t src_cols, const int32_t* dst_lut, int64_t dst_cols, const int32_t* keep,
+                      int64_t max_keep, const int32_t* keep_len, int64_t B, uocr_stream_t stream) {
+    if (int rc = check_pages("compact_rows", pages, layers, row_bytes)) return rc;
+    if (B < 0 || B > 65535 || max_keep < 0 || max_keep > (1 << 29) || src_cols < 1 || src_cols > (1 << 22) ||
+        dst_cols < 1 || dst_cols > (1 << 22))
+        return fail(UOCR_EINVAL, "compact_rows: bad shape (B %lld, max_keep %lld, src_cols %lld, dst_cols %lld)",
+                    (long long)B, (long long)max_keep, (long long)src_cols, (long long)dst_cols);
+    if (B == 0 || max_keep == 0) return ok();
+    if (!kv_pool || !src_lut || !dst_lut || !keep || !keep_len) return fail(UOCR_EINVAL, "compact_rows: null pointer");
+    if (!a16(kv_pool)) return fail(UOCR_EINVAL, "compact_rows: the pool must be 16-byte aligned");
+    return cuda_status(uocr::launch_compact_rows(kv_pool, (int)pages, (int)layers, (int)row_bytes, src_lut, (int)src_cols,
+                                                 dst_lut, (int)dst_cols, keep, (int)max_keep, keep_len, (int)B, S(stream)),
+                       "compact_rows: launch");
+}
+
 int uocr_rope_qkv(const float* qkv, int64_t B, int64_t heads, int64_t head_dim, const float* cos, const float* sin,
                   float* q, float* k, float* v, uocr_stream_t stream) {
     // Attention._rope / Attention.decode, decoder.py:459-462, 478-493

@@ -47,6 +47,28 @@ cudaError_t launch_paged_decode_attention(const float* q, const float* k_new, co
                                           int heads, float scale, uint32_t* ctl, float* partial, int S,
                                           cudaStream_t st);
 
+// chunk.cu: attention of a chunk of new tokens over the paged cache (q, k, v, out and the pool fp32 or bf16)
+struct ChunkArgs {
+    const void *q, *k, *v;              // new row t at t * ld elements, [heads or kv_heads][128] in it
+    long long q_ld, k_ld, v_ld;
+    void* out;                          // [T][heads][128]
+    void* pool;                         // [pages][2][layers][128 rows][kv_heads][128]
+    const uint32_t* lut;                // [B][lut_cols]
+    const int32_t *offsets, *start;     // [B + 1], [B]
+    const int32_t* prefix;              // [B] or null
+    int T, B, heads, kv_heads, pages, layers, layer, lut_cols, window, bf16;
+    float scale;
+};
+size_t chunk_workspace_bytes(int sms);
+cudaError_t launch_chunk_attention(const ChunkArgs& a, void* ws, int sms, cudaStream_t st);
+
+// pages.cu: pages copied (their first rows[i] rows; null: whole), and kept rows moved to the front
+cudaError_t launch_copy_pages(void* pool, int pages, int layers, int row_bytes, const int32_t* src, const int32_t* dst,
+                              const int32_t* rows, int n, cudaStream_t st);
+cudaError_t launch_compact_rows(void* pool, int pages, int layers, int row_bytes, const int32_t* src_lut, int src_cols,
+                                const int32_t* dst_lut, int dst_cols, const int32_t* keep, int max_keep,
+                                const int32_t* keep_len, int B, cudaStream_t st);
+
 // rope.cu: RoPE on the fused q|k|v rows [B, 3 x heads x dim] -> q, k (rotated), v, each [B, heads, dim]
 cudaError_t launch_rope_qkv(const float* qkv, int B, int heads, int dim, const float* cos, const float* sin, float* q,
                             float* k, float* v, cudaStream_t st);

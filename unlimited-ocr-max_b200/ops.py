@@ -271,3 +271,145 @@ def silu_mul(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Te
         out = torch.empty((gate_up.shape[0], inter), dtype=torch.float32, device=gate_up.device)
     check(load().uocr_silu_mul(gate_up.data_ptr(), gate_up.shape[0], inter, out.data_ptr(), _stream(gate_up)))
     return out
+
+
+def _pool_dims(op: str, kv_pool: torch.Tensor) -> tuple[int, int, int, int]:
+    """(pages, layers, heads, bytes of a row) of a page pool, which is used in place."""
+    if kv_pool.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{op}: the pool must be fp32 or bf16, got {kv_pool.dtype}")
+    if kv_pool.dim() != 6 or kv_pool.shape[1] != 2 or kv_pool.shape[3] != 128 or kv_pool.shape[5] != 128:
+        raise ValueError(f"{op}: the pool must be [pages, 2, layers, 128, heads, 128], got {tuple(kv_pool.shape)}")
+    if not kv_pool.is_contiguous():
+        raise ValueError(f"{op}: the pool must be contiguous (it is written in place)")
+    pages, _, layers, _, heads, dim = kv_pool.shape
+    return pages, layers, heads, heads * dim * kv_pool.element_size()
+
+
+def _index(op: str, t: torch.Tensor, name: str, shape: tuple[int, ...]) -> torch.Tensor:
+    t = _need(op, t, name, torch.int32, len(shape))
+    if t.shape != shape:
+        raise ValueError(f"{op}: {name} must be {list(shape)}, got {list(t.shape)}")
+    return t
+
+
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    """The byte range that a tensor's elements lie in."""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def paged_chunk_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, kv_pool: torch.Tensor, layer: int,
+                          lut: torch.Tensor, row_offsets: torch.Tensor, start: torch.Tensor, scale: float, *,
+                          window: int = 0, prefix: torch.Tensor | None = None,
+                          out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a chunk of new tokens per request over the paged cache (decoder.py:425-437 for any
+    number of new rows): store them in ``layer`` of ``kv_pool [pages, 2, layers, 128, kv_heads, 128]`` and
+    attend.
+
+    ``q [T, heads, 128]`` and ``k_new`` / ``v_new [T, kv_heads, 128]`` are of the pool's type, fp32 or bf16;
+    ``heads`` is a multiple of ``kv_heads``; rows may be strided (slices of a fused projection's rows).
+    Request ``b`` owns rows ``row_offsets[b]`` to ``row_offsets[b + 1]`` (int32 ``[B + 1]``, none for an empty
+    request) at its logical rows ``start[b]``, ``start[b] + 1``, ... (int32 ``[B]``); ``lut [B, cols]`` (int32
+    or uint32) holds its page ids. A token at logical row ``p`` sees the rows ``r <= p``; with ``window >= 1``
+    only those with ``r > p - window`` or ``r < prefix[b]`` (int32 ``[B]``; None: 0). ``out [T, heads, 128]``
+    (contiguous, overlapping no input) is returned; its rows in no request keep what they held. All index
+    tensors are on the device, and nothing synchronises; the workspace is the call's own, so calls may run
+    on several streams and be captured. The result is deterministic.
+    """
+    op = "paged_chunk_attention"
+    extra = [t for t in (prefix, out) if t is not None]
+    _need_cuda(op, q, k_new, v_new, kv_pool, lut, row_offsets, start, *extra)
+    pages, layers, kv_heads, _ = _pool_dims(op, kv_pool)
+    dt = kv_pool.dtype
+    for name, t in (("q", q), ("k_new", k_new), ("v_new", v_new)):
+        if t.dtype != dt:
+            raise TypeError(f"{op}: {name} must be {dt} like the pool, got {t.dtype}")
+        if t.dim() != 3:
+            raise ValueError(f"{op}: {name} must be rank 3, got shape {tuple(t.shape)}")
+    T, heads, dim = q.shape
+    if k_new.shape != (T, kv_heads, 128) or v_new.shape != k_new.shape or dim != 128:
+        raise ValueError(f"{op}: q [T, heads, 128], k_new and v_new [T, {kv_heads}, 128] expected, got {tuple(q.shape)}, "
+                         f"{tuple(k_new.shape)}, {tuple(v_new.shape)}")
+    if lut.dtype not in (torch.int32, torch.uint32):
+        raise TypeError(f"{op}: lut must be int32 or uint32, got {lut.dtype}")
+    if lut.dim() != 2:
+        raise ValueError(f"{op}: lut must be [B, cols], got {tuple(lut.shape)}")
+    lut = lut.contiguous()
+    B = lut.shape[0]
+    row_offsets = _index(op, row_offsets, "row_offsets", (B + 1,))
+    start = _index(op, start, "start", (B,))
+    if prefix is not None:
+        prefix = _index(op, prefix, "prefix", (B,))
+    step = 16 // dt.itemsize
+
+    def rows(t):  # a row's heads are read as one run; rows may lie apart
+        whole = t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == 128)
+        if whole and (T <= 1 or (t.stride(0) >= t.shape[1] * 128 and t.stride(0) % step == 0)) and t.data_ptr() % 16 == 0:
+            return t, (t.stride(0) if T > 1 else t.shape[1] * 128)
+        t = t.clone(memory_format=torch.contiguous_format)
+        return t, t.shape[1] * 128
+
+    q, q_ld = rows(q)
+    k_new, k_ld = rows(k_new)
+    v_new, v_ld = rows(v_new)
+    if out is None:
+        out = torch.empty((T, heads, 128), dtype=dt, device=q.device)
+    elif out.dtype != dt or out.shape != (T, heads, 128) or not out.is_contiguous():
+        raise ValueError(f"{op}: out must be a contiguous {dt} tensor of shape {(T, heads, 128)}")
+    else:
+        lo, hi = _extent(out)
+        for name, t in (("q", q), ("k_new", k_new), ("v_new", v_new), ("the pool", kv_pool)):
+            a, z = _extent(t)
+            if a < hi and lo < z:
+                raise ValueError(f"{op}: out overlaps {name}")
+    with torch.cuda.device(q.device):
+        need = load().uocr_paged_chunk_workspace_bytes()
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        check(load().uocr_paged_chunk_attention(
+            q.data_ptr(), q_ld, k_new.data_ptr(), k_ld, v_new.data_ptr(), v_ld, T, heads, kv_heads, dim,
+            1 if dt == torch.bfloat16 else 0, kv_pool.data_ptr(), pages, layers, layer, lut.data_ptr(), lut.shape[1],
+            row_offsets.data_ptr(), start.data_ptr(), B, float(scale), int(window),
+            0 if prefix is None else prefix.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(q)))
+    return out
+
+
+def copy_pages(kv_pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *, rows: torch.Tensor | None = None) -> None:
+    """Page ``dst[i]`` of ``kv_pool [pages, 2, layers, 128, heads, 128]`` (fp32 or bf16) takes the first
+    ``rows[i]`` rows (None: all 128) of page ``src[i]``, in every layer, k and v; the rest of it stays.
+    ``src``, ``dst`` and ``rows`` are int32 ``[n]`` on the device. The ``dst`` pages are distinct and hold no
+    ``src`` page; an entry with a page id outside the pool is skipped."""
+    op = "copy_pages"
+    _need_cuda(op, kv_pool, src, dst, *([] if rows is None else [rows]))
+    pages, layers, _, row_bytes = _pool_dims(op, kv_pool)
+    src = _need(op, src, "src", torch.int32, 1)
+    dst = _index(op, dst, "dst", tuple(src.shape))
+    if rows is not None:
+        rows = _index(op, rows, "rows", tuple(src.shape))
+    with torch.cuda.device(kv_pool.device):
+        check(load().uocr_copy_pages(kv_pool.data_ptr(), pages, layers, row_bytes, src.data_ptr(), dst.data_ptr(),
+                                     0 if rows is None else rows.data_ptr(), src.shape[0], _stream(kv_pool)))
+
+
+def compact_rows(kv_pool: torch.Tensor, src_lut: torch.Tensor, dst_lut: torch.Tensor, keep: torch.Tensor,
+                 keep_len: torch.Tensor) -> None:
+    """Logical row ``i`` of request ``b`` in ``dst_lut [B, dst_cols]`` takes its logical row ``keep[b, i]`` in
+    ``src_lut [B, src_cols]``, for ``i < keep_len[b]``, in every layer of ``kv_pool`` (fp32 or bf16), k and v.
+    All are int32 on the device; ``keep[b]`` ascends strictly. ``dst_lut`` may hold the same pages at the
+    same places as ``src_lut`` (in place); its other pages occur in no request's ``src_lut``. Rows beyond
+    the tables, or with a page id outside the pool, are skipped."""
+    op = "compact_rows"
+    _need_cuda(op, kv_pool, src_lut, dst_lut, keep, keep_len)
+    pages, layers, _, row_bytes = _pool_dims(op, kv_pool)
+    src_lut = _need(op, src_lut, "src_lut", torch.int32, 2)
+    dst_lut = _need(op, dst_lut, "dst_lut", torch.int32, 2)
+    keep = _need(op, keep, "keep", torch.int32, 2)
+    keep_len = _need(op, keep_len, "keep_len", torch.int32, 1)
+    B = keep_len.shape[0]
+    if src_lut.shape[0] != B or dst_lut.shape[0] != B or keep.shape[0] != B:
+        raise ValueError(f"{op}: src_lut, dst_lut, keep and keep_len disagree on the number of requests")
+    with torch.cuda.device(kv_pool.device):
+        check(load().uocr_compact_rows(kv_pool.data_ptr(), pages, layers, row_bytes, src_lut.data_ptr(), src_lut.shape[1],
+                                       dst_lut.data_ptr(), dst_lut.shape[1], keep.data_ptr(), keep.shape[1],
+                                       keep_len.data_ptr(), B, _stream(kv_pool)))
