@@ -146,7 +146,7 @@ UOCR_API int uocr_paged_decode_attention(const float* q, const float* k_new, con
  * does not reach it, whatever it holds (NaN and infinities included).
  * Sums and softmax in fp32. The workspace (uocr_paged_chunk_workspace_bytes() bytes on the current
  * device, 256-byte aligned, no initial contents) belongs to the call until it has finished. The
- * result is deterministic (a fixed split and order on one kind of GPU). */
+ * result is deterministic (a fixed split and order on one kind of GPU). B <= 8192. */
 UOCR_API size_t uocr_paged_chunk_workspace_bytes(void);
 UOCR_API int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, int64_t k_ld, const void* v_new,
                                int64_t v_ld, int64_t T, int64_t heads, int64_t kv_heads, int64_t head_dim, int dtype,

@@ -325,13 +325,20 @@ int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, i
     if (heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 1024)
         return fail(UOCR_EINVAL, "paged_chunk_attention: %lld heads over %lld KV heads (a multiple, at most 1024)",
                     (long long)heads, (long long)kv_heads);
-    // rows and pairs are counted in 32 bits: T x the heads of a group, and the tables' rows, stay below 2^30
-    if (T < 0 || T * (heads / kv_heads) > (int64_t(1) << 30) || B < 0 || B > (1 << 20))
+    // rows are counted in 32 bits: T x the heads of a group, and the tables' rows, stay below 2^30
+    if (T < 0 || T > (int64_t(1) << 30) / (heads / kv_heads) || B < 0)
         return fail(UOCR_EINVAL, "paged_chunk_attention: bad T %lld or B %lld", (long long)T, (long long)B);
+    if (B > uocr::kChunkMaxRequests)
+        return fail(UOCR_EUNSUPPORTED, "paged_chunk_attention: %lld requests (this build: <= %d)", (long long)B,
+                    uocr::kChunkMaxRequests);
     if (pages < 1 || pages > INT32_MAX || layers < 1 || layers > INT32_MAX || layer < 0 || layer >= layers ||
         lut_cols < 1 || lut_cols > (1 << 22))
         return fail(UOCR_EINVAL, "paged_chunk_attention: bad pool (pages %lld, layers %lld, layer %lld, lut_cols %lld)",
                     (long long)pages, (long long)layers, (long long)layer, (long long)lut_cols);
+    // a CTA counts its (query tile, head, page) units in 32 bits
+    if ((T * (heads / kv_heads) / 128 + B) * kv_heads > (int64_t(1) << 38) / (lut_cols + T / 128 + 2))
+        return fail(UOCR_EUNSUPPORTED, "paged_chunk_attention: T %lld over %lld pages a request is too much for one call",
+                    (long long)T, (long long)lut_cols);
     if (window < 0 || window > INT32_MAX)
         return fail(UOCR_EINVAL, "paged_chunk_attention: window %lld (0: none, else at least 1)", (long long)window);
     const int64_t unit = dtype == UOCR_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes

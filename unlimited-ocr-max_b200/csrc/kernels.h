@@ -59,6 +59,7 @@ struct ChunkArgs {
     int T, B, heads, kv_heads, pages, layers, layer, lut_cols, window, bf16;
     float scale;
 };
+constexpr int kChunkMaxRequests = 8192;
 size_t chunk_workspace_bytes(int sms);
 cudaError_t launch_chunk_attention(const ChunkArgs& a, void* ws, int sms, cudaStream_t st);
 
