@@ -16,7 +16,7 @@
 // straight to out; the parts of one that was cut go to the workspace as (m, l, sum) and a second launch
 // joins them in the order of the pages. Every CTA finds its run from the lengths on the device.
 //
-// A CTA: 8 warps load the page's rows into registers (two 32 KB granules in flight), turn them into
+// A CTA: 7 warps load the page's rows into registers (two 32 KB granules in flight), turn them into
 // tensor-core operands in a ring of shared memory, and store the new rows; one warp issues tcgen05.mma;
 // 8 warps do the softmax, two threads per query row. The query operand and the weights P are read by the
 // tensor core from TMEM, so shared memory carries each key and value once:
@@ -43,9 +43,17 @@ namespace {
 constexpr int kPageRows = 128;  // rows of a page, and of a unit
 constexpr int kDim = 128;
 constexpr int kTile = 128;      // (token, head) rows of a query tile
-constexpr int kTeamWarps = 8, kLoadWarps = 8;
+constexpr int kTeamWarps = 8, kLoadWarps = 7;  // with the issuing warp 16: 128 registers a thread
 constexpr int kThreads = 32 * (kTeamWarps + kLoadWarps + 1);
-constexpr int kStages = 6;      // ring of granules: 64 rows of k, or 64 columns of v
+constexpr int kTeamRegs = 112, kLoadRegs = 144;  // of the launch's 16 warps x 128
+static_assert(kTeamWarps * kTeamRegs + (kLoadWarps + 1) * kLoadRegs <= 16 * 128, "the split draws on the launch's registers");
+// Ring of operands: a page's 128 rows of k or of v, as two blocks of 64 columns [128 rows][128 bytes]; fp32: the
+// lo halves behind the hi halves.
+template <bool kF32>
+constexpr int kStageBytes = kF32 ? 65536 : 32768;
+template <bool kF32>
+constexpr int kStages = kF32 ? 3 : 6;
+constexpr int kMaxStages = 6;
 constexpr int kSlotFloats = kTile * (kDim + 2);  // a part: sums [128 columns][128 rows], m [128], l [128]
 constexpr int kInfoInts = 8;    // per CTA: states of its two slots, then the tile's place
 constexpr uint32_t kTeamBar = 1, kLoadBar = 2;
@@ -54,19 +62,6 @@ constexpr float kLog2e = 1.44269504088896341f;
 // TMEM columns
 constexpr uint32_t kColS = 0, kColPv = 256, kColQ = 384;
 
-struct Shared {
-    uint64_t full[kStages], empty[kStages], s_full[2], p_full[2], pv_full, pv_free, q_full, drain;
-    uint32_t tmem;
-    volatile int abort;
-    int left;                    // this CTA's units
-    int b, qt, head, j;          // and where they begin
-    float kscale[8][16];         // by unit: 1 / scale of 8 rows of k
-    float vscale[8][2];          // by unit: 1 / scale of 64 columns of v
-    alignas(16) uint16_t vbad[8][2][8];      // by unit: rows with values that are not finite
-    float vmax[2][kLoadWarps];
-    float xmax[2][2][kTile], xsum[2][kTile];
-};
-
 struct Request {
     int lo, n, start, prefix;
 };
@@ -74,8 +69,8 @@ struct Request {
 UOCR_DEV Request request_at(const ChunkArgs& a, int b) {
     Request r;
     r.lo = min(max(__ldg(a.offsets + b), 0), a.T);
-    r.n = max(min(__ldg(a.offsets + b + 1), a.T) - r.lo, 0);
     r.start = min(max(__ldg(a.start + b), 0), a.lut_cols * kPageRows);
+    r.n = max(min(min(__ldg(a.offsets + b + 1), a.T) - r.lo, a.lut_cols * kPageRows - r.start), 0);
     r.prefix = a.prefix ? max(__ldg(a.prefix + b), 0) : 0;
     return r;
 }
@@ -101,8 +96,13 @@ UOCR_DEV Tile tile_at(const ChunkArgs& a, const Request& r, int qt, int g) {
     return t;
 }
 
+// A CTA's run: its units, and where they begin.
+struct Run {
+    int left, b, qt, head, j;
+};
+
 // The walk over a CTA's units, a segment (pages of one tile and head) at a time; every warp walks by
-// itself.
+// itself, with its walk in shared memory (a register per field would spill).
 struct Walk {
     int b, qt, head, j, n, tiles;  // segment: pages j .. j + n - 1 of the tile's
     int left;                      // units behind this segment
@@ -113,7 +113,7 @@ struct Walk {
         n = min(t.count - j, left);
         left -= n;
     }
-    UOCR_DEV bool begin(const ChunkArgs& a, const Shared& s, int g) {
+    UOCR_DEV bool begin(const ChunkArgs& a, const Run& s, int g) {
         left = s.left;
         if (left <= 0) return false;
         b = s.b, qt = s.qt, head = s.head, j = s.j;
@@ -140,6 +140,19 @@ struct Walk {
         return true;
     }
     UOCR_DEV bool whole() const { return j == 0 && n == t.count; }
+};
+
+struct Shared {
+    uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], p_full[2], pv_full, pv_free, q_full, drain;
+    uint32_t tmem;
+    volatile int abort;
+    Run run;
+    Walk walk[kThreads / 32], done[kTeamWarps];
+    alignas(16) float kscale[8][kPageRows];  // by unit: 1 / scale of each row of k
+    float vscale[8];                         // by unit: 1 / scale of v
+    alignas(16) uint32_t vbad[8][8];         // by unit: each loading warp's rows of v that are not finite
+    float vmax[2][8];
+    float xmax[2][2][kTile], xsum[2][kTile];
 };
 
 template <typename T>
@@ -173,7 +186,7 @@ __device__ void find_run(const ChunkArgs& a, Shared& s, long long* scratch, int 
         const long long ctas = min((long long)gridDim.x, total);
         long long u0 = 0, u1 = 0;
         if ((long long)blockIdx.x < ctas) u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
-        if (lane == 0) s.left = (int)(u1 - u0);
+        if (lane == 0) s.run.left = (int)(u1 - u0);
         if (u1 > u0) {
             int b = 0;
             long long before = 0;  // units in front of request b
@@ -198,7 +211,7 @@ __device__ void find_run(const ChunkArgs& a, Shared& s, long long* scratch, int 
                 if (hit) {
                     if (lane == __ffs(hit) - 1) {
                         const long long in = u0 - (upto - (long long)count * a.kv_heads);
-                        s.b = b, s.qt = q0 + lane, s.head = (int)(in / count), s.j = (int)(in % count);
+                        s.run = Run{s.run.left, b, q0 + lane, (int)(in / count), (int)(in % count)};
                     }
                     break;
                 }
@@ -216,24 +229,28 @@ UOCR_DEV bool wait(Shared& s, uint64_t* bar, uint32_t parity) {
 }
 
 // ---- tensor-core operands ---------------------------------------------------------------------
-// D[tmem] (+)= A[tmem] * B[smem], kind::f16, one thread issues.
-UOCR_DEV void umma_ts_f16(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] * B[smem], kind::f16, one thread issues. The descriptor's upper word is a constant.
+UOCR_DEV void umma_ts_f16(uint32_t d, uint32_t a, uint32_t desc_lo, uint32_t desc_hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(desc_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// A value granule: 64 columns contiguous per row (MN-major), 128-byte swizzle, 8-row groups 1024 bytes
-// apart; the granule is one column block wide, so the stride between column blocks is never used.
-UOCR_DEV uint64_t desc_mn_sw128(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)(1024 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+UOCR_DEV bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
 }
-// M 128, N 64; fp16 or bf16 operands; B from keys (K-major) or values (MN-major: bit 16)
+// Shared-memory descriptors, 128-byte swizzle: 8-row groups 1024 bytes apart (the upper word); keys K-major (the
+// leading stride is not used), values MN-major, their 64-column blocks 16 KB apart.
+constexpr uint32_t kDescHi = (1024 >> 4) | 1u << 14 | 2u << 29;
+constexpr uint32_t kDescKeys = 1u << 16, kDescValues = (16384u >> 4) << 16;
+UOCR_DEV uint32_t desc_lo(uint32_t addr, uint32_t kind) { return ((addr >> 4) & 0x3FFFu) | kind; }
+// M 128, N 128; fp16 or bf16 operands; B from keys (K-major) or values (MN-major: bit 16)
 template <bool kF32>
 constexpr uint32_t idesc(bool mn) {
-    return (1u << 4) | (kF32 ? 0u : (1u << 7) | (1u << 10)) | (mn ? 1u << 16 : 0u) | (64u >> 3) << 17 | (128u >> 4) << 24;
+    return (1u << 4) | (kF32 ? 0u : (1u << 7) | (1u << 10)) | (mn ? 1u << 16 : 0u) | (128u >> 3) << 17 | (128u >> 4) << 24;
 }
 
 template <int N>
@@ -280,320 +297,268 @@ UOCR_DEV void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
 UOCR_DEV float scale_up(uint32_t bits) { return __uint_as_float((268u - max(bits >> 23, 15u)) << 23); }
 UOCR_DEV float scale_down(uint32_t bits) { return __uint_as_float((max(bits >> 23, 15u) - 14u) << 23); }
 
-UOCR_DEV uint4 ldg_stream(const void* p) { return ldg_nc_v4(p); }
-
 // ---- loading warps ----------------------------------------------------------------------------
-// The granules of a segment in the order in which the tensor core takes them: K(0), K(1), V(0), K(2),
-// V(1), ..., each as two halves (64 rows of k; 64 columns of v).
-struct Granules {
-    Walk w;
-    int jj, half;
+// Operands in the order in which the tensor core takes them, over a segment: K(0), K(1), V(0), K(2), V(1), ...,
+// V(n - 1). A warp takes a run of rows of each, a word (16 bytes of a thread) being one row of fp32 or two of bf16.
+template <bool kF32>
+struct Rows {
+    static constexpr int kElt = kF32 ? 4 : 2;
+    static constexpr int kPer = kF32 ? 1 : 2;      // rows of a word
+    static constexpr int kWords = kF32 ? 19 : 10;  // words of a thread
+    static constexpr int kRun = kWords * kPer;     // rows of a warp (the last one has fewer)
+    static_assert(kRun * kLoadWarps >= kPageRows && kRun <= 32, "the warps cover a page");
+};
+
+// One operand to load: where this thread's words lie.
+struct Op {
+    char* pool;          // its first word in the pool's page
+    const char* fresh;   // and where it lies among the new rows (rows from `cached` on are read there)
+    long long fresh_step;
+    int cached, known;   // page rows [0, cached) are in the pool, [cached, known) new, the others not there
+    int own0, own1;      // new rows that this tile stores: those whose first query head lies in it
+    uint32_t unit;
+    bool v;
+};
+
+struct Ops {
+    Walk& w;
+    int jj;
     bool v, more;
     uint32_t unit0;  // units in front of the segment
+    uint32_t id;     // the operand's page id, read one operand ahead of its rows
+    UOCR_DEV int page() const { return w.t.page(w.j + (v ? jj - 1 : jj)); }
+    UOCR_DEV void fetch(const ChunkArgs& a) { id = __ldg(a.lut + (size_t)w.b * a.lut_cols + page()); }
     UOCR_DEV void begin(const ChunkArgs& a, const Shared& s, int g) {
-        more = w.begin(a, s, g);
-        jj = half = 0, v = false, unit0 = 0;
+        more = w.begin(a, s.run, g);
+        __syncwarp();
+        jj = 0, v = false, unit0 = 0;
+        if (more) fetch(a);
     }
     UOCR_DEV void next(const ChunkArgs& a, int g) {
-        if (half == 0) {
-            half = 1;
-            return;
-        }
-        half = 0;
         if (!v && jj >= 1) {
             v = true;
-            return;
+        } else {
+            ++jj;
+            v = jj >= w.n;
+            if (jj > w.n) {
+                unit0 += w.n;
+                __syncwarp();
+                more = w.next(a, g);
+                __syncwarp();
+                jj = 0, v = false;
+            }
         }
-        ++jj;
-        v = jj >= w.n;
-        if (jj > w.n) {
-            unit0 += w.n;
-            more = w.next(a, g);
-            jj = 0, v = false;
-        }
+        if (more) fetch(a);
     }
-};
-
-// What a loaded granule needs when it is turned into an operand.
-struct Loaded {
-    char* store;    // the page's row 0 of this head (this half) in the pool, for the new rows to store
-    uint32_t bits;  // first page row to store, rows to store (8 bits each), half, v, unit & 7
-    UOCR_DEV void set(uint32_t unit, int half, bool v, int row0, int own) {
-        bits = (uint32_t)row0 | (uint32_t)own << 8 | (uint32_t)half << 16 | (uint32_t)v << 17 | (unit & 7) << 18;
-    }
-    UOCR_DEV int row0() const { return bits & 255; }
-    UOCR_DEV int own() const { return bits >> 8 & 255; }
-    UOCR_DEV int half() const { return bits >> 16 & 1; }
-    UOCR_DEV bool v() const { return bits >> 17 & 1; }
-    UOCR_DEV uint32_t unit() const { return bits >> 18 & 7; }
-};
-
-// fp32: a thread holds 8 x 16 bytes: 4 dimensions of 8 rows of k, or 4 columns of 8 rows of v.
-// bf16: 4 x 16 bytes: 8 dimensions of 4 rows.
-template <bool kF32>
-struct Lanes {
-    static constexpr int kWords = kF32 ? 8 : 4;
-    static constexpr int kElt = kF32 ? 4 : 2;
-    // page row of word i, and the byte of the row's 128 (k) or 64 (v) elements
-    static UOCR_DEV int row(bool v, int half, int i, int wc, int lane) {
-        if (kF32) return v ? wc * 16 + 2 * i + (lane >> 4) : half * 64 + wc * 8 + i;
-        return v ? wc * 16 + 4 * i + (lane >> 3) : half * 64 + wc * 8 + 2 * i + (lane >> 4);
-    }
-    static UOCR_DEV int byte(bool v, int lane) {
-        if (kF32) return (v ? lane & 15 : lane) * 16;
-        return (v ? lane & 7 : lane & 15) * 16;
+    template <bool kF32>
+    UOCR_DEV Op op(const ChunkArgs& a, int g, int row0, int byte) const {
+        using R = Rows<kF32>;
+        const size_t row_bytes = (size_t)a.kv_heads * (kDim * R::kElt);
+        const int column = w.head * (kDim * R::kElt) + byte, r0 = page() * kPageRows;
+        const long long ld = (v ? a.v_ld : a.k_ld) * R::kElt;
+        Op o;
+        o.pool = static_cast<char*>(a.pool) +
+                 ((((size_t)min(id, (uint32_t)(a.pages - 1)) * 2 + v) * a.layers + a.layer) * kPageRows + row0) * row_bytes + column;
+        o.cached = w.r.start - r0;
+        o.fresh = static_cast<const char*>(v ? a.v : a.k) + (w.r.lo + row0 - o.cached) * ld + column;
+        o.fresh_step = ld * R::kPer;
+        o.known = min(kPageRows, w.t.last_pos + 1 - r0);
+        const bool stored = id < (uint32_t)a.pages;
+        o.own0 = w.r.start + (w.qt * kTile + g - 1) / g - r0;
+        o.own1 = stored ? w.r.start + min(w.r.n, (w.qt * kTile + kTile + g - 1) / g) - r0 : o.own0;
+        o.unit = unit0 + (v ? jj - 1 : jj), o.v = v;
+        return o;
     }
 };
 
 template <bool kF32>
-UOCR_DEV void load_granule(const ChunkArgs& a, const Granules& gr, int g, int wc, int lane,
-                           uint4 (&x)[Lanes<kF32>::kWords], Loaded& info) {
-    using L = Lanes<kF32>;
-    const Walk& w = gr.w;
-    const int j = gr.v ? gr.jj - 1 : gr.jj, t = w.t.page(w.j + j);
-    const size_t row_bytes = (size_t)a.kv_heads * kDim * L::kElt;
-    const size_t column = (size_t)w.head * kDim * L::kElt + (gr.v ? gr.half * 64 * L::kElt : 0);
-    const uint32_t id = t < a.lut_cols ? __ldg(a.lut + (size_t)w.b * a.lut_cols + t) : 0xFFFFFFFFu;
-    char* page = static_cast<char*>(a.pool) +
-                 (((size_t)min(id, (uint32_t)(a.pages - 1)) * 2 + (gr.v ? 1 : 0)) * a.layers + a.layer) * (kPageRows * row_bytes) +
-                 column;
-    const char* fresh = static_cast<const char*>(gr.v ? a.v : a.k) + column;
-    const size_t fresh_ld = (size_t)(gr.v ? a.v_ld : a.k_ld) * L::kElt;
-    const int r0 = t * kPageRows;
-#pragma unroll
-    for (int i = 0; i < L::kWords; ++i) {
-        const int row = L::row(gr.v, gr.half, i, wc, lane), r = r0 + row;
-        const char* p = r >= w.r.start ? fresh + (size_t)(w.r.lo + r - w.r.start) * fresh_ld : page + (size_t)row * row_bytes;
-        x[i] = r <= w.t.last_pos ? ldg_stream(p + L::byte(gr.v, lane)) : make_uint4(0, 0, 0, 0);
-    }
-    // This tile stores the new rows whose first query head lies in it: every new row is of one tile.
-    const int i0 = (w.qt * kTile + g - 1) / g, i1 = min(w.r.n, (w.qt * kTile + kTile + g - 1) / g);
-    const int s0 = min(max(w.r.start + i0 - r0, 0), kPageRows), s1 = min(w.r.start + i1 - r0, kPageRows);
-    info.store = page;
-    info.set(gr.unit0 + j, gr.half, gr.v, s0, id < (uint32_t)a.pages ? max(s1 - s0, 0) : 0);
+UOCR_DEV uint4 load_word(const ChunkArgs& a, const Op& o, int row0, int i) {
+    using R = Rows<kF32>;
+    const int row = row0 + i * R::kPer;
+    if (row >= o.known) return make_uint4(0, 0, 0, 0);
+    return ldg_nc_v4(row < o.cached ? o.pool + (size_t)i * (a.kv_heads * (kDim * R::kElt * R::kPer))
+                                    : o.fresh + i * o.fresh_step);
 }
 
-template <bool kF32>
-UOCR_DEV void convert_granule(const ChunkArgs& a, Shared& s, unsigned char* stage, int wc, int lane,
-                              uint4 (&x)[Lanes<kF32>::kWords], const Loaded& info) {
-    using L = Lanes<kF32>;
-    const size_t row_bytes = (size_t)a.kv_heads * kDim * L::kElt;
-    const int half = info.half();
-    const bool is_v = info.v();
-    if (info.own() > 0) {
-#pragma unroll
-        for (int i = 0; i < L::kWords; ++i) {
-            const int row = L::row(is_v, half, i, wc, lane);
-            if ((unsigned)(row - info.row0()) < (unsigned)info.own())
-                *reinterpret_cast<uint4*>(info.store + (size_t)row * row_bytes + L::byte(is_v, lane)) = x[i];
-        }
-    }
-    const uint32_t ub = info.unit();
-    if constexpr (kF32) {
-        uint32_t top = 0;
-        auto largest = [&] {
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                m = max(m, max(x[i].x & 0x7FFFFFFFu, x[i].y & 0x7FFFFFFFu));
-                m = max(m, max(x[i].z & 0x7FFFFFFFu, x[i].w & 0x7FFFFFFFu));
-            }
-            return __reduce_max_sync(0xffffffffu, m);
-        };
-        top = largest();
-        uint32_t bad = 0;  // v rows of this warp with values that are not finite
-        if (top >= 0x7F800000u) {
-            // rare: v loses these values here (the softmax warps add them to the rows that see them);
-            // a key keeps them (its scores become NaN), but they set no scale
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                uint32_t* e = &x[i].x;
-                bool row_bad = false;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const bool inf = (e[c] & 0x7F800000u) == 0x7F800000u;
-                    row_bad |= inf;
-                    if (inf && is_v) e[c] = 0;
-                    else if (inf) e[c] = 0x7FFFFFFFu;
-                    else m = max(m, e[c] & 0x7FFFFFFFu);
-                }
-                const uint32_t who = __ballot_sync(0xffffffffu, row_bad);
-                if (who & 0x0000FFFFu) bad |= 1u << (2 * i);
-                if (who & 0xFFFF0000u) bad |= 2u << (2 * i);
-            }
-            top = __reduce_max_sync(0xffffffffu, m);
-        }
-        if (is_v) {
-            // one scale for the granule: the rows are summed over
-            if (lane == 0) {
-                s.vmax[half][wc] = __uint_as_float(top);
-                s.vbad[ub][half][wc] = (uint16_t)bad;
-            }
-            named_bar_sync(kLoadBar, 32 * kLoadWarps);
-            top = __reduce_max_sync(0xffffffffu, __float_as_uint(s.vmax[half][lane & 7]));
-            if (wc == 0 && lane == 0) s.vscale[ub][half] = scale_down(top);
-        } else if (lane == 0) {
-            s.kscale[ub][half * 8 + wc] = scale_down(top);
-        }
-        const float up = scale_up(top);
-        const uint32_t base = smem_addr(stage);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float f0 = __uint_as_float(x[i].x) * up, f1 = __uint_as_float(x[i].y) * up;
-            const float f2 = __uint_as_float(x[i].z) * up, f3 = __uint_as_float(x[i].w) * up;
-            uint2 hi, lo;
-            split2(f0, f1, hi.x, lo.x);
-            split2(f2, f3, hi.y, lo.y);
-            // 8 bytes (4 elements) of a 128-byte operand row, its 16-byte chunks swizzled by the row
-            int row = L::row(is_v, half, i, wc, lane);
-            const int c8 = lane & 15;  // 8-byte word of the 64-element row
-            uint32_t at;
-            if (is_v) at = row * 128;
-            else row &= 63, at = (lane >> 4) * 8192 + row * 128;
-            at += (((c8 >> 1) ^ (row & 7)) << 4) + (c8 & 1) * 8;
-            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(base + at), "r"(hi.x), "r"(hi.y) : "memory");
-            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(base + 16384 + at), "r"(lo.x), "r"(lo.y) : "memory");
-        }
-    } else {
-        if (is_v) {
-            uint32_t any = 0;
-            auto odd = [](uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; };
-#pragma unroll
-            for (int i = 0; i < 4; ++i) any |= odd(x[i].x) | odd(x[i].y) | odd(x[i].z) | odd(x[i].w);
-            uint32_t bad = 0;
-            if (__any_sync(0xffffffffu, any != 0)) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t* e = &x[i].x;
-                    uint32_t row_bad = 0;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const uint32_t o = odd(e[c]);
-                        row_bad |= o;
-                        if (o & 0x00008000u) e[c] &= 0xFFFF0000u;
-                        if (o & 0x80000000u) e[c] &= 0x0000FFFFu;
-                    }
-                    const uint32_t who = __ballot_sync(0xffffffffu, row_bad != 0);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (who >> (8 * q) & 0xFFu) bad |= 1u << (4 * i + q);
-                }
-            }
-            if (lane == 0) s.vbad[ub][half][wc] = (uint16_t)bad;
-        }
-        const uint32_t base = smem_addr(stage);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            int row = L::row(is_v, half, i, wc, lane);
-            uint32_t at;
-            if (is_v) at = row * 128;
-            else row &= 63, at = ((lane >> 3) & 1) * 8192 + row * 128;
-            at += ((lane & 7) ^ (row & 7)) << 4;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(base + at), "r"(x[i].x), "r"(x[i].y), "r"(x[i].z),
-                         "r"(x[i].w)
-                         : "memory");
-        }
-    }
+UOCR_DEV bool odd_f32(uint32_t e) { return (e & 0x7F800000u) == 0x7F800000u; }
+UOCR_DEV uint32_t odd_bf16(uint32_t e) { return ((e & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }  // per half, its top bit
+UOCR_DEV uint32_t top_of(const uint4& x) {
+    return max(max(x.x & 0x7FFFFFFFu, x.y & 0x7FFFFFFFu), max(x.z & 0x7FFFFFFFu, x.w & 0x7FFFFFFFu));
 }
 
 template <bool kF32>
 __device__ void load_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int g) {
-    constexpr int kBytes = kF32 ? 32768 : 16384;
+    using R = Rows<kF32>;
     const int wc = (threadIdx.x >> 5) - kTeamWarps, lane = threadIdx.x & 31;
-    Granules gr;
-    gr.begin(a, s, g);
-    if (!gr.more) return;
-    uint4 x[2][Lanes<kF32>::kWords];
-    Loaded info[2];
-    load_granule<kF32>(a, gr, g, wc, lane, x[0], info[0]);
-    bool have = true;
+    const int row0 = wc * R::kRun + (kF32 ? 0 : lane >> 4), byte = (kF32 ? lane : lane & 15) * 16;
+    Ops ops{s.walk[kTeamWarps + wc]};
+    ops.begin(a, s, g);
+    if (!ops.more) return;
+    // an operand's words: as each is turned into its halves, its register takes the next operand's word
+    uint4 x[R::kWords];
+    Op now = ops.template op<kF32>(a, g, row0, byte);
+#pragma unroll
+    for (int i = 0; i < R::kWords; ++i) x[i] = load_word<kF32>(a, now, row0, i);
     uint32_t stage = 0, phase = 0;
-    auto step = [&](int now, int ahead) {
-        gr.next(a, g);
-        const bool more = gr.more;
-        if (more) load_granule<kF32>(a, gr, g, wc, lane, x[ahead], info[ahead]);
-        if (!wait(s, &s.empty[stage], phase ^ 1)) return false;
-        convert_granule<kF32>(a, s, ring + stage * kBytes, wc, lane, x[now], info[now]);
+    for (;;) {
+        ops.next(a, g);
+        const bool more = ops.more;
+        Op ahead = now;
+        if (more) ahead = ops.template op<kF32>(a, g, row0, byte);
+        else ahead.known = 0;
+        if (now.own0 < kPageRows && now.own1 > now.own0) {
+#pragma unroll
+            for (int i = 0; i < R::kWords; ++i) {
+                const int row = row0 + i * R::kPer;
+                if (row >= now.own0 && row < min(now.own1, kPageRows))
+                    *reinterpret_cast<uint4*>(now.pool + (size_t)i * (a.kv_heads * (kDim * R::kElt * R::kPer))) = x[i];
+            }
+        }
+        const uint32_t ub = now.unit & 7;
+        float up = 1.f;
+        if (now.v) {
+            // values that are not finite leave the operand; fp32: one scale for the page, whose rows are summed over
+            uint32_t top = 0, bad = 0;
+#pragma unroll
+            for (int i = 0; i < R::kWords; ++i)
+                top = kF32 ? max(top, top_of(x[i])) : top | odd_bf16(x[i].x) | odd_bf16(x[i].y) | odd_bf16(x[i].z) | odd_bf16(x[i].w);
+            if (kF32) top = __reduce_max_sync(0xffffffffu, top);
+            if (kF32 ? top >= 0x7F800000u : __any_sync(0xffffffffu, top != 0)) {  // rare
+                top = 0;
+#pragma unroll
+                for (int i = 0; i < R::kWords; ++i) {
+                    bool row_bad = false;
+                    auto drop = [&](uint32_t& e) {
+                        if (kF32) {
+                            if (odd_f32(e)) e = 0, row_bad = true;
+                        } else {
+                            const uint32_t o = odd_bf16(e);
+                            if (o & 0x00008000u) e &= 0xFFFF0000u;
+                            if (o & 0x80000000u) e &= 0x0000FFFFu;
+                            row_bad |= o != 0;
+                        }
+                    };
+                    drop(x[i].x), drop(x[i].y), drop(x[i].z), drop(x[i].w);
+                    const uint32_t who = __ballot_sync(0xffffffffu, row_bad);
+                    if (kF32) bad |= (who ? 1u : 0u) << i;
+                    else bad |= ((who & 0xFFFFu ? 1u : 0u) | (who >> 16 ? 2u : 0u)) << (2 * i);
+                    if (kF32) top = max(top, top_of(x[i]));
+                }
+                if (kF32) top = __reduce_max_sync(0xffffffffu, top);
+            }
+            if (lane == 0) s.vbad[ub][wc] = bad;
+            if constexpr (kF32) {
+                if (lane == 0) s.vmax[now.unit & 1][wc] = __uint_as_float(top);
+                named_bar_sync(kLoadBar, 32 * kLoadWarps);
+                top = __reduce_max_sync(0xffffffffu, __float_as_uint(s.vmax[now.unit & 1][lane % kLoadWarps]));
+                if (wc == 0 && lane == 0) s.vscale[ub] = scale_down(top);
+                up = scale_up(top);
+            }
+        }
+        if (!wait(s, &s.empty[stage], phase ^ 1)) return;
+        const uint32_t base = smem_addr(ring) + stage * kStageBytes<kF32>;
+        uint32_t my_top = 0;  // lane i: the largest magnitude of row i of k
+#pragma unroll
+        for (int i = 0; i < R::kWords; ++i) {
+            const int row = row0 + i * R::kPer;
+            if constexpr (kF32) {
+                if (!now.v) {
+                    uint32_t top = __reduce_max_sync(0xffffffffu, top_of(x[i]));
+                    if (top >= 0x7F800000u) {  // rare: its scores become NaN; it sets no scale
+                        uint32_t m = 0;
+                        auto mark = [&](uint32_t& e) {
+                            if (odd_f32(e)) e = 0x7FFFFFFFu;
+                            else m = max(m, e & 0x7FFFFFFFu);
+                        };
+                        mark(x[i].x), mark(x[i].y), mark(x[i].z), mark(x[i].w);
+                        top = __reduce_max_sync(0xffffffffu, m);
+                    }
+                    if (lane == i) my_top = top;
+                    up = scale_up(top);
+                }
+                uint2 hi, lo;
+                split2(__uint_as_float(x[i].x) * up, __uint_as_float(x[i].y) * up, hi.x, lo.x);
+                split2(__uint_as_float(x[i].z) * up, __uint_as_float(x[i].w) * up, hi.y, lo.y);
+                x[i] = load_word<kF32>(a, ahead, row0, i);
+                // 8 bytes (4 columns) of a block's 128-byte row, whose 16-byte chunks are swizzled by the row
+                const uint32_t at = base + (lane >> 4) * 16384 + row * 128 + ((((lane & 15) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
+                if (row < kPageRows) {
+                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(hi.x), "r"(hi.y) : "memory");
+                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + 32768), "r"(lo.x), "r"(lo.y) : "memory");
+                }
+            } else {
+                const uint32_t at = base + ((lane >> 3) & 1) * 16384 + row * 128 + (((lane & 7) ^ (row & 7)) << 4);
+                if (row < kPageRows)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[i].x), "r"(x[i].y), "r"(x[i].z),
+                                 "r"(x[i].w)
+                                 : "memory");
+                x[i] = load_word<kF32>(a, ahead, row0, i);
+            }
+        }
+        if (kF32 && !now.v && lane < R::kRun && wc * R::kRun + lane < kPageRows)
+            s.kscale[ub][wc * R::kRun + lane] = scale_down(my_top);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.full[stage]);
-        if (++stage == kStages) stage = 0, phase ^= 1;
-        have = more;
-        return true;
-    };
-    while (have) {
-        if (!step(0, 1)) return;
-        if (!have) break;
-        if (!step(1, 0)) return;
+        if (++stage == kStages<kF32>) stage = 0, phase ^= 1;
+        if (!more) return;
+        now = ahead;
     }
 }
 
 // ---- the issuing warp -------------------------------------------------------------------------
 template <bool kF32>
 __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int g) {
-    constexpr int kBytes = kF32 ? 32768 : 16384;
-    const int lane = threadIdx.x & 31;
     const uint32_t tmem = s.tmem, base = smem_addr(ring);
     uint32_t stage = 0, phase = 0, unit0 = 0, seg = 0;
-    Walk w;
-    // a finished granule: its MMAs issued, its stage given back
-    auto granule = [&](auto&& issue) {
+    Walk& w = s.walk[kTeamWarps + kLoadWarps];
+    // one operand: its MMAs issued (D = sum over the products of A's halves and the operand's, 16 of the summed
+    // dimension at a time), its stage given back, the result announced
+    auto product = [&](uint32_t d, uint32_t ta, uint32_t a_step, uint32_t a_lo, uint32_t kind, uint32_t b_step2, uint32_t b_step8,
+                       uint32_t id, uint64_t* done) {
         if (!wait(s, &s.full[stage], phase)) return false;
         tc_fence_after();
-        if (lane == 0) {
-            issue(base + stage * kBytes);
+        if (elect_one()) {
+            const uint32_t b = desc_lo(base + stage * kStageBytes<kF32>, kind);
+#pragma unroll
+            for (int p = kF32 ? 0 : 2; p < 3; ++p) {  // lo x hi, hi x lo, hi x hi
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    umma_ts_f16(d, ta + i * a_step + (p == 0 ? a_lo : 0),
+                                b + (i & 3) * b_step2 + (i >> 2) * b_step8 + (p == 1 ? 32768 >> 4 : 0), kDescHi, id,
+                                p != (kF32 ? 0 : 2) || i != 0);
+            }
             umma_commit(&s.empty[stage]);
+            umma_commit(done);
         }
         __syncwarp();
-        if (++stage == kStages) stage = 0, phase ^= 1;
+        if (++stage == kStages<kF32>) stage = 0, phase ^= 1;
         return true;
     };
     auto run = [&] {
-        for (bool more = w.begin(a, s, g); more; more = w.next(a, g), ++seg) {
+        auto next = [&](bool first) {
+            __syncwarp();
+            const bool more = first ? w.begin(a, s.run, g) : w.next(a, g);
+            __syncwarp();
+            return more;
+        };
+        for (bool more = next(true); more; more = next(false), ++seg) {
             if (!wait(s, &s.q_full, seg & 1)) return;
             tc_fence_after();
             const int n = w.n;
             for (int jj = 0; jj <= n; ++jj) {
-                if (jj < n) {
-                    const uint32_t u = unit0 + jj, d = tmem + kColS + (u & 1) * 128;
-                    for (int half = 0; half < 2; ++half) {
-                        const bool ok = granule([&](uint32_t k) {
-                            const uint32_t dh = d + half * 64, q = tmem + kColQ;
-#pragma unroll
-                            for (int p = kF32 ? 0 : 2; p < 3; ++p) {  // q lo x k hi, q hi x k lo, q hi x k hi
-#pragma unroll
-                                for (int i = 0; i < 8; ++i)
-                                    umma_ts_f16(dh, q + (p == 0 ? 64 : 0) + i * 8,
-                                                umma_desc_sw128(k + (p == 1 ? 16384 : 0) + (i >> 2) * 8192 + (i & 3) * 32),
-                                                idesc<kF32>(false), p != (kF32 ? 0 : 2) || i != 0);
-                            }
-                        });
-                        if (!ok) return;
-                    }
-                    if (lane == 0) umma_commit(&s.s_full[u & 1]);
-                    __syncwarp();
+                if (jj < n) {  // S = Q K^T: 16 dimensions of K are 32 bytes of a row, 64 a block
+                    const uint32_t u = unit0 + jj;
+                    if (!product(tmem + kColS + (u & 1) * 128, tmem + kColQ, 8, 64, kDescKeys, 32 >> 4, 16384 >> 4,
+                                 idesc<kF32>(false), &s.s_full[u & 1]))
+                        return;
                 }
-                if (jj >= 1) {
-                    const uint32_t u = unit0 + jj - 1, pa = tmem + kColS + (u & 1) * 128;
+                if (jj >= 1) {  // P V: 16 rows of V are 2048 bytes of both its blocks
+                    const uint32_t u = unit0 + jj - 1;
                     if (!wait(s, &s.p_full[u & 1], (u >> 1) & 1) || !wait(s, &s.pv_free, (u & 1) ^ 1)) return;
-                    tc_fence_after();
-                    for (int half = 0; half < 2; ++half) {
-                        const bool ok = granule([&](uint32_t v) {
-                            const uint32_t dh = tmem + kColPv + half * 64;
-#pragma unroll
-                            for (int p = kF32 ? 0 : 2; p < 3; ++p) {  // p lo x v hi, p hi x v lo, p hi x v hi
-#pragma unroll
-                                for (int i = 0; i < 8; ++i)
-                                    umma_ts_f16(dh, pa + i * 16 + (p == 0 ? 8 : 0),
-                                                desc_mn_sw128(v + (p == 1 ? 16384 : 0) + i * 2048), idesc<kF32>(true),
-                                                p != (kF32 ? 0 : 2) || i != 0);
-                            }
-                        });
-                        if (!ok) return;
-                    }
-                    if (lane == 0) umma_commit(&s.pv_full);
-                    __syncwarp();
+                    if (!product(tmem + kColPv, tmem + kColS + (u & 1) * 128, 16, 8, kDescValues, 2048 >> 4, 8192 >> 4,
+                                 idesc<kF32>(true), &s.pv_full))
+                        return;
                 }
             }
             unit0 += n;
@@ -601,7 +566,7 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
     };
     run();
     // every MMA of this CTA has finished before its TMEM is freed
-    if (lane == 0) umma_commit(&s.drain);
+    if (elect_one()) umma_commit(&s.drain);
     __syncwarp();
     mbar_wait_warp(&s.drain, 0, nullptr, nullptr);
 }
@@ -614,7 +579,7 @@ __device__ __noinline__ void add_bad_values(const ChunkArgs& a, const Walk& w, i
     // value row `row` of page t: what is not finite of this half's 64 columns, into out64 (else 0)
     const int r = t * kPageRows + row;
     const size_t elt = kF32 ? 4 : 2;
-    const uint32_t id = t < a.lut_cols ? __ldg(a.lut + (size_t)w.b * a.lut_cols + t) : 0xFFFFFFFFu;
+    const uint32_t id = __ldg(a.lut + (size_t)w.b * a.lut_cols + t);
     const size_t row_elts = (size_t)a.kv_heads * kDim;
     const char* p = r >= w.r.start
                         ? static_cast<const char*>(a.v) + ((size_t)(w.r.lo + r - w.r.start) * a.v_ld + w.head * kDim) * elt
@@ -707,7 +672,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
         if (alive && !wait(s, &s.pv_full, u & 1)) alive = false;
         if (alive && live) {
             tc_fence_after();
-            const float f = kF32 ? s.vscale[u & 7][half] : 1.f;
+            const float f = kF32 ? s.vscale[u & 7] : 1.f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t x[16];
@@ -716,12 +681,10 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fmaf(acc[c * 16 + i], alpha, __uint_as_float(x[i]) * f);
             }
-            uint32_t bad = 0;
-            const uint4* vb = reinterpret_cast<const uint4*>(s.vbad[u & 7][half]);  // 8 x 16 rows
-            bad = vb->x | vb->y | vb->z | vb->w;
-            if (bad) {
-                for (int q = 0; q < 128; ++q) {
-                    if (!(s.vbad[u & 7][half][q >> 4] >> (q & 15) & 1)) continue;
+            const uint4* vb = reinterpret_cast<const uint4*>(s.vbad[u & 7]);
+            if (vb[0].x | vb[0].y | vb[0].z | vb[0].w | vb[1].x | vb[1].y | vb[1].z) {
+                for (int q = 0; q < kPageRows; ++q) {
+                    if (!(s.vbad[u & 7][q / Rows<kF32>::kRun] >> (q % Rows<kF32>::kRun) & 1)) continue;
                     const int r = t * kPageRows + q;
                     const bool seen = r <= pos && (a.window <= 0 || r > pos - a.window || r < w.r.prefix);
                     float extra[64];
@@ -737,8 +700,10 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
         if (lane == 0) mbar_arrive(&s.pv_free);
     };
 
-    Walk w;
-    bool more = w.begin(a, s, g);
+    Walk& w = s.walk[warp];
+    Walk& done = s.done[warp];
+    bool more = w.begin(a, s.run, g);
+    __syncwarp();
     int state[2] = {0, 0}, place[4] = {0, 0, 0, 0};
     uint32_t unit0 = 0;
     if (more) load_query(w);
@@ -765,8 +730,8 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
 #pragma unroll
                 for (int c = 0; c < 2; ++c) mask[c] = seen_mask(half * 64 + c * 32, pos - c0, lo, w.r.prefix - c0);
             }
-            // 1 / (scale of 8 columns' keys) x the query's: read where it is used
-            auto f = [&](int i) { return kF32 ? s.kscale[u & 7][half * 8 + i] * qscale : qscale; };
+            // 1 / scale of a column's keys
+            const float* ks = &s.kscale[u & 7][half * 64];
             float top = -INFINITY;
             if (alive && live) {
 #pragma unroll
@@ -780,14 +745,14 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
                             if (!(mask[c >> 1] >> ((c & 1) * 16 + i) & 1)) x[i] = 0xFF800000u;
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; i += 8) {
-                        float t8 = __uint_as_float(x[i]);
-#pragma unroll
-                        for (int e = 1; e < 8; ++e) t8 = fmaxf(t8, __uint_as_float(x[i + e]));
-                        top = fmaxf(top, t8 == -INFINITY ? t8 : t8 * f(c * 2 + i / 8));
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 k4 = kF32 ? *reinterpret_cast<const float4*>(ks + c * 16 + i) : make_float4(1.f, 1.f, 1.f, 1.f);
+                        top = fmaxf(fmaxf(top, __uint_as_float(x[i]) * k4.x), __uint_as_float(x[i + 1]) * k4.y);
+                        top = fmaxf(fmaxf(top, __uint_as_float(x[i + 2]) * k4.z), __uint_as_float(x[i + 3]) * k4.w);
                     }
                 }
             }
+            top *= qscale;  // -inf * 0 (nothing seen, a query of zeros): NaN, which is no maximum
             s.xmax[buf][half][row] = top;
             named_bar_sync(kTeamBar, 32 * kTeamWarps);
             top = fmaxf(top, s.xmax[buf][half ^ 1][row]);
@@ -803,10 +768,16 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
                     tmem_ld_32x32b_x16(sa + c * 16, x);
                     tmem_wait_ld16(x);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float y = fmaf(__uint_as_float(x[i]), f(c * 2 + i / 8), -shift);
-                        if (!all && !(mask[c >> 1] >> ((c & 1) * 16 + i) & 1)) y = -INFINITY;
-                        x[i] = __float_as_uint(exp2_fast(y));
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 k4 = kF32 ? *reinterpret_cast<const float4*>(ks + c * 16 + i) : make_float4(1.f, 1.f, 1.f, 1.f);
+                        const float kk[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float y = __uint_as_float(x[i + e]);
+                            y = fmaf(kF32 ? y * kk[e] : y, qscale, -shift);
+                            if (!all && !(mask[c >> 1] >> ((c & 1) * 16 + i + e) & 1)) y = -INFINITY;
+                            x[i + e] = __float_as_uint(exp2_fast(y));
+                        }
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sum += __uint_as_float(x[i]);
@@ -830,10 +801,12 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
             if (j > 0) add_pv(w, u - 1, w.t.page(w.j + j - 1), live, pos);
             alpha = alpha_next;
         }
-        const Walk done = w;
         const uint32_t last = unit0 + w.n - 1;
         unit0 += w.n;
+        done = w;
+        __syncwarp();
         more = w.next(a, g);
+        __syncwarp();
         if (more) load_query(w);  // every score of the finished segment has been read: its query is free
         add_pv(done, last, done.t.page(done.j + done.n - 1), live, pos);
         s.xsum[half][row] = l;
@@ -893,20 +866,26 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs 
     const int warp = threadIdx.x >> 5;
     const int g = a.heads / a.kv_heads;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) mbar_init(&s.full[i], kLoadWarps), mbar_init(&s.empty[i], 1);
+        for (int i = 0; i < kMaxStages; ++i) mbar_init(&s.full[i], kLoadWarps), mbar_init(&s.empty[i], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&s.s_full[i], 1), mbar_init(&s.p_full[i], kTeamWarps);
         mbar_init(&s.pv_full, 1), mbar_init(&s.pv_free, kTeamWarps), mbar_init(&s.q_full, kTeamWarps), mbar_init(&s.drain, 1);
         fence_mbar_init();
         s.abort = 0;
+        for (int i = 0; i < 8; ++i) s.vbad[i][7] = 0;
     }
     if (warp == kTeamWarps + kLoadWarps) tmem_alloc(&s.tmem, 512);
     tc_fence_before();
     find_run(a, s, reinterpret_cast<long long*>(ring), g);
     tc_fence_after();
     pdl_launch_dependents();
-    if (warp < kTeamWarps) team_role<kF32>(a, s, slots, info, g);
-    else if (warp < kTeamWarps + kLoadWarps) load_role<kF32>(a, s, ring, g);
-    else mma_role<kF32>(a, s, ring, g);
+    if (warp < kTeamWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTeamRegs));
+        team_role<kF32>(a, s, slots, info, g);
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
+        if (warp < kTeamWarps + kLoadWarps) load_role<kF32>(a, s, ring, g);
+        else mma_role<kF32>(a, s, ring, g);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -957,7 +936,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a, const floa
 
 template <bool kF32>
 cudaError_t launch(const ChunkArgs& a, void* ws, int sms, cudaStream_t st) {
-    const size_t smem = (size_t)kStages * (kF32 ? 32768 : 16384) + 1024;
+    const size_t smem = (size_t)kStages<kF32> * kStageBytes<kF32> + 1024;
     auto kernel = chunk_attention_kernel<kF32>;
     cudaError_t err = ensure_smem_optin(reinterpret_cast<const void*>(kernel), smem);
     if (err != cudaSuccess) return err;
