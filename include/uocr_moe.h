@@ -141,13 +141,14 @@ UOCR_API int uocr_paged_decode_attention(const float* q, const float* k_new, con
  * p = start[b] + i, stored at row p % 128 of page lut[b * lut_cols + p / 128], and attends the logical
  * rows r <= p, all of them (window 0) or those with r > p - window or r < prefix[b] (window >= 1; prefix
  * null: 0). Rows below start[b] are read from the pool (page ids past the pool read its last page), the
- * new rows from k_new and v_new; new rows beyond the lookup table or with a page id past the pool are
- * attended but not stored. Rows of out in no request are left as they were. What a row does not see
+ * new rows from k_new and v_new; new rows with a page id past the pool are attended but not stored, new
+ * rows beyond the lookup table are in no request. Rows of out in no request are left as they were. What a row does not see
  * does not reach it, whatever it holds (NaN and infinities included).
- * Sums and softmax in fp32. The workspace (uocr_paged_chunk_workspace_bytes() bytes on the current
- * device, 256-byte aligned, no initial contents) belongs to the call until it has finished. The
+ * Sums and softmax in fp32. The workspace (uocr_paged_chunk_workspace_bytes(...) bytes on the current
+ * device, 0 for sizes that the call refuses; 256-byte aligned, no initial contents) belongs to the call until it has finished. The
  * result is deterministic (a fixed split and order on one kind of GPU). B <= 8192. */
-UOCR_API size_t uocr_paged_chunk_workspace_bytes(void);
+UOCR_API size_t uocr_paged_chunk_workspace_bytes(int64_t T, int64_t heads, int64_t kv_heads, int dtype,
+                               int64_t lut_cols, int64_t B);
 UOCR_API int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, int64_t k_ld, const void* v_new,
                                int64_t v_ld, int64_t T, int64_t heads, int64_t kv_heads, int64_t head_dim, int dtype,
                                void* kv_pool, int64_t pages, int64_t layers, int64_t layer, const uint32_t* lut,

@@ -73,7 +73,7 @@ SIGNATURES: dict[str, tuple] = {
     "uocr_paged_attention_workspace_bytes": (SZ, [I64, I64, I64]),
     "uocr_paged_decode_attention": (I32, [P, P, P, I64, I64, I64, P, I64, I64, I64, P, I64, P, P, ctypes.c_float, P, P,
                                           SZ, P]),
-    "uocr_paged_chunk_workspace_bytes": (SZ, []),
+    "uocr_paged_chunk_workspace_bytes": (SZ, [I64, I64, I64, I32, I64, I64]),
     "uocr_paged_chunk_attention": (I32, [P, I64, P, I64, P, I64, I64, I64, I64, I64, I32, P, I64, I64, I64, P, I64, P, P,
                                          I64, ctypes.c_float, I64, P, P, P, SZ, P]),
     "uocr_copy_pages": (I32, [P, I64, I64, I64, P, P, P, I64, P]),

@@ -310,7 +310,16 @@ int uocr_paged_decode_attention(const float* q, const float* k_new, const float*
                        "paged_decode_attention: launch");
 }
 
-size_t uocr_paged_chunk_workspace_bytes(void) { return uocr::chunk_workspace_bytes(current_sms()); }
+size_t uocr_paged_chunk_workspace_bytes(int64_t T, int64_t heads, int64_t kv_heads, int dtype, int64_t lut_cols, int64_t B) {
+    if (T < 1 || B < 1 || B > uocr::kChunkMaxRequests || heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 1024 ||
+        T > (int64_t(1) << 30) / (heads / kv_heads) || lut_cols < 1 || lut_cols > (1 << 22) ||
+        (dtype != UOCR_DTYPE_F32 && dtype != UOCR_DTYPE_BF16))
+        return 0;
+    uocr::ChunkArgs a{};
+    a.T = (int)T; a.B = (int)B; a.heads = (int)heads; a.kv_heads = (int)kv_heads; a.lut_cols = (int)lut_cols;
+    a.bf16 = dtype == UOCR_DTYPE_BF16;
+    return uocr::chunk_workspace_bytes(a, current_sms());
+}
 
 int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, int64_t k_ld, const void* v_new,
                                int64_t v_ld, int64_t T, int64_t heads, int64_t kv_heads, int64_t head_dim, int dtype,
@@ -348,7 +357,7 @@ int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, i
     if (!(scale == scale) || scale - scale != 0.f)
         return fail(UOCR_EINVAL, "paged_chunk_attention: the scale is not finite");
     if (B == 0 || T == 0) return ok();
-    const size_t need = uocr_paged_chunk_workspace_bytes();
+    const size_t need = uocr_paged_chunk_workspace_bytes(T, heads, kv_heads, dtype, lut_cols, B);
     if (!q || !k_new || !v_new || !kv_pool || !lut || !row_offsets || !start || !out || (need && !workspace))
         return fail(UOCR_EINVAL, "paged_chunk_attention: null pointer");
     if (!a16(q) || !a16(k_new) || !a16(v_new) || !a16(kv_pool) || !a16(out))

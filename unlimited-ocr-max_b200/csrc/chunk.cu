@@ -31,196 +31,54 @@
 // weights are rounded to bf16, as the tensor core takes both operands in one type.
 // Values that are not finite are kept out of the V operand (0 x inf would reach rows that do not see
 // them) and added to the rows that do see them.
-#include <algorithm>
-
-#include "common.cuh"
-#include "kernels.h"
-#include "sm100.cuh"
+#include "chunk.cuh"
 
 namespace uocr {
 namespace {
 
-constexpr int kPageRows = 128;  // rows of a page, and of a unit
-constexpr int kDim = 128;
 constexpr int kTile = 128;      // (token, head) rows of a query tile
-constexpr int kTeamWarps = 8, kLoadWarps = 7;  // with the issuing warp 16: 128 registers a thread
-constexpr int kThreads = 32 * (kTeamWarps + kLoadWarps + 1);
-constexpr int kTeamRegs = 112, kLoadRegs = 144;  // of the launch's 16 warps x 128
-static_assert(kTeamWarps * kTeamRegs + (kLoadWarps + 1) * kLoadRegs <= 16 * 128, "the split draws on the launch's registers");
-// Ring of operands: a page's 128 rows of k or of v, as two blocks of 64 columns [128 rows][128 bytes]; fp32: the
-// lo halves behind the hi halves.
+constexpr int kTeamWarps = 8;   // softmax; then the issuing warp and the copying warp
+constexpr int kThreads = 32 * (kTeamWarps + 2);
+// An operand: a page's 128 rows of k or of v of one head, as two blocks of 64 columns [128 rows][128 bytes]; fp32:
+// the lo halves behind the hi halves.
 template <bool kF32>
-constexpr int kStageBytes = kF32 ? 65536 : 32768;
+constexpr int kOperandBytes = kF32 ? 65536 : 32768;
 template <bool kF32>
-constexpr int kStages = kF32 ? 3 : 6;
+constexpr int kStages = kF32 ? 3 : 6;  // of operands in shared memory
 constexpr int kMaxStages = 6;
-constexpr int kSlotFloats = kTile * (kDim + 2);  // a part: sums [128 columns][128 rows], m [128], l [128]
-constexpr int kInfoInts = 8;    // per CTA: states of its two slots, then the tile's place
-constexpr uint32_t kTeamBar = 1, kLoadBar = 2;
-constexpr float kLog2e = 1.44269504088896341f;
+constexpr uint32_t kTeamBar = 1;
 
 // TMEM columns
 constexpr uint32_t kColS = 0, kColPv = 256, kColQ = 384;
 
-struct Request {
-    int lo, n, start, prefix;
+// Beside a page's operands: 1 / scale of each row of k; of v, and which rows of it are not finite.
+struct alignas(16) ValueMeta {
+    float scale;
+    float pad[3];
+    uint32_t bad[4];
+};
+struct alignas(16) PageMeta {
+    float kscale[kPageRows];
+    ValueMeta v;
 };
 
-UOCR_DEV Request request_at(const ChunkArgs& a, int b) {
-    Request r;
-    r.lo = min(max(__ldg(a.offsets + b), 0), a.T);
-    r.start = min(max(__ldg(a.start + b), 0), a.lut_cols * kPageRows);
-    r.n = max(min(min(__ldg(a.offsets + b + 1), a.T) - r.lo, a.lut_cols * kPageRows - r.start), 0);
-    r.prefix = a.prefix ? max(__ldg(a.prefix + b), 0) : 0;
-    return r;
-}
-
-// A query tile's pages: columns [0, head_pages) and [tail_page, ...) of its lookup row, `count` in all.
-struct Tile {
-    int first_pos, last_pos;  // logical rows of its first and last token
-    int head_pages, tail_page, count;
-    UOCR_DEV int page(int j) const { return j < head_pages ? j : j - head_pages + tail_page; }
-};
-
-UOCR_DEV Tile tile_at(const ChunkArgs& a, const Request& r, int qt, int g) {
-    Tile t;
-    const int r0 = qt * kTile;
-    t.first_pos = r.start + r0 / g;
-    t.last_pos = r.start + min(r.n - 1, (r0 + kTile - 1) / g);
-    t.head_pages = t.tail_page = 0;
-    if (a.window > 0) {
-        t.tail_page = max(0, t.first_pos - a.window + 1) / kPageRows;
-        t.head_pages = min((min(r.prefix, t.last_pos + 1) + kPageRows - 1) / kPageRows, t.tail_page);
-    }
-    t.count = t.head_pages + t.last_pos / kPageRows + 1 - t.tail_page;
-    return t;
-}
-
-// A CTA's run: its units, and where they begin.
-struct Run {
-    int left, b, qt, head, j;
-};
-
-// The walk over a CTA's units, a segment (pages of one tile and head) at a time; every warp walks by
-// itself, with its walk in shared memory (a register per field would spill).
-struct Walk {
-    int b, qt, head, j, n, tiles;  // segment: pages j .. j + n - 1 of the tile's
-    int left;                      // units behind this segment
-    Request r;
-    Tile t;
-    UOCR_DEV void enter(const ChunkArgs& a, int g) {
-        t = tile_at(a, r, qt, g);
-        n = min(t.count - j, left);
-        left -= n;
-    }
-    UOCR_DEV bool begin(const ChunkArgs& a, const Run& s, int g) {
-        left = s.left;
-        if (left <= 0) return false;
-        b = s.b, qt = s.qt, head = s.head, j = s.j;
-        r = request_at(a, b);
-        tiles = (r.n * g + kTile - 1) / kTile;
-        enter(a, g);
-        return true;
-    }
-    UOCR_DEV bool next(const ChunkArgs& a, int g) {
-        if (left <= 0) return false;
-        j = 0;
-        if (++head == a.kv_heads) {
-            head = 0;
-            if (++qt >= tiles) {
-                qt = 0;
-                do {  // left > 0: another request with rows follows
-                    ++b;
-                    r = request_at(a, b);
-                } while (r.n == 0 && b < a.B - 1);
-                tiles = (r.n * g + kTile - 1) / kTile;
-            }
-        }
-        enter(a, g);
-        return true;
-    }
-    UOCR_DEV bool whole() const { return j == 0 && n == t.count; }
+// The operands of a pass, made by the first launch: page `p` of request b and head h (of the pass) at
+// index (b * lut_cols + p) * pass_heads + h: k, then v.
+struct Images {
+    unsigned char* operands;
+    PageMeta* meta;
 };
 
 struct Shared {
+    alignas(16) float kscale[8][kPageRows];  // by unit
+    ValueMeta vmeta[8];
     uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], p_full[2], pv_full, pv_free, q_full, drain;
     uint32_t tmem;
     volatile int abort;
     Run run;
     Walk walk[kThreads / 32], done[kTeamWarps];
-    alignas(16) float kscale[8][kPageRows];  // by unit: 1 / scale of each row of k
-    float vscale[8];                         // by unit: 1 / scale of v
-    alignas(16) uint32_t vbad[8][8];         // by unit: each loading warp's rows of v that are not finite
-    float vmax[2][8];
     float xmax[2][2][kTile], xsum[2][kTile];
 };
-
-template <typename T>
-UOCR_DEV T warp_scan(T v, int lane) {  // inclusive
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        const T u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-    }
-    return v;
-}
-
-// All threads: this CTA's run of units, into s. scratch: B long longs of shared memory.
-__device__ void find_run(const ChunkArgs& a, Shared& s, long long* scratch, int g) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int b = warp; b < a.B; b += kThreads / 32) {
-        const Request r = request_at(a, b);
-        const int tiles = (r.n * g + kTile - 1) / kTile;
-        long long sum = 0;
-        for (int qt = lane; qt < tiles; qt += 32) sum += tile_at(a, r, qt, g).count;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) scratch[b] = sum * a.kv_heads;
-    }
-    __syncthreads();
-    if (warp == 0) {
-        long long total = 0;
-        for (int b = lane; b < a.B; b += 32) total += scratch[b];
-#pragma unroll
-        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        const long long ctas = min((long long)gridDim.x, total);
-        long long u0 = 0, u1 = 0;
-        if ((long long)blockIdx.x < ctas) u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
-        if (lane == 0) s.run.left = (int)(u1 - u0);
-        if (u1 > u0) {
-            int b = 0;
-            long long before = 0;  // units in front of request b
-            for (int b0 = 0; b0 < a.B; b0 += 32) {
-                const long long mine = b0 + lane < a.B ? scratch[b0 + lane] : 0;
-                const long long upto = before + warp_scan(mine, lane);
-                const uint32_t hit = __ballot_sync(0xffffffffu, upto > u0);
-                if (hit) {
-                    const int f = __ffs(hit) - 1;
-                    b = b0 + f;
-                    before = __shfl_sync(0xffffffffu, upto - mine, f);
-                    break;
-                }
-                before = __shfl_sync(0xffffffffu, upto, 31);
-            }
-            const Request r = request_at(a, b);
-            const int tiles = (r.n * g + kTile - 1) / kTile;
-            for (int q0 = 0; q0 < tiles; q0 += 32) {
-                const int count = q0 + lane < tiles ? tile_at(a, r, q0 + lane, g).count : 0;
-                const long long upto = before + warp_scan((long long)count * a.kv_heads, lane);
-                const uint32_t hit = __ballot_sync(0xffffffffu, upto > u0);
-                if (hit) {
-                    if (lane == __ffs(hit) - 1) {
-                        const long long in = u0 - (upto - (long long)count * a.kv_heads);
-                        s.run = Run{s.run.left, b, q0 + lane, (int)(in / count), (int)(in % count)};
-                    }
-                    break;
-                }
-                before = __shfl_sync(0xffffffffu, upto, 31);
-            }
-        }
-    }
-    __syncthreads();
-}
 
 UOCR_DEV bool wait(Shared& s, uint64_t* bar, uint32_t parity) {
     if (mbar_wait_warp(bar, parity, &s.abort, nullptr)) return true;
@@ -271,21 +129,6 @@ UOCR_DEV void tmem_wait_ld16(uint32_t (&r)[16]) {
 }
 UOCR_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-UOCR_DEV uint32_t pack_f16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-UOCR_DEV uint32_t pack_bf16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-UOCR_DEV float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // two values as fp16 halves: hi takes the upper 11 bits (exactly), lo the rest (rounded to 11 bits)
 UOCR_DEV void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
     const float xh = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u), yh = __uint_as_float(__float_as_uint(y) & 0xFFFFE000u);
@@ -297,136 +140,65 @@ UOCR_DEV void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
 UOCR_DEV float scale_up(uint32_t bits) { return __uint_as_float((268u - max(bits >> 23, 15u)) << 23); }
 UOCR_DEV float scale_down(uint32_t bits) { return __uint_as_float((max(bits >> 23, 15u) - 14u) << 23); }
 
-// ---- loading warps ----------------------------------------------------------------------------
-// Operands in the order in which the tensor core takes them, over a segment: K(0), K(1), V(0), K(2), V(1), ...,
-// V(n - 1). A warp takes a run of rows of each, a word (16 bytes of a thread) being one row of fp32 or two of bf16.
-template <bool kF32>
-struct Rows {
-    static constexpr int kElt = kF32 ? 4 : 2;
-    static constexpr int kPer = kF32 ? 1 : 2;      // rows of a word
-    static constexpr int kWords = kF32 ? 19 : 10;  // words of a thread
-    static constexpr int kRun = kWords * kPer;     // rows of a warp (the last one has fewer)
-    static_assert(kRun * kLoadWarps >= kPageRows && kRun <= 32, "the warps cover a page");
-};
-
-// One operand to load: where this thread's words lie.
-struct Op {
-    char* pool;          // its first word in the pool's page
-    const char* fresh;   // and where it lies among the new rows (rows from `cached` on are read there)
-    long long fresh_step;
-    int cached, known;   // page rows [0, cached) are in the pool, [cached, known) new, the others not there
-    int own0, own1;      // new rows that this tile stores: those whose first query head lies in it
-    uint32_t unit;
-    bool v;
-};
-
-struct Ops {
-    Walk& w;
-    int jj;
-    bool v, more;
-    uint32_t unit0;  // units in front of the segment
-    uint32_t id;     // the operand's page id, read one operand ahead of its rows
-    UOCR_DEV int page() const { return w.t.page(w.j + (v ? jj - 1 : jj)); }
-    UOCR_DEV void fetch(const ChunkArgs& a) { id = __ldg(a.lut + (size_t)w.b * a.lut_cols + page()); }
-    UOCR_DEV void begin(const ChunkArgs& a, const Shared& s, int g) {
-        more = w.begin(a, s.run, g);
-        __syncwarp();
-        jj = 0, v = false, unit0 = 0;
-        if (more) fetch(a);
-    }
-    UOCR_DEV void next(const ChunkArgs& a, int g) {
-        if (!v && jj >= 1) {
-            v = true;
-        } else {
-            ++jj;
-            v = jj >= w.n;
-            if (jj > w.n) {
-                unit0 += w.n;
-                __syncwarp();
-                more = w.next(a, g);
-                __syncwarp();
-                jj = 0, v = false;
-            }
-        }
-        if (more) fetch(a);
-    }
-    template <bool kF32>
-    UOCR_DEV Op op(const ChunkArgs& a, int g, int row0, int byte) const {
-        using R = Rows<kF32>;
-        const size_t row_bytes = (size_t)a.kv_heads * (kDim * R::kElt);
-        const int column = w.head * (kDim * R::kElt) + byte, r0 = page() * kPageRows;
-        const long long ld = (v ? a.v_ld : a.k_ld) * R::kElt;
-        Op o;
-        o.pool = static_cast<char*>(a.pool) +
-                 ((((size_t)min(id, (uint32_t)(a.pages - 1)) * 2 + v) * a.layers + a.layer) * kPageRows + row0) * row_bytes + column;
-        o.cached = w.r.start - r0;
-        o.fresh = static_cast<const char*>(v ? a.v : a.k) + (w.r.lo + row0 - o.cached) * ld + column;
-        o.fresh_step = ld * R::kPer;
-        o.known = min(kPageRows, w.t.last_pos + 1 - r0);
-        const bool stored = id < (uint32_t)a.pages;
-        o.own0 = w.r.start + (w.qt * kTile + g - 1) / g - r0;
-        o.own1 = stored ? w.r.start + min(w.r.n, (w.qt * kTile + kTile + g - 1) / g) - r0 : o.own0;
-        o.unit = unit0 + (v ? jj - 1 : jj), o.v = v;
-        return o;
-    }
-};
-
-template <bool kF32>
-UOCR_DEV uint4 load_word(const ChunkArgs& a, const Op& o, int row0, int i) {
-    using R = Rows<kF32>;
-    const int row = row0 + i * R::kPer;
-    if (row >= o.known) return make_uint4(0, 0, 0, 0);
-    return ldg_nc_v4(row < o.cached ? o.pool + (size_t)i * (a.kv_heads * (kDim * R::kElt * R::kPer))
-                                    : o.fresh + i * o.fresh_step);
-}
-
+// ---- the first launch: rows into operands ------------------------------------------------------
 UOCR_DEV bool odd_f32(uint32_t e) { return (e & 0x7F800000u) == 0x7F800000u; }
 UOCR_DEV uint32_t odd_bf16(uint32_t e) { return ((e & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }  // per half, its top bit
 UOCR_DEV uint32_t top_of(const uint4& x) {
     return max(max(x.x & 0x7FFFFFFFu, x.y & 0x7FFFFFFFu), max(x.z & 0x7FFFFFFFu, x.w & 0x7FFFFFFFu));
 }
 
+// A CTA per (page, head, request): its rows of k and v become operands, and its new rows are stored in the
+// pool. A warp takes 16 rows; a word (16 bytes of a thread) is one row of fp32 or two of bf16. Bound: HBM.
 template <bool kF32>
-__device__ void load_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int g) {
-    using R = Rows<kF32>;
-    const int wc = (threadIdx.x >> 5) - kTeamWarps, lane = threadIdx.x & 31;
-    const int row0 = wc * R::kRun + (kF32 ? 0 : lane >> 4), byte = (kF32 ? lane : lane & 15) * 16;
-    Ops ops{s.walk[kTeamWarps + wc]};
-    ops.begin(a, s, g);
-    if (!ops.more) return;
-    // an operand's words: as each is turned into its halves, its register takes the next operand's word
-    uint4 x[R::kWords];
-    Op now = ops.template op<kF32>(a, g, row0, byte);
+__global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Images im) {
+    pdl_launch_dependents();
+    constexpr int kElt = kF32 ? 4 : 2, kPer = kF32 ? 1 : 2, kWords = 16 / kPer;
+    __shared__ uint32_t tops[8], bads[8];
+    const int page = blockIdx.x, b = blockIdx.z, head = a.head0 + blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = a.heads / a.kv_heads;
+    const Request r = request_at(a, b);
+    if (r.n == 0) return;
+    const Tile first = tile_at(a, r, 0, g, kTile);
+    const int last = r.start + r.n - 1, r0 = page * kPageRows;
+    if (r0 > last || (page < first.tail_page && r0 >= r.prefix)) return;  // no token of the request sees it
+    const uint32_t id = __ldg(a.lut + (size_t)b * a.lut_cols + page);
+    const size_t row_bytes = (size_t)a.kv_heads * (kDim * kElt);
+    const size_t index = ((size_t)b * a.lut_cols + page) * a.pass_heads + blockIdx.y;
+    const int row0 = warp * 16 + (kF32 ? 0 : lane >> 4), byte = (kF32 ? lane : lane & 15) * 16;
+    const int cached = r.start - r0, known = min(kPageRows, last + 1 - r0);
+    PageMeta& meta = im.meta[index];
+    for (int v = 0; v < 2; ++v) {
+        char* pool = static_cast<char*>(a.pool) +
+                     ((((size_t)min(id, (uint32_t)(a.pages - 1)) * 2 + v) * a.layers + a.layer) * kPageRows) * row_bytes +
+                     (size_t)head * (kDim * kElt) + byte;
+        const long long ld = (v ? a.v_ld : a.k_ld) * kElt;
+        const char* fresh = static_cast<const char*>(v ? a.v : a.k) + (r.lo - cached) * ld + head * (kDim * kElt) + byte;
+        uint4 x[kWords];
 #pragma unroll
-    for (int i = 0; i < R::kWords; ++i) x[i] = load_word<kF32>(a, now, row0, i);
-    uint32_t stage = 0, phase = 0;
-    for (;;) {
-        ops.next(a, g);
-        const bool more = ops.more;
-        Op ahead = now;
-        if (more) ahead = ops.template op<kF32>(a, g, row0, byte);
-        else ahead.known = 0;
-        if (now.own0 < kPageRows && now.own1 > now.own0) {
+        for (int i = 0; i < kWords; ++i) {
+            const int row = row0 + i * kPer;
+            x[i] = make_uint4(0, 0, 0, 0);
+            if (row < known) x[i] = ldg_nc_v4(row < cached ? pool + row * row_bytes : fresh + row * ld);
+        }
+        if (known > cached && id < (uint32_t)a.pages) {
 #pragma unroll
-            for (int i = 0; i < R::kWords; ++i) {
-                const int row = row0 + i * R::kPer;
-                if (row >= now.own0 && row < min(now.own1, kPageRows))
-                    *reinterpret_cast<uint4*>(now.pool + (size_t)i * (a.kv_heads * (kDim * R::kElt * R::kPer))) = x[i];
+            for (int i = 0; i < kWords; ++i) {
+                const int row = row0 + i * kPer;
+                if (row >= cached && row < known) *reinterpret_cast<uint4*>(pool + row * row_bytes) = x[i];
             }
         }
-        const uint32_t ub = now.unit & 7;
         float up = 1.f;
-        if (now.v) {
+        if (v) {
             // values that are not finite leave the operand; fp32: one scale for the page, whose rows are summed over
             uint32_t top = 0, bad = 0;
 #pragma unroll
-            for (int i = 0; i < R::kWords; ++i)
+            for (int i = 0; i < kWords; ++i)
                 top = kF32 ? max(top, top_of(x[i])) : top | odd_bf16(x[i].x) | odd_bf16(x[i].y) | odd_bf16(x[i].z) | odd_bf16(x[i].w);
             if (kF32) top = __reduce_max_sync(0xffffffffu, top);
             if (kF32 ? top >= 0x7F800000u : __any_sync(0xffffffffu, top != 0)) {  // rare
                 top = 0;
 #pragma unroll
-                for (int i = 0; i < R::kWords; ++i) {
+                for (int i = 0; i < kWords; ++i) {
                     bool row_bad = false;
                     auto drop = [&](uint32_t& e) {
                         if (kF32) {
@@ -446,23 +218,22 @@ __device__ void load_role(const ChunkArgs& a, Shared& s, unsigned char* ring, in
                 }
                 if (kF32) top = __reduce_max_sync(0xffffffffu, top);
             }
-            if (lane == 0) s.vbad[ub][wc] = bad;
-            if constexpr (kF32) {
-                if (lane == 0) s.vmax[now.unit & 1][wc] = __uint_as_float(top);
-                named_bar_sync(kLoadBar, 32 * kLoadWarps);
-                top = __reduce_max_sync(0xffffffffu, __float_as_uint(s.vmax[now.unit & 1][lane % kLoadWarps]));
-                if (wc == 0 && lane == 0) s.vscale[ub] = scale_down(top);
+            if (lane == 0) tops[warp] = top, bads[warp] = bad;
+            __syncthreads();
+            if (kF32) {
+                top = __reduce_max_sync(0xffffffffu, tops[lane & 7]);
                 up = scale_up(top);
+                if (threadIdx.x == 0) meta.v.scale = scale_down(top);
             }
+            if (threadIdx.x < 4) meta.v.bad[threadIdx.x] = bads[2 * threadIdx.x] | bads[2 * threadIdx.x + 1] << 16;
         }
-        if (!wait(s, &s.empty[stage], phase ^ 1)) return;
-        const uint32_t base = smem_addr(ring) + stage * kStageBytes<kF32>;
+        unsigned char* out = im.operands + (index * 2 + v) * kOperandBytes<kF32>;
         uint32_t my_top = 0;  // lane i: the largest magnitude of row i of k
 #pragma unroll
-        for (int i = 0; i < R::kWords; ++i) {
-            const int row = row0 + i * R::kPer;
+        for (int i = 0; i < kWords; ++i) {
+            const int row = row0 + i * kPer;
             if constexpr (kF32) {
-                if (!now.v) {
+                if (!v) {
                     uint32_t top = __reduce_max_sync(0xffffffffu, top_of(x[i]));
                     if (top >= 0x7F800000u) {  // rare: its scores become NaN; it sets no scale
                         uint32_t m = 0;
@@ -479,30 +250,56 @@ __device__ void load_role(const ChunkArgs& a, Shared& s, unsigned char* ring, in
                 uint2 hi, lo;
                 split2(__uint_as_float(x[i].x) * up, __uint_as_float(x[i].y) * up, hi.x, lo.x);
                 split2(__uint_as_float(x[i].z) * up, __uint_as_float(x[i].w) * up, hi.y, lo.y);
-                x[i] = load_word<kF32>(a, ahead, row0, i);
                 // 8 bytes (4 columns) of a block's 128-byte row, whose 16-byte chunks are swizzled by the row
-                const uint32_t at = base + (lane >> 4) * 16384 + row * 128 + ((((lane & 15) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
-                if (row < kPageRows) {
-                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(hi.x), "r"(hi.y) : "memory");
-                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + 32768), "r"(lo.x), "r"(lo.y) : "memory");
-                }
+                unsigned char* at = out + (lane >> 4) * 16384 + row * 128 + ((((lane & 15) >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8;
+                *reinterpret_cast<uint2*>(at) = hi;
+                *reinterpret_cast<uint2*>(at + 32768) = lo;
             } else {
-                const uint32_t at = base + ((lane >> 3) & 1) * 16384 + row * 128 + (((lane & 7) ^ (row & 7)) << 4);
-                if (row < kPageRows)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[i].x), "r"(x[i].y), "r"(x[i].z),
-                                 "r"(x[i].w)
-                                 : "memory");
-                x[i] = load_word<kF32>(a, ahead, row0, i);
+                *reinterpret_cast<uint4*>(out + ((lane >> 3) & 1) * 16384 + row * 128 + (((lane & 7) ^ (row & 7)) << 4)) = x[i];
             }
         }
-        if (kF32 && !now.v && lane < R::kRun && wc * R::kRun + lane < kPageRows)
-            s.kscale[ub][wc * R::kRun + lane] = scale_down(my_top);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.full[stage]);
+        if (kF32 && !v && lane < 16) meta.kscale[warp * 16 + lane] = scale_down(my_top);
+    }
+}
+
+// ---- the copying warp ---------------------------------------------------------------------------
+// Operands in the order in which the tensor core takes them, over a segment: K(0), K(1), V(0), K(2), V(1), ...,
+// V(n - 1). One thread.
+template <bool kF32>
+__device__ void copy_role(const ChunkArgs& a, Shared& s, unsigned char* ring, const Images& im, int g) {
+    Walk& w = s.walk[kTeamWarps + 1];
+    uint32_t stage = 0, phase = 0, unit0 = 0, issued = 0;
+    auto copy = [&](bool v, int j) {
+        const size_t index = ((size_t)w.b * a.lut_cols + w.t.page(w.j + j)) * a.pass_heads + w.head;
+        const uint32_t u = (unit0 + j) & 7;
+        const PageMeta& meta = im.meta[index];
+        if (!mbar_wait(&s.empty[stage], phase ^ 1, nullptr)) return false;
+        const uint32_t extra = v ? sizeof(ValueMeta) : kF32 ? sizeof(meta.kscale) : 0;
+        mbar_arrive_expect_tx(&s.full[stage], kOperandBytes<kF32> + extra);
+        bulk_g2s(ring + stage * kOperandBytes<kF32>, im.operands + (index * 2 + v) * kOperandBytes<kF32>, kOperandBytes<kF32>,
+                 &s.full[stage]);
+        if (v) bulk_g2s(&s.vmeta[u], &meta.v, sizeof(ValueMeta), &s.full[stage]);
+        else if (kF32) bulk_g2s(s.kscale[u], meta.kscale, sizeof(meta.kscale), &s.full[stage]);
+        ++issued;
         if (++stage == kStages<kF32>) stage = 0, phase ^= 1;
-        if (!more) return;
-        now = ahead;
+        return true;
+    };
+    auto run = [&] {
+        for (bool more = w.begin(a, s.run, g, kTile); more; more = w.next(a, g, kTile)) {
+            const int n = w.n;
+            for (int jj = 0; jj <= n; ++jj) {
+                if (jj < n && !copy(false, jj)) return false;
+                if (jj >= 1 && !copy(true, jj - 1)) return false;
+            }
+            unit0 += n;
+        }
+        return true;
+    };
+    if (run()) return;
+    s.abort = 1;  // a wait gave up: the copies in flight land before this CTA's memory is given back
+    for (uint32_t k = 0; k < kStages<kF32> && k < issued; ++k) {
+        if (stage == 0) stage = kStages<kF32>, phase ^= 1;
+        mbar_wait(&s.full[--stage], phase, nullptr);
     }
 }
 
@@ -511,7 +308,7 @@ template <bool kF32>
 __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int g) {
     const uint32_t tmem = s.tmem, base = smem_addr(ring);
     uint32_t stage = 0, phase = 0, unit0 = 0, seg = 0;
-    Walk& w = s.walk[kTeamWarps + kLoadWarps];
+    Walk& w = s.walk[kTeamWarps];
     // one operand: its MMAs issued (D = sum over the products of A's halves and the operand's, 16 of the summed
     // dimension at a time), its stage given back, the result announced
     auto product = [&](uint32_t d, uint32_t ta, uint32_t a_step, uint32_t a_lo, uint32_t kind, uint32_t b_step2, uint32_t b_step8,
@@ -519,7 +316,7 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
         if (!wait(s, &s.full[stage], phase)) return false;
         tc_fence_after();
         if (elect_one()) {
-            const uint32_t b = desc_lo(base + stage * kStageBytes<kF32>, kind);
+            const uint32_t b = desc_lo(base + stage * kOperandBytes<kF32>, kind);
 #pragma unroll
             for (int p = kF32 ? 0 : 2; p < 3; ++p) {  // lo x hi, hi x lo, hi x hi
 #pragma unroll
@@ -538,7 +335,7 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
     auto run = [&] {
         auto next = [&](bool first) {
             __syncwarp();
-            const bool more = first ? w.begin(a, s.run, g) : w.next(a, g);
+            const bool more = first ? w.begin(a, s.run, g, kTile) : w.next(a, g, kTile);
             __syncwarp();
             return more;
         };
@@ -582,11 +379,11 @@ __device__ __noinline__ void add_bad_values(const ChunkArgs& a, const Walk& w, i
     const uint32_t id = __ldg(a.lut + (size_t)w.b * a.lut_cols + t);
     const size_t row_elts = (size_t)a.kv_heads * kDim;
     const char* p = r >= w.r.start
-                        ? static_cast<const char*>(a.v) + ((size_t)(w.r.lo + r - w.r.start) * a.v_ld + w.head * kDim) * elt
+                        ? static_cast<const char*>(a.v) + ((size_t)(w.r.lo + r - w.r.start) * a.v_ld + (a.head0 + w.head) * kDim) * elt
                         : static_cast<const char*>(a.pool) +
                               (((((size_t)min(id, (uint32_t)(a.pages - 1)) * 2 + 1) * a.layers + a.layer) * kPageRows + row) *
                                    row_elts +
-                               w.head * kDim) *
+                               (a.head0 + w.head) * kDim) *
                                   elt;
     for (int d = 0; d < 64; ++d) {
         const float v = kF32 ? reinterpret_cast<const float*>(p)[half * 64 + d]
@@ -602,7 +399,7 @@ UOCR_DEV uint32_t seen_mask(int c0, int hi, int lo, int pre) {
 }
 
 template <bool kF32>
-__device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info, int g) {
+__device__ void team_role(const ChunkArgs& a, Shared& s, const ChunkParts& parts, int g) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = s.tmem + ((uint32_t)(warp & 3) << 21);  // lane field: bits 16 up, 32 lanes a warp
@@ -615,7 +412,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
         const int R = w.qt * kTile + row;
         const bool valid = R < w.r.n * g;
         const char* p = static_cast<const char*>(a.q) +
-                        ((size_t)(w.r.lo + (valid ? R / g : 0)) * a.q_ld + (size_t)(w.head * g + (valid ? R % g : 0)) * kDim) *
+                        ((size_t)(w.r.lo + (valid ? R / g : 0)) * a.q_ld + (size_t)((a.head0 + w.head) * g + (valid ? R % g : 0)) * kDim) *
                             (kF32 ? 4 : 2);
         if constexpr (kF32) {
             const float4* q4 = reinterpret_cast<const float4*>(p);
@@ -672,7 +469,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
         if (alive && !wait(s, &s.pv_full, u & 1)) alive = false;
         if (alive && live) {
             tc_fence_after();
-            const float f = kF32 ? s.vscale[u & 7] : 1.f;
+            const float f = kF32 ? s.vmeta[u & 7].scale : 1.f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t x[16];
@@ -681,10 +478,10 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fmaf(acc[c * 16 + i], alpha, __uint_as_float(x[i]) * f);
             }
-            const uint4* vb = reinterpret_cast<const uint4*>(s.vbad[u & 7]);
-            if (vb[0].x | vb[0].y | vb[0].z | vb[0].w | vb[1].x | vb[1].y | vb[1].z) {
+            const uint4 vb = *reinterpret_cast<const uint4*>(s.vmeta[u & 7].bad);
+            if (vb.x | vb.y | vb.z | vb.w) {
                 for (int q = 0; q < kPageRows; ++q) {
-                    if (!(s.vbad[u & 7][q / Rows<kF32>::kRun] >> (q % Rows<kF32>::kRun) & 1)) continue;
+                    if (!(s.vmeta[u & 7].bad[q >> 5] >> (q & 31) & 1)) continue;
                     const int r = t * kPageRows + q;
                     const bool seen = r <= pos && (a.window <= 0 || r > pos - a.window || r < w.r.prefix);
                     float extra[64];
@@ -702,7 +499,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
 
     Walk& w = s.walk[warp];
     Walk& done = s.done[warp];
-    bool more = w.begin(a, s.run, g);
+    bool more = w.begin(a, s.run, g, kTile);
     __syncwarp();
     int state[2] = {0, 0}, place[4] = {0, 0, 0, 0};
     uint32_t unit0 = 0;
@@ -805,7 +602,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
         unit0 += w.n;
         done = w;
         __syncwarp();
-        more = w.next(a, g);
+        more = w.next(a, g, kTile);
         __syncwarp();
         if (more) load_query(w);  // every score of the finished segment has been read: its query is free
         add_pv(done, last, done.t.page(done.j + done.n - 1), live, pos);
@@ -820,7 +617,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
         if (done.whole()) {
             if (mine) {
                 const float inv = 1.f / total;
-                const size_t at = ((size_t)(done.r.lo + R / g) * a.heads + done.head * g + R % g) * kDim + half * 64;
+                const size_t at = ((size_t)(done.r.lo + R / g) * a.heads + (a.head0 + done.head) * g + R % g) * kDim + half * 64;
                 if constexpr (kF32) {
                     float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.out) + at);
 #pragma unroll
@@ -838,7 +635,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
             }
         } else {
             const int slot = done.j == 0 ? 1 : 0;
-            float* part = slots + ((size_t)blockIdx.x * 2 + slot) * kSlotFloats;
+            float* part = parts.slots + ((size_t)blockIdx.x * 2 + slot) * slot_floats(kTile);
             if (mine) {
 #pragma unroll
                 for (int i = 0; i < 64; ++i) part[(half * 64 + i) * kTile + row] = acc[i];
@@ -848,77 +645,82 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, float* slots, int* info
                 }
             }
             state[slot] = slot == 0 && done.j + done.n == done.t.count ? 2 : 1;
-            if (slot == 1) place[0] = done.r.lo, place[1] = done.qt * kTile, place[2] = min(rows, kTile), place[3] = done.head;
+            if (slot == 1) place[0] = done.r.lo, place[1] = done.qt * kTile, place[2] = min(rows, kTile), place[3] = a.head0 + done.head;
         }
     }
     if (threadIdx.x == 0) {
-        int* o = info + blockIdx.x * kInfoInts;
+        int* o = parts.info + blockIdx.x * kInfoInts;
         o[0] = state[0], o[1] = state[1];
         for (int i = 0; i < 4; ++i) o[2 + i] = place[i];
     }
 }
 
 template <bool kF32>
-__global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs a, float* slots, int* info) {
+__global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs a, Images im, ChunkParts parts) {
     extern __shared__ unsigned char raw[];
     __shared__ Shared s;
     unsigned char* ring = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
     const int warp = threadIdx.x >> 5;
     const int g = a.heads / a.kv_heads;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kMaxStages; ++i) mbar_init(&s.full[i], kLoadWarps), mbar_init(&s.empty[i], 1);
+        for (int i = 0; i < kMaxStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&s.s_full[i], 1), mbar_init(&s.p_full[i], kTeamWarps);
         mbar_init(&s.pv_full, 1), mbar_init(&s.pv_free, kTeamWarps), mbar_init(&s.q_full, kTeamWarps), mbar_init(&s.drain, 1);
         fence_mbar_init();
         s.abort = 0;
-        for (int i = 0; i < 8; ++i) s.vbad[i][7] = 0;
     }
-    if (warp == kTeamWarps + kLoadWarps) tmem_alloc(&s.tmem, 512);
+    if (warp == kTeamWarps) tmem_alloc(&s.tmem, 512);
     tc_fence_before();
-    find_run(a, s, reinterpret_cast<long long*>(ring), g);
+    find_run(a, s.run, reinterpret_cast<long long*>(ring), g, kTile);
     tc_fence_after();
     pdl_launch_dependents();
     if (warp < kTeamWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTeamRegs));
-        team_role<kF32>(a, s, slots, info, g);
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
-        if (warp < kTeamWarps + kLoadWarps) load_role<kF32>(a, s, ring, g);
-        else mma_role<kF32>(a, s, ring, g);
+        team_role<kF32>(a, s, parts, g);
+    } else if (warp == kTeamWarps) {
+        mma_role<kF32>(a, s, ring, g);
+    } else if ((threadIdx.x & 31) == 0) {
+        fence_proxy_async_smem();  // the ring was find_run's scratch
+        pdl_wait_prior_grid();
+        copy_role<kF32>(a, s, ring, im, g);
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == kTeamWarps + kLoadWarps) tmem_dealloc(s.tmem, 512);
+    if (warp == kTeamWarps) tmem_dealloc(s.tmem, 512);
 }
 
 // The parts of a tile that was cut: CTA c's slot 1 begins it, slot 0 of the CTAs behind it continues it.
-// out = sum_i 2^(m_i - M) sum_i / sum_i 2^(m_i - M) l_i, in the order of the pages. A block joins 16
-// columns of one tile.
+// out = sum_i 2^(m_i - M) sum_i / sum_i 2^(m_i - M) l_i, in the order of the pages. A block joins as
+// many groups of 8 columns of a tile as it has threads for.
 template <bool kF32>
-__global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a, const float* slots, const int* info, int ctas) {
+__global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a, ChunkParts p) {
     pdl_wait_prior_grid();
+    const float* slots = p.slots;
+    const int* info = p.info;
+    const int ctas = p.ctas, tile = p.tile;
+    const size_t slot = slot_floats(tile);
     const int c = blockIdx.x, g = a.heads / a.kv_heads;
     const int* o = info + c * kInfoInts;
     if (o[1] == 0) return;
     const int lo = o[2], r0 = o[3], rows = o[4], head = o[5];
-    const int row = threadIdx.x & 127, c0 = blockIdx.y * 16 + (threadIdx.x >> 7) * 8;
-    if (row >= rows) return;
+    // threads by row, then by 8 columns: few rows take few threads' time
+    const int group = blockIdx.y * (256 / tile) + threadIdx.x / tile, row = threadIdx.x % tile, c0 = group * 8;
+    if (row >= rows || group >= kDim / 8) return;
     int end = c + 1;  // one behind the last CTA of this tile
     while (end < ctas && info[end * kInfoInts] == 1) ++end;
     end = min(end + 1, ctas);
     float M = -INFINITY;
-    for (int d = c; d < end; ++d) M = fmaxf(M, slots[((size_t)d * 2 + (d == c)) * kSlotFloats + kDim * kTile + row]);
+    for (int d = c; d < end; ++d) M = fmaxf(M, slots[((size_t)d * 2 + (d == c)) * slot + kDim * tile + row]);
     float l = 0.f, x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.f;
     for (int d = c; d < end; ++d) {
-        const float* part = slots + ((size_t)d * 2 + (d == c)) * kSlotFloats;
-        const float md = part[kDim * kTile + row];
+        const float* part = slots + ((size_t)d * 2 + (d == c)) * slot;
+        const float md = part[kDim * tile + row];
         const float f = md == -INFINITY ? 0.f : exp2_fast(md - M);  // a part in which the row sees nothing
-        l = fmaf(part[(kDim + 1) * kTile + row], f, l);
+        l = fmaf(part[(kDim + 1) * tile + row], f, l);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fmaf(part[(c0 + i) * kTile + row], f, x[i]);
+        for (int i = 0; i < 8; ++i) x[i] = fmaf(part[(c0 + i) * tile + row], f, x[i]);
     }
     const float inv = 1.f / l;
     const int R = r0 + row;
@@ -934,36 +736,73 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a, const floa
     }
 }
 
-template <bool kF32>
-cudaError_t launch(const ChunkArgs& a, void* ws, int sms, cudaStream_t st) {
-    const size_t smem = (size_t)kStages<kF32> * kStageBytes<kF32> + 1024;
-    auto kernel = chunk_attention_kernel<kF32>;
-    cudaError_t err = ensure_smem_optin(reinterpret_cast<const void*>(kernel), smem);
-    if (err != cudaSuccess) return err;
-    int* info = static_cast<int*>(ws);
-    float* slots = reinterpret_cast<float*>(static_cast<char*>(ws) + ((size_t)sms * kInfoInts * 4 + 255) / 256 * 256);
-    kernel<<<sms, kThreads, smem, st>>>(a, slots, info);
-    err = cudaGetLastError();
-    if (err != cudaSuccess) return err;
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(sms, kDim / 16), cfg.blockDim = dim3(256), cfg.stream = st;
+    cfg.gridDim = grid, cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr, cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, chunk_join_kernel<kF32>, a, static_cast<const float*>(slots),
-                              static_cast<const int*>(info), sms);
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
+template <bool kF32>
+cudaError_t launch(const ChunkArgs& a, const Images& im, const ChunkParts& parts, cudaStream_t st) {
+    const size_t smem = (size_t)kStages<kF32> * kOperandBytes<kF32> + 1024;
+    auto kernel = chunk_attention_kernel<kF32>;
+    cudaError_t err = ensure_smem_optin(reinterpret_cast<const void*>(kernel), smem);
+    if (err != cudaSuccess) return err;
+    chunk_operands_kernel<kF32><<<dim3(a.lut_cols, a.pass_heads, a.B), 256, 0, st>>>(a, im);
+    err = cudaGetLastError();
+    if (err != cudaSuccess) return err;
+    err = launch_dependent(kernel, dim3(parts.ctas), kThreads, smem, st, a, im, parts);
+    if (err != cudaSuccess) return err;
+    return launch_chunk_join(a, parts, st);
+}
+
+// Bytes of a page's operands and their meta data, one head.
+size_t image_bytes(bool bf16) { return 2 * (size_t)(bf16 ? kOperandBytes<false> : kOperandBytes<true>) + sizeof(PageMeta); }
+
+// The KV heads of one pass: their operands stay within 1 GiB (one head at least); a call with more takes several.
+constexpr size_t kPassBytes = size_t(1) << 30;
+int heads_of_pass(const ChunkArgs& a) {
+    const size_t head = (size_t)a.B * a.lut_cols * image_bytes(a.bf16);
+    return (int)std::max<size_t>(1, std::min<size_t>(a.kv_heads, kPassBytes / head));
+}
+
+size_t parts_bytes(int sms, int tile) {
+    return ((size_t)sms * kInfoInts * 4 + 255) / 256 * 256 + ((size_t)sms * 2 * tile * (kDim + 2) * 4 + 255) / 256 * 256;
 }
 
 }  // namespace
 
-size_t chunk_workspace_bytes(int sms) {
-    return ((size_t)sms * kInfoInts * 4 + 255) / 256 * 256 + (size_t)sms * 2 * kSlotFloats * sizeof(float);
+cudaError_t launch_chunk_join(const ChunkArgs& a, const ChunkParts& p, cudaStream_t st) {
+    const int groups = 256 / p.tile;  // of 8 columns, a block
+    const dim3 grid(p.ctas, (kDim / 8 + groups - 1) / groups);
+    return launch_dependent(a.bf16 ? chunk_join_kernel<false> : chunk_join_kernel<true>, grid, 256, 0, st, a, p);
 }
 
-cudaError_t launch_chunk_attention(const ChunkArgs& a, void* ws, int sms, cudaStream_t st) {
+size_t chunk_workspace_bytes(const ChunkArgs& a, int sms) {
+    return parts_bytes(sms, kTile) + (size_t)a.B * a.lut_cols * heads_of_pass(a) * image_bytes(a.bf16);
+}
+
+cudaError_t launch_chunk_attention(const ChunkArgs& args, void* ws, int sms, cudaStream_t st) {
+    ChunkArgs a = args;
     if (a.B <= 0 || a.T <= 0) return cudaSuccess;
-    return a.bf16 ? launch<false>(a, ws, sms, st) : launch<true>(a, ws, sms, st);
+    char* w = static_cast<char*>(ws);
+    ChunkParts parts{reinterpret_cast<float*>(w + ((size_t)sms * kInfoInts * 4 + 255) / 256 * 256), reinterpret_cast<int*>(w), sms,
+                     kTile};
+    const int heads = heads_of_pass(a);
+    Images im;
+    im.operands = reinterpret_cast<unsigned char*>(w + parts_bytes(sms, kTile));
+    im.meta = reinterpret_cast<PageMeta*>(im.operands + (size_t)a.B * a.lut_cols * heads * (image_bytes(a.bf16) - sizeof(PageMeta)));
+    for (a.head0 = 0; a.head0 < a.kv_heads; a.head0 += heads) {
+        a.pass_heads = std::min(heads, a.kv_heads - a.head0);
+        const cudaError_t err = a.bf16 ? launch<false>(a, im, parts, st) : launch<true>(a, im, parts, st);
+        if (err != cudaSuccess) return err;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace uocr

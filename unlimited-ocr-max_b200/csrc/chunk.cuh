@@ -1,0 +1,195 @@
+// What the two forms of the chunk attention share: the division of a call's work over the CTAs, and the parts
+// that they leave for the joining launch.
+#pragma once
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "sm100.cuh"
+
+namespace uocr {
+
+// Parts of query tiles that were cut: per CTA two slots of [128 columns][tile rows] sums, m [tile], l [tile], and
+// what the joining launch needs to know.
+struct ChunkParts {
+    float* slots;
+    int* info;     // [CTAs][kInfoInts]: states of the two slots, then the place of the tile that slot 1 begins
+    int ctas, tile;
+};
+cudaError_t launch_chunk_join(const ChunkArgs& a, const ChunkParts& p, cudaStream_t st);
+cudaError_t launch_chunk_rows(const ChunkArgs& a, const ChunkParts& p, cudaStream_t st);
+
+namespace {
+
+constexpr int kPageRows = 128;  // rows of a page, and of a unit
+constexpr int kDim = 128;
+constexpr int kInfoInts = 8;
+constexpr float kLog2e = 1.44269504088896341f;
+
+UOCR_DEV size_t slot_floats(int tile) { return (size_t)tile * (kDim + 2); }
+
+struct Request {
+    int lo, n, start, prefix;
+};
+
+UOCR_DEV Request request_at(const ChunkArgs& a, int b) {
+    Request r;
+    r.lo = min(max(__ldg(a.offsets + b), 0), a.T);
+    r.start = min(max(__ldg(a.start + b), 0), a.lut_cols * kPageRows);
+    r.n = max(min(min(__ldg(a.offsets + b + 1), a.T) - r.lo, a.lut_cols * kPageRows - r.start), 0);
+    r.prefix = a.prefix ? max(__ldg(a.prefix + b), 0) : 0;
+    return r;
+}
+
+// A query tile is `tile` (token, query head of the KV head) rows of a request. Its pages: columns [0, head_pages) and [tail_page, ...) of its lookup row, `count` in all.
+struct Tile {
+    int first_pos, last_pos;  // logical rows of its first and last token
+    int head_pages, tail_page, count;
+    UOCR_DEV int page(int j) const { return j < head_pages ? j : j - head_pages + tail_page; }
+};
+
+UOCR_DEV Tile tile_at(const ChunkArgs& a, const Request& r, int qt, int g, int tile) {
+    Tile t;
+    const int r0 = qt * tile;
+    t.first_pos = r.start + r0 / g;
+    t.last_pos = r.start + min(r.n - 1, (r0 + tile - 1) / g);
+    t.head_pages = t.tail_page = 0;
+    if (a.window > 0) {
+        t.tail_page = max(0, t.first_pos - a.window + 1) / kPageRows;
+        t.head_pages = min((min(r.prefix, t.last_pos + 1) + kPageRows - 1) / kPageRows, t.tail_page);
+    }
+    t.count = t.head_pages + t.last_pos / kPageRows + 1 - t.tail_page;
+    return t;
+}
+
+// A CTA's run: its units, and where they begin (heads are counted from the pass's first).
+struct Run {
+    int left, b, qt, head, j;
+};
+
+// The walk over a CTA's units, a segment (pages of one tile and head) at a time; every warp walks by
+// itself.
+struct Walk {
+    int b, qt, head, j, n, tiles;  // segment: pages j .. j + n - 1 of the tile's
+    int left;                      // units behind this segment
+    Request r;
+    Tile t;
+    UOCR_DEV void enter(const ChunkArgs& a, int g, int tile) {
+        t = tile_at(a, r, qt, g, tile);
+        n = min(t.count - j, left);
+        left -= n;
+    }
+    UOCR_DEV bool begin(const ChunkArgs& a, const Run& s, int g, int tile) {
+        left = s.left;
+        if (left <= 0) return false;
+        b = s.b, qt = s.qt, head = s.head, j = s.j;
+        r = request_at(a, b);
+        tiles = (r.n * g + tile - 1) / tile;
+        enter(a, g, tile);
+        return true;
+    }
+    UOCR_DEV bool next(const ChunkArgs& a, int g, int tile) {
+        if (left <= 0) return false;
+        j = 0;
+        if (++head == a.pass_heads) {
+            head = 0;
+            if (++qt >= tiles) {
+                qt = 0;
+                do {  // left > 0: another request with rows follows
+                    ++b;
+                    r = request_at(a, b);
+                } while (r.n == 0 && b < a.B - 1);
+                tiles = (r.n * g + tile - 1) / tile;
+            }
+        }
+        enter(a, g, tile);
+        return true;
+    }
+    UOCR_DEV bool whole() const { return j == 0 && n == t.count; }
+};
+
+template <typename T>
+UOCR_DEV T warp_scan(T v, int lane) {  // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const T u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+// All threads: this CTA's run of units. scratch: B long longs of shared memory.
+__device__ __noinline__ void find_run(const ChunkArgs& a, Run& run, long long* scratch, int g, int tile) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int b = warp; b < a.B; b += blockDim.x / 32) {
+        const Request r = request_at(a, b);
+        const int tiles = (r.n * g + tile - 1) / tile;
+        long long sum = 0;
+        for (int qt = lane; qt < tiles; qt += 32) sum += tile_at(a, r, qt, g, tile).count;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) scratch[b] = sum * a.pass_heads;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        long long total = 0;
+        for (int b = lane; b < a.B; b += 32) total += scratch[b];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        const long long ctas = min((long long)gridDim.x, total);
+        long long u0 = 0, u1 = 0;
+        if ((long long)blockIdx.x < ctas) u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
+        if (lane == 0) run.left = (int)(u1 - u0);
+        if (u1 > u0) {
+            int b = 0;
+            long long before = 0;  // units in front of request b
+            for (int b0 = 0; b0 < a.B; b0 += 32) {
+                const long long mine = b0 + lane < a.B ? scratch[b0 + lane] : 0;
+                const long long upto = before + warp_scan(mine, lane);
+                const uint32_t hit = __ballot_sync(0xffffffffu, upto > u0);
+                if (hit) {
+                    const int f = __ffs(hit) - 1;
+                    b = b0 + f;
+                    before = __shfl_sync(0xffffffffu, upto - mine, f);
+                    break;
+                }
+                before = __shfl_sync(0xffffffffu, upto, 31);
+            }
+            const Request r = request_at(a, b);
+            const int tiles = (r.n * g + tile - 1) / tile;
+            for (int q0 = 0; q0 < tiles; q0 += 32) {
+                const int count = q0 + lane < tiles ? tile_at(a, r, q0 + lane, g, tile).count : 0;
+                const long long upto = before + warp_scan((long long)count * a.pass_heads, lane);
+                const uint32_t hit = __ballot_sync(0xffffffffu, upto > u0);
+                if (hit) {
+                    if (lane == __ffs(hit) - 1) {
+                        const long long in = u0 - (upto - (long long)count * a.pass_heads);
+                        run.b = b, run.qt = q0 + lane, run.head = (int)(in / count), run.j = (int)(in % count);
+                    }
+                    break;
+                }
+                before = __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+    }
+    __syncthreads();
+}
+
+UOCR_DEV uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+UOCR_DEV uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+UOCR_DEV float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+}  // namespace
+}  // namespace uocr

@@ -58,9 +58,10 @@ struct ChunkArgs {
     const int32_t* prefix;              // [B] or null
     int T, B, heads, kv_heads, pages, layers, layer, lut_cols, window, bf16;
     float scale;
+    int head0, pass_heads;              // the KV heads of one pass over the call (set by the launcher)
 };
 constexpr int kChunkMaxRequests = 8192;
-size_t chunk_workspace_bytes(int sms);
+size_t chunk_workspace_bytes(const ChunkArgs& a, int sms);
 cudaError_t launch_chunk_attention(const ChunkArgs& a, void* ws, int sms, cudaStream_t st);
 
 // pages.cu: pages copied (their first rows[i] rows; null: whole), and kept rows moved to the front

@@ -365,7 +365,7 @@ def paged_chunk_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Ten
             if a < hi and lo < z:
                 raise ValueError(f"{op}: out overlaps {name}")
     with torch.cuda.device(q.device):
-        need = load().uocr_paged_chunk_workspace_bytes()
+        need = load().uocr_paged_chunk_workspace_bytes(T, heads, kv_heads, 1 if dt == torch.bfloat16 else 0, lut.shape[1], B)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         check(load().uocr_paged_chunk_attention(
             q.data_ptr(), q_ld, k_new.data_ptr(), k_ld, v_new.data_ptr(), v_ld, T, heads, kv_heads, dim,
