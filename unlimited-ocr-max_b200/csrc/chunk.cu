@@ -37,8 +37,10 @@ namespace uocr {
 namespace {
 
 constexpr int kTile = 128;      // (token, head) rows of a query tile
-constexpr int kTeamWarps = 8;   // softmax; then the issuing warp and the copying warp
-constexpr int kThreads = 32 * (kTeamWarps + 2);
+constexpr int kTeamWarps = 8;   // softmax; then a warpgroup of the issuing warp, the copying warp and two idle ones
+constexpr int kThreads = 32 * (kTeamWarps + 4);
+constexpr int kLaunchRegs = 168, kTeamRegs = 208, kOtherRegs = 88;  // a thread
+static_assert(kTeamWarps * kTeamRegs + 4 * kOtherRegs <= (kTeamWarps + 4) * kLaunchRegs, "a split of the launch's registers");
 // An operand: a page's 128 rows of k or of v of one head, as two blocks of 64 columns [128 rows][128 bytes]; fp32:
 // the lo halves behind the hi halves.
 template <bool kF32>
@@ -46,7 +48,9 @@ constexpr int kOperandBytes = kF32 ? 65536 : 32768;
 template <bool kF32>
 constexpr int kStages = kF32 ? 3 : 6;  // of operands in shared memory
 constexpr int kMaxStages = 6;
-constexpr uint32_t kTeamBar = 1;
+constexpr uint32_t kTeamBar = 1, kPairBar = 2;  // all softmax warps; the two of 32 rows (kPairBar + 0..3)
+constexpr int kStagingBytes = kTile * 128;  // a quarter (fp32) or half (bf16) of a tile's rows, between the row-wise and the
+                                            // lane-wise order; 16-byte chunks swizzled by the row
 
 // TMEM columns
 constexpr uint32_t kColS = 0, kColPv = 256, kColQ = 384;
@@ -77,7 +81,7 @@ struct Shared {
     volatile int abort;
     Run run;
     Walk walk[kThreads / 32], done[kTeamWarps];
-    float xmax[2][2][kTile], xsum[2][kTile];
+    float xmax[2][2][kTile], xsum[2][kTile], qscale[kTile];
 };
 
 UOCR_DEV bool wait(Shared& s, uint64_t* bar, uint32_t parity) {
@@ -119,21 +123,51 @@ UOCR_DEV void tmem_st<8>(uint32_t addr, const uint32_t* r) {
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
-// tcgen05.wait::ld that marks r[] as written by it: no use of r[] moves in front of it
-UOCR_DEV void tmem_wait_ld16(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
+// 64 columns into x, complete on return (the waits mark x as written by them: no use moves in front of them).
+UOCR_DEV void tmem_ld64(uint32_t addr, uint32_t (&x)[64]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]), "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31])
+                 : "r"(addr + 0));
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(x[32]), "=r"(x[33]), "=r"(x[34]), "=r"(x[35]), "=r"(x[36]), "=r"(x[37]), "=r"(x[38]), "=r"(x[39]), "=r"(x[40]), "=r"(x[41]), "=r"(x[42]), "=r"(x[43]), "=r"(x[44]), "=r"(x[45]), "=r"(x[46]), "=r"(x[47]), "=r"(x[48]), "=r"(x[49]), "=r"(x[50]), "=r"(x[51]), "=r"(x[52]), "=r"(x[53]), "=r"(x[54]), "=r"(x[55]), "=r"(x[56]), "=r"(x[57]), "=r"(x[58]), "=r"(x[59]), "=r"(x[60]), "=r"(x[61]), "=r"(x[62]), "=r"(x[63])
+                 : "r"(addr + 32));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]), "+r"(x[9]), "+r"(x[10]), "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15]) : : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[16]), "+r"(x[17]), "+r"(x[18]), "+r"(x[19]), "+r"(x[20]), "+r"(x[21]), "+r"(x[22]), "+r"(x[23]), "+r"(x[24]), "+r"(x[25]), "+r"(x[26]), "+r"(x[27]), "+r"(x[28]), "+r"(x[29]), "+r"(x[30]), "+r"(x[31]) : : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[32]), "+r"(x[33]), "+r"(x[34]), "+r"(x[35]), "+r"(x[36]), "+r"(x[37]), "+r"(x[38]), "+r"(x[39]), "+r"(x[40]), "+r"(x[41]), "+r"(x[42]), "+r"(x[43]), "+r"(x[44]), "+r"(x[45]), "+r"(x[46]), "+r"(x[47]) : : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[48]), "+r"(x[49]), "+r"(x[50]), "+r"(x[51]), "+r"(x[52]), "+r"(x[53]), "+r"(x[54]), "+r"(x[55]), "+r"(x[56]), "+r"(x[57]), "+r"(x[58]), "+r"(x[59]), "+r"(x[60]), "+r"(x[61]), "+r"(x[62]), "+r"(x[63]) : : "memory");
+}
+// Two fp32 operations an instruction (each rounded as its scalar form).
+UOCR_DEV uint64_t pair(uint32_t x, uint32_t y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
+    return r;
+}
+UOCR_DEV uint64_t pair(float x, float y) { return pair(__float_as_uint(x), __float_as_uint(y)); }
+UOCR_DEV void unpair(uint64_t v, uint32_t& x, uint32_t& y) { asm("mov.b64 {%0, %1}, %2;" : "=r"(x), "=r"(y) : "l"(v)); }
+UOCR_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+UOCR_DEV uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+UOCR_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
 UOCR_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // two values as fp16 halves: hi takes the upper 11 bits (exactly), lo the rest (rounded to 11 bits)
 UOCR_DEV void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const float xh = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u), yh = __uint_as_float(__float_as_uint(y) & 0xFFFFE000u);
-    hi = pack_f16(xh, yh);
-    lo = pack_f16(__fsub_rn(x, xh), __fsub_rn(y, yh));
+    const uint32_t xh = __float_as_uint(x) & 0xFFFFE000u, yh = __float_as_uint(y) & 0xFFFFE000u;
+    uint32_t xl, yl;
+    unpair(add2(pair(x, y), pair(xh ^ 0x80000000u, yh ^ 0x80000000u)), xl, yl);
+    hi = pack_f16(__uint_as_float(xh), __uint_as_float(yh));
+    lo = pack_f16(__uint_as_float(xl), __uint_as_float(yl));
 }
 // 2^(14 - e) and its inverse for the largest magnitude's bits (e its exponent, from -112 up: below that
 // the values are smaller than 2^14 after scaling, which costs them bits they do not have)
@@ -370,26 +404,15 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
 
 // ---- the softmax warps ------------------------------------------------------------------------
 // Thread (row, half): row of the query tile (its TMEM lane), columns and dimensions [64 half, 64 half + 64).
+// Row `row` of the values of page t (this head's 128 columns).
 template <bool kF32>
-__device__ __noinline__ void add_bad_values(const ChunkArgs& a, const Walk& w, int t, int row, bool seen, int half,
-                                            float* out64) {
-    // value row `row` of page t: what is not finite of this half's 64 columns, into out64 (else 0)
-    const int r = t * kPageRows + row;
-    const size_t elt = kF32 ? 4 : 2;
-    const uint32_t id = __ldg(a.lut + (size_t)w.b * a.lut_cols + t);
-    const size_t row_elts = (size_t)a.kv_heads * kDim;
-    const char* p = r >= w.r.start
-                        ? static_cast<const char*>(a.v) + ((size_t)(w.r.lo + r - w.r.start) * a.v_ld + (a.head0 + w.head) * kDim) * elt
-                        : static_cast<const char*>(a.pool) +
-                              (((((size_t)min(id, (uint32_t)(a.pages - 1)) * 2 + 1) * a.layers + a.layer) * kPageRows + row) *
-                                   row_elts +
-                               (a.head0 + w.head) * kDim) *
-                                  elt;
-    for (int d = 0; d < 64; ++d) {
-        const float v = kF32 ? reinterpret_cast<const float*>(p)[half * 64 + d]
-                             : bf16f(reinterpret_cast<const uint16_t*>(p)[half * 64 + d]);
-        if (seen && (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u) out64[d] += v;
-    }
+UOCR_DEV const char* value_row(const ChunkArgs& a, const Walk& w, int t, int row) {
+    constexpr int kElt = kF32 ? 4 : 2;
+    const int r = t * kPageRows + row, column = (a.head0 + w.head) * kDim;
+    if (r >= w.r.start) return static_cast<const char*>(a.v) + ((size_t)(w.r.lo + r - w.r.start) * a.v_ld + column) * kElt;
+    const uint32_t id = min(__ldg(a.lut + (size_t)w.b * a.lut_cols + t), (uint32_t)(a.pages - 1));
+    return static_cast<const char*>(a.pool) +
+           (((((size_t)id * 2 + 1) * a.layers + a.layer) * kPageRows + row) * ((size_t)a.kv_heads * kDim) + column) * kElt;
 }
 
 // Which of 32 columns from c0 on a row sees: c <= hi and (c >= lo or c < pre), all relative to the page.
@@ -399,84 +422,106 @@ UOCR_DEV uint32_t seen_mask(int c0, int hi, int lo, int pre) {
 }
 
 template <bool kF32>
-__device__ void team_role(const ChunkArgs& a, Shared& s, const ChunkParts& parts, int g) {
+__device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging, const ChunkParts& parts, int g) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = s.tmem + ((uint32_t)(warp & 3) << 21);  // lane field: bits 16 up, 32 lanes a warp
     const float factor = fabsf(a.scale) * kLog2e;  // the scale's sign is in the query operand
     float qscale = 0.f;
     bool alive = true;
+    const uint32_t pair_bar = kPairBar + (warp & 3), tid = threadIdx.x;
+    auto chunk = [&](int row, int c) { return staging + row * 128 + ((c ^ (row & 7)) << 4); };
 
-    // the query row of a segment into TMEM; qscale: 1 / its scale, times the softmax's factor
-    auto load_query = [&](const Walk& w) {
-        const int R = w.qt * kTile + row;
-        const bool valid = R < w.r.n * g;
-        const char* p = static_cast<const char*>(a.q) +
-                        ((size_t)(w.r.lo + (valid ? R / g : 0)) * a.q_ld + (size_t)((a.head0 + w.head) * g + (valid ? R % g : 0)) * kDim) *
-                            (kF32 ? 4 : 2);
+    // The query rows of a segment into TMEM. A row is read by 8 threads, 16 bytes each, and turned into its halves
+    // there (qscale: 1 / its scale, times the softmax's factor); by way of shared memory, a quarter of the row at a
+    // time (bf16: a half), it comes to the threads of its lane.
+    auto load_query = [&](const Walk& w) __attribute__((always_inline)) {
+        constexpr int kElt = kF32 ? 4 : 2, kRounds = kF32 ? 4 : 2;
+        uint4 x[kRounds][4];
+        const int row8 = tid >> 3, c8 = tid & 7, rows = w.r.n * g - w.qt * kTile;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int rr = k * 32 + row8, R = w.qt * kTile + rr;
+            const char* p = static_cast<const char*>(a.q) +
+                            ((size_t)(w.r.lo + (rr < rows ? R / g : 0)) * a.q_ld +
+                             (size_t)((a.head0 + w.head) * g + (rr < rows ? R % g : 0)) * kDim) * kElt + c8 * 16;
+#pragma unroll
+            for (int i = 0; i < kRounds; ++i)
+                x[i][k] = rr < rows ? *reinterpret_cast<const uint4*>(p + i * 128) : make_uint4(0, 0, 0, 0);
+        }
         if constexpr (kF32) {
-            const float4* q4 = reinterpret_cast<const float4*>(p);
-            uint32_t m = 0;
-            if (valid) {
-#pragma unroll 8
-                for (int i = 0; i < 32; ++i) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(q4 + i);
-                    const uint32_t e[4] = {v.x & 0x7FFFFFFFu, v.y & 0x7FFFFFFFu, v.z & 0x7FFFFFFFu, v.w & 0x7FFFFFFFu};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) m = max(m, e[c] < 0x7F800000u ? e[c] : 0u);
-                }
-            }
-            const float up = a.scale < 0.f ? -scale_up(m) : scale_up(m);
-            qscale = scale_down(m) * factor;
+            for (int k = 0; k < 4; ++k) {
+                uint32_t m = 0;
+                auto take = [&](uint32_t e) {
+                    e &= 0x7FFFFFFFu;
+                    m = max(m, e < 0x7F800000u ? e : 0u);
+                };
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {  // 16 dimensions at a time
-                uint32_t hi[8], lo[8];
+                for (int i = 0; i < 4; ++i) take(x[i][k].x), take(x[i][k].y), take(x[i][k].z), take(x[i][k].w);
+#pragma unroll
+                for (int o = 4; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                // never 0: a hidden score is -inf times this
+                if (c8 == 0) s.qscale[k * 32 + row8] = fmaxf(scale_down(m) * factor, 1e-37f);
+                const float up = a.scale < 0.f ? -scale_up(m) : scale_up(m);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float4 v = valid ? q4[half * 16 + c * 4 + i] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    split2(v.x * up, v.y * up, hi[2 * i], lo[2 * i]);
-                    split2(v.z * up, v.w * up, hi[2 * i + 1], lo[2 * i + 1]);
+                    uint4 y;  // two words of hi halves, two of lo halves
+                    split2(__uint_as_float(x[i][k].x) * up, __uint_as_float(x[i][k].y) * up, y.x, y.z);
+                    split2(__uint_as_float(x[i][k].z) * up, __uint_as_float(x[i][k].w) * up, y.y, y.w);
+                    x[i][k] = y;
                 }
-                tmem_st<8>(lanes + kColQ + half * 32 + c * 8, hi);
-                tmem_st<8>(lanes + kColQ + 64 + half * 32 + c * 8, lo);
-            }
-        } else {
-            qscale = factor;
-            const uint4* q4 = reinterpret_cast<const uint4*>(p) + half * 8;
-            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t x[8];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint4 v = valid ? q4[c * 2 + i] : make_uint4(0, 0, 0, 0);
-                    x[4 * i] = v.x ^ flip, x[4 * i + 1] = v.y ^ flip, x[4 * i + 2] = v.z ^ flip, x[4 * i + 3] = v.w ^ flip;
-                }
-                tmem_st<8>(lanes + kColQ + half * 32 + c * 8, x);
             }
         }
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i) {
+            named_bar_sync(kTeamBar, 32 * kTeamWarps);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int rr = k * 32 + row8;
+                if constexpr (kF32) {  // chunks 0-3 of the row: hi halves, 4-7: lo halves
+                    *reinterpret_cast<uint2*>(chunk(rr, c8 >> 1) + (c8 & 1) * 8) = make_uint2(x[i][k].x, x[i][k].y);
+                    *reinterpret_cast<uint2*>(chunk(rr, 4 + (c8 >> 1)) + (c8 & 1) * 8) = make_uint2(x[i][k].z, x[i][k].w);
+                } else {
+                    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+                    *reinterpret_cast<uint4*>(chunk(rr, c8)) =
+                        make_uint4(x[i][k].x ^ flip, x[i][k].y ^ flip, x[i][k].z ^ flip, x[i][k].w ^ flip);
+                }
+            }
+            named_bar_sync(kTeamBar, 32 * kTeamWarps);
+            uint32_t y[16];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const uint4 v = *reinterpret_cast<const uint4*>(chunk(row, half * 4 + c));
+                y[4 * c] = v.x, y[4 * c + 1] = v.y, y[4 * c + 2] = v.z, y[4 * c + 3] = v.w;
+            }
+            const uint32_t to = lanes + kColQ + (kF32 ? half * 64 + i * 16 : i * 32 + half * 16);
+            tmem_st<8>(to, y);
+            tmem_st<8>(to + 8, y + 8);
+        }
+        qscale = kF32 ? s.qscale[row] : fmaxf(factor, 1e-37f);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.q_full);
     };
 
-    float acc[64];
+    uint64_t acc[32];  // 64 sums, in pairs
     float m = 0.f, l = 0.f, alpha = 1.f;
 
     // acc = acc * alpha + (P V of unit u), and the values of page t that were kept out of it
-    auto add_pv = [&](const Walk& w, uint32_t u, int t, bool live, int pos) {
+    auto add_pv = [&](const Walk& w, uint32_t u, int t, bool live, int pos) __attribute__((always_inline)) {
         if (alive && !wait(s, &s.pv_full, u & 1)) alive = false;
         if (alive && live) {
             tc_fence_after();
             const float f = kF32 ? s.vmeta[u & 7].scale : 1.f;
+            uint32_t x[64];
+            tmem_ld64(lanes + kColPv + half * 64, x);
+            const uint64_t a2 = pair(alpha, alpha), f2 = pair(f, f);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t x[16];
-                tmem_ld_32x32b_x16(lanes + kColPv + half * 64 + c * 16, x);
-                tmem_wait_ld16(x);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fmaf(acc[c * 16 + i], alpha, __uint_as_float(x[i]) * f);
+            for (int i = 0; i < 32; ++i) {
+                uint64_t v = pair(x[2 * i], x[2 * i + 1]);
+                acc[i] = fma2(acc[i], a2, kF32 ? mul2(v, f2) : v);
             }
             const uint4 vb = *reinterpret_cast<const uint4*>(s.vmeta[u & 7].bad);
             if (vb.x | vb.y | vb.z | vb.w) {
@@ -484,17 +529,98 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const ChunkParts& parts
                     if (!(s.vmeta[u & 7].bad[q >> 5] >> (q & 31) & 1)) continue;
                     const int r = t * kPageRows + q;
                     const bool seen = r <= pos && (a.window <= 0 || r > pos - a.window || r < w.r.prefix);
-                    float extra[64];
-                    for (int d = 0; d < 64; ++d) extra[d] = 0.f;
-                    add_bad_values<kF32>(a, w, t, q, seen, half, extra);
+                    if (!seen) continue;
+                    const char* p = value_row<kF32>(a, w, t, q) + half * (kF32 ? 256 : 128);
+                    auto odd = [](float v) { return odd_f32(__float_as_uint(v)) ? v : 0.f; };
 #pragma unroll
-                    for (int d = 0; d < 64; ++d) acc[d] += extra[d];
+                    for (int d = 0; d < 32; ++d) {
+                        float v0, v1;
+                        if constexpr (kF32) {
+                            const float2 v = reinterpret_cast<const float2*>(p)[d];
+                            v0 = v.x, v1 = v.y;
+                        } else {
+                            const uint32_t v = reinterpret_cast<const uint32_t*>(p)[d];
+                            v0 = bf16lo(v), v1 = bf16hi(v);
+                        }
+                        acc[d] = add2(acc[d], pair(odd(v0), odd(v1)));
+                    }
                 }
             }
             tc_fence_before();
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.pv_free);
+    };
+
+    // The scores of unit u to weights: the running maximum and sum, P in the scores' place; masked: the row does not
+    // see all of the page.
+    float alpha_next = 1.f;
+    bool run = false;
+    auto softmax = [&](const Walk& w, uint32_t u, uint32_t sa, bool masked, int pos, int c0) __attribute__((always_inline)) {
+        uint32_t x[64];
+        float top = -INFINITY;
+        if (run) {
+            tmem_ld64(sa, x);
+            if constexpr (kF32) {  // 1 / scale of each column's key
+                const float* ks = &s.kscale[u & 7][half * 64];
+#pragma unroll
+                for (int i = 0; i < 64; i += 4) {
+                    const float4 k4 = *reinterpret_cast<const float4*>(ks + i);
+                    unpair(mul2(pair(x[i], x[i + 1]), pair(k4.x, k4.y)), x[i], x[i + 1]);
+                    unpair(mul2(pair(x[i + 2], x[i + 3]), pair(k4.z, k4.w)), x[i + 2], x[i + 3]);
+                }
+            }
+            if (masked) {
+                asm volatile("");  // a branch, not 64 selects on every page
+                const int lo = a.window > 0 ? pos - a.window + 1 - c0 : -kPageRows;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t mask = seen_mask(half * 64 + c * 32, pos - c0, lo, w.r.prefix - c0);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (!(mask >> i & 1)) x[c * 32 + i] = 0xFF800000u;
+                }
+            }
+            float top2 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 64; i += 4) {
+                top = fmaxf(fmaxf(top, __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
+                top2 = fmaxf(fmaxf(top2, __uint_as_float(x[i + 2])), __uint_as_float(x[i + 3]));
+            }
+            top = fmaxf(top, top2) * qscale;
+        }
+        s.xmax[u & 1][half][row] = top;
+        named_bar_sync(pair_bar, 64);
+        top = fmaxf(top, s.xmax[u & 1][half ^ 1][row]);
+        const float mn = fmaxf(m, top);
+        alpha_next = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
+        m = mn;
+        const float shift = (mn == -INFINITY ? 0.f : mn) - (kF32 ? 14.f : 0.f);
+        if (run) {
+            const uint64_t q2 = pair(qscale, qscale), s2 = pair(-shift, -shift);
+            uint64_t sum2[2] = {0, 0};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t p0, p1;
+                    unpair(fma2(pair(x[c * 16 + 2 * i], x[c * 16 + 2 * i + 1]), q2, s2), p0, p1);
+                    const float e0 = exp2_fast(__uint_as_float(p0)), e1 = exp2_fast(__uint_as_float(p1));
+                    sum2[i & 1] = add2(sum2[i & 1], pair(e0, e1));
+                    if constexpr (kF32) split2(e0, e1, hi[i], lo[i]);
+                    else hi[i] = pack_bf16(e0, e1);
+                }
+                // in the place of the 16 scores just read
+                tmem_st<8>(sa + c * 16, hi);
+                if constexpr (kF32) tmem_st<8>(sa + c * 16 + 8, lo);
+            }
+            uint32_t u0, u1;
+            unpair(add2(sum2[0], sum2[1]), u0, u1);
+            l = l * alpha_next + (__uint_as_float(u0) + __uint_as_float(u1));
+            tmem_wait_st();
+            tc_fence_before();
+        }
     };
 
     Walk& w = s.walk[warp];
@@ -509,90 +635,19 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const ChunkParts& parts
         const bool live = (warp & 3) * 32 < rows;                           // this warp has some
         const int pos = w.r.start + R / g;
         m = -INFINITY, l = 0.f;
-        float alpha_next = 1.f;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) acc[i] = 0.f;
+        for (int i = 0; i < 32; ++i) acc[i] = 0;
         for (int j = 0; j < w.n; ++j) {
             const uint32_t u = unit0 + j, buf = u & 1;
             const int t = w.t.page(w.j + j), c0 = t * kPageRows;
             if (alive && !wait(s, &s.s_full[buf], (u >> 1) & 1)) alive = false;
             tc_fence_after();
+            run = alive && live;
             const uint32_t sa = lanes + kColS + buf * 128 + half * 64;
             // does every row of the tile see the whole page?
             const bool all = c0 + kPageRows - 1 <= w.t.first_pos &&
                              (a.window <= 0 || c0 > w.t.last_pos - a.window || c0 + kPageRows <= w.r.prefix);
-            uint32_t mask[2] = {0xffffffffu, 0xffffffffu};
-            if (!all) {
-                const int lo = a.window > 0 ? pos - a.window + 1 - c0 : -kPageRows;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) mask[c] = seen_mask(half * 64 + c * 32, pos - c0, lo, w.r.prefix - c0);
-            }
-            // 1 / scale of a column's keys
-            const float* ks = &s.kscale[u & 7][half * 64];
-            float top = -INFINITY;
-            if (alive && live) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[16];
-                    tmem_ld_32x32b_x16(sa + c * 16, x);
-                    tmem_wait_ld16(x);
-                    if (!all) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (!(mask[c >> 1] >> ((c & 1) * 16 + i) & 1)) x[i] = 0xFF800000u;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const float4 k4 = kF32 ? *reinterpret_cast<const float4*>(ks + c * 16 + i) : make_float4(1.f, 1.f, 1.f, 1.f);
-                        top = fmaxf(fmaxf(top, __uint_as_float(x[i]) * k4.x), __uint_as_float(x[i + 1]) * k4.y);
-                        top = fmaxf(fmaxf(top, __uint_as_float(x[i + 2]) * k4.z), __uint_as_float(x[i + 3]) * k4.w);
-                    }
-                }
-            }
-            top *= qscale;  // -inf * 0 (nothing seen, a query of zeros): NaN, which is no maximum
-            s.xmax[buf][half][row] = top;
-            named_bar_sync(kTeamBar, 32 * kTeamWarps);
-            top = fmaxf(top, s.xmax[buf][half ^ 1][row]);
-            const float mn = fmaxf(m, top);
-            alpha_next = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
-            m = mn;
-            const float shift = (mn == -INFINITY ? 0.f : mn) - (kF32 ? 14.f : 0.f);
-            if (alive && live) {
-                float sum = 0.f;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[16];
-                    tmem_ld_32x32b_x16(sa + c * 16, x);
-                    tmem_wait_ld16(x);
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const float4 k4 = kF32 ? *reinterpret_cast<const float4*>(ks + c * 16 + i) : make_float4(1.f, 1.f, 1.f, 1.f);
-                        const float kk[4] = {k4.x, k4.y, k4.z, k4.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float y = __uint_as_float(x[i + e]);
-                            y = fmaf(kF32 ? y * kk[e] : y, qscale, -shift);
-                            if (!all && !(mask[c >> 1] >> ((c & 1) * 16 + i + e) & 1)) y = -INFINITY;
-                            x[i + e] = __float_as_uint(exp2_fast(y));
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sum += __uint_as_float(x[i]);
-                    uint32_t hi[8], lo[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float p0 = __uint_as_float(x[2 * i]), p1 = __uint_as_float(x[2 * i + 1]);
-                        if constexpr (kF32) split2(p0, p1, hi[i], lo[i]);
-                        else hi[i] = pack_bf16(p0, p1);
-                    }
-                    // in the place of the 16 scores just read
-                    tmem_st<8>(sa + c * 16, hi);
-                    if constexpr (kF32) tmem_st<8>(sa + c * 16 + 8, lo);
-                }
-                l = l * alpha_next + sum;
-                tmem_wait_st();
-                tc_fence_before();
-            }
+            softmax(w, u, sa, !all, pos, c0);
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.p_full[buf]);
             if (j > 0) add_pv(w, u - 1, w.t.page(w.j + j - 1), live, pos);
@@ -607,30 +662,49 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const ChunkParts& parts
         if (more) load_query(w);  // every score of the finished segment has been read: its query is free
         add_pv(done, last, done.t.page(done.j + done.n - 1), live, pos);
         s.xsum[half][row] = l;
-        named_bar_sync(kTeamBar, 32 * kTeamWarps);
+        named_bar_sync(pair_bar, 64);
         const float total = s.xsum[0][row] + s.xsum[1][row];
+        named_bar_sync(pair_bar, 64);
         const bool mine = row < rows;
         if (!alive) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = NAN;
+            for (int i = 0; i < 32; ++i) acc[i] = pair(NAN, NAN);
         }
         if (done.whole()) {
-            if (mine) {
-                const float inv = 1.f / total;
-                const size_t at = ((size_t)(done.r.lo + R / g) * a.heads + (a.head0 + done.head) * g + R % g) * kDim + half * 64;
-                if constexpr (kF32) {
-                    float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.out) + at);
+            // rows of the tile to rows of out by way of shared memory: 64 bytes of each half a round
+            const float inv = 1.f / total;
+            const uint64_t inv2 = pair(inv, inv);
+            constexpr int kElt = kF32 ? 4 : 2, kRounds = kF32 ? 4 : 2;
+            const int row8 = tid >> 3, c8 = tid & 7;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        o[i] = make_float4(acc[4 * i] * inv, acc[4 * i + 1] * inv, acc[4 * i + 2] * inv, acc[4 * i + 3] * inv);
-                } else {
-                    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at);
+            for (int i = 0; i < kRounds; ++i) {
+                named_bar_sync(kTeamBar, 32 * kTeamWarps);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        o[i] = make_uint4(pack_bf16(acc[8 * i] * inv, acc[8 * i + 1] * inv),
-                                          pack_bf16(acc[8 * i + 2] * inv, acc[8 * i + 3] * inv),
-                                          pack_bf16(acc[8 * i + 4] * inv, acc[8 * i + 5] * inv),
-                                          pack_bf16(acc[8 * i + 6] * inv, acc[8 * i + 7] * inv));
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t y[8];
+                    uint4 v;
+                    if constexpr (kF32) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) unpair(mul2(acc[i * 8 + c * 2 + e], inv2), y[2 * e], y[2 * e + 1]);
+                        v = make_uint4(y[0], y[1], y[2], y[3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) unpair(mul2(acc[i * 16 + c * 4 + e], inv2), y[2 * e], y[2 * e + 1]);
+                        auto two = [&](int k) { return pack_bf16(__uint_as_float(y[k]), __uint_as_float(y[k + 1])); };
+                        v = make_uint4(two(0), two(2), two(4), two(6));
+                    }
+                    *reinterpret_cast<uint4*>(chunk(row, half * 4 + c)) = v;
+                }
+                named_bar_sync(kTeamBar, 32 * kTeamWarps);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int rr = k * 32 + row8, T = done.qt * kTile + rr;
+                    if (rr < rows)
+                        *reinterpret_cast<uint4*>(static_cast<char*>(a.out) +
+                                                  ((size_t)(done.r.lo + T / g) * a.heads + (a.head0 + done.head) * g + T % g) *
+                                                      (kDim * kElt) +
+                                                  (c8 >> 2) * (64 * kElt) + i * 64 + (c8 & 3) * 16) =
+                            *reinterpret_cast<const uint4*>(chunk(rr, c8));
                 }
             }
         } else {
@@ -638,7 +712,12 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const ChunkParts& parts
             float* part = parts.slots + ((size_t)blockIdx.x * 2 + slot) * slot_floats(kTile);
             if (mine) {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) part[(half * 64 + i) * kTile + row] = acc[i];
+                for (int i = 0; i < 32; ++i) {
+                    uint32_t y0, y1;
+                    unpair(acc[i], y0, y1);
+                    part[(half * 64 + 2 * i) * kTile + row] = __uint_as_float(y0);
+                    part[(half * 64 + 2 * i + 1) * kTile + row] = __uint_as_float(y1);
+                }
                 if (half == 0) {
                     part[kDim * kTile + row] = m;
                     part[(kDim + 1) * kTile + row] = total;
@@ -675,13 +754,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs 
     tc_fence_after();
     pdl_launch_dependents();
     if (warp < kTeamWarps) {
-        team_role<kF32>(a, s, parts, g);
-    } else if (warp == kTeamWarps) {
-        mma_role<kF32>(a, s, ring, g);
-    } else if ((threadIdx.x & 31) == 0) {
-        fence_proxy_async_smem();  // the ring was find_run's scratch
-        pdl_wait_prior_grid();
-        copy_role<kF32>(a, s, ring, im, g);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTeamRegs));
+        team_role<kF32>(a, s, ring + kStages<kF32> * kOperandBytes<kF32>, parts, g);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kTeamWarps) {
+            mma_role<kF32>(a, s, ring, g);
+        } else if (threadIdx.x == 32 * (kTeamWarps + 1)) {
+            fence_proxy_async_smem();  // the ring was find_run's scratch
+            pdl_wait_prior_grid();
+            copy_role<kF32>(a, s, ring, im, g);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -749,7 +832,7 @@ cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_
 
 template <bool kF32>
 cudaError_t launch(const ChunkArgs& a, const Images& im, const ChunkParts& parts, cudaStream_t st) {
-    const size_t smem = (size_t)kStages<kF32> * kOperandBytes<kF32> + 1024;
+    const size_t smem = (size_t)kStages<kF32> * kOperandBytes<kF32> + kStagingBytes + 1024;
     auto kernel = chunk_attention_kernel<kF32>;
     cudaError_t err = ensure_smem_optin(reinterpret_cast<const void*>(kernel), smem);
     if (err != cudaSuccess) return err;
