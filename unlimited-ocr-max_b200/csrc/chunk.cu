@@ -37,9 +37,10 @@ namespace uocr {
 namespace {
 
 constexpr int kTile = 128;      // (token, head) rows of a query tile
+constexpr int kLead = 6;        // what a tile costs beside its pages
 constexpr int kTeamWarps = 8;   // softmax; then a warpgroup of the issuing warp, the copying warp and two idle ones
 constexpr int kThreads = 32 * (kTeamWarps + 4);
-constexpr int kLaunchRegs = 168, kTeamRegs = 208, kOtherRegs = 88;  // a thread
+constexpr int kLaunchRegs = 168, kTeamRegs = 216, kOtherRegs = 72;  // a thread
 static_assert(kTeamWarps * kTeamRegs + 4 * kOtherRegs <= (kTeamWarps + 4) * kLaunchRegs, "a split of the launch's registers");
 // An operand: a page's 128 rows of k or of v of one head, as two blocks of 64 columns [128 rows][128 bytes]; fp32:
 // the lo halves behind the hi halves.
@@ -48,7 +49,7 @@ constexpr int kOperandBytes = kF32 ? 65536 : 32768;
 template <bool kF32>
 constexpr int kStages = kF32 ? 3 : 6;  // of operands in shared memory
 constexpr int kMaxStages = 6;
-constexpr uint32_t kTeamBar = 1, kPairBar = 2;  // all softmax warps; the two of 32 rows (kPairBar + 0..3)
+constexpr uint32_t kTeamBar = 1;
 constexpr int kStagingBytes = kTile * 128;  // a quarter (fp32) or half (bf16) of a tile's rows, between the row-wise and the
                                             // lane-wise order; 16-byte chunks swizzled by the row
 
@@ -76,12 +77,12 @@ struct Images {
 struct Shared {
     alignas(16) float kscale[8][kPageRows];  // by unit
     ValueMeta vmeta[8];
-    uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], p_full[2], pv_full, pv_free, q_full, drain;
+    uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], p_full[2], pv_full[2], pv_free[2], q_full, drain;
     uint32_t tmem;
     volatile int abort;
     Run run;
     Walk walk[kThreads / 32], done[kTeamWarps];
-    float xmax[2][2][kTile], xsum[2][kTile], qscale[kTile];
+    float xmax[2][kTile], xsum[2][kTile], qscale[kTile];
 };
 
 UOCR_DEV bool wait(Shared& s, uint64_t* bar, uint32_t parity) {
@@ -122,19 +123,6 @@ UOCR_DEV void tmem_st<8>(uint32_t addr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
-}
-// 64 columns into x, complete on return (the waits mark x as written by them: no use moves in front of them).
-UOCR_DEV void tmem_ld64(uint32_t addr, uint32_t (&x)[64]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]), "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31])
-                 : "r"(addr + 0));
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : "=r"(x[32]), "=r"(x[33]), "=r"(x[34]), "=r"(x[35]), "=r"(x[36]), "=r"(x[37]), "=r"(x[38]), "=r"(x[39]), "=r"(x[40]), "=r"(x[41]), "=r"(x[42]), "=r"(x[43]), "=r"(x[44]), "=r"(x[45]), "=r"(x[46]), "=r"(x[47]), "=r"(x[48]), "=r"(x[49]), "=r"(x[50]), "=r"(x[51]), "=r"(x[52]), "=r"(x[53]), "=r"(x[54]), "=r"(x[55]), "=r"(x[56]), "=r"(x[57]), "=r"(x[58]), "=r"(x[59]), "=r"(x[60]), "=r"(x[61]), "=r"(x[62]), "=r"(x[63])
-                 : "r"(addr + 32));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]), "+r"(x[9]), "+r"(x[10]), "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15]) : : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[16]), "+r"(x[17]), "+r"(x[18]), "+r"(x[19]), "+r"(x[20]), "+r"(x[21]), "+r"(x[22]), "+r"(x[23]), "+r"(x[24]), "+r"(x[25]), "+r"(x[26]), "+r"(x[27]), "+r"(x[28]), "+r"(x[29]), "+r"(x[30]), "+r"(x[31]) : : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[32]), "+r"(x[33]), "+r"(x[34]), "+r"(x[35]), "+r"(x[36]), "+r"(x[37]), "+r"(x[38]), "+r"(x[39]), "+r"(x[40]), "+r"(x[41]), "+r"(x[42]), "+r"(x[43]), "+r"(x[44]), "+r"(x[45]), "+r"(x[46]), "+r"(x[47]) : : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[48]), "+r"(x[49]), "+r"(x[50]), "+r"(x[51]), "+r"(x[52]), "+r"(x[53]), "+r"(x[54]), "+r"(x[55]), "+r"(x[56]), "+r"(x[57]), "+r"(x[58]), "+r"(x[59]), "+r"(x[60]), "+r"(x[61]), "+r"(x[62]), "+r"(x[63]) : : "memory");
 }
 // Two fp32 operations an instruction (each rounded as its scalar form).
 UOCR_DEV uint64_t pair(uint32_t x, uint32_t y) {
@@ -319,7 +307,7 @@ __device__ void copy_role(const ChunkArgs& a, Shared& s, unsigned char* ring, co
         return true;
     };
     auto run = [&] {
-        for (bool more = w.begin(a, s.run, g, kTile); more; more = w.next(a, g, kTile)) {
+        for (bool more = w.begin(a, s.run, g, kTile, kLead); more; more = w.next(a, g, kTile, kLead)) {
             const int n = w.n;
             for (int jj = 0; jj <= n; ++jj) {
                 if (jj < n && !copy(false, jj)) return false;
@@ -369,7 +357,7 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
     auto run = [&] {
         auto next = [&](bool first) {
             __syncwarp();
-            const bool more = first ? w.begin(a, s.run, g, kTile) : w.next(a, g, kTile);
+            const bool more = first ? w.begin(a, s.run, g, kTile, kLead) : w.next(a, g, kTile, kLead);
             __syncwarp();
             return more;
         };
@@ -386,9 +374,10 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
                 }
                 if (jj >= 1) {  // P V: 16 rows of V are 2048 bytes of both its blocks
                     const uint32_t u = unit0 + jj - 1;
-                    if (!wait(s, &s.p_full[u & 1], (u >> 1) & 1) || !wait(s, &s.pv_free, (u & 1) ^ 1)) return;
+                    if (!wait(s, &s.p_full[u & 1], (u >> 1) & 1)) return;
+                    if (u > 0 && !wait(s, &s.pv_free[(u - 1) & 1], ((u - 1) >> 1) & 1)) return;
                     if (!product(tmem + kColPv, tmem + kColS + (u & 1) * 128, 16, 8, kDescValues, 2048 >> 4, 8192 >> 4,
-                                 idesc<kF32>(true), &s.pv_full))
+                                 idesc<kF32>(true), &s.pv_full[u & 1]))
                         return;
                 }
             }
@@ -403,8 +392,9 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
 }
 
 // ---- the softmax warps ------------------------------------------------------------------------
-// Thread (row, half): row of the query tile (its TMEM lane), columns and dimensions [64 half, 64 half + 64).
-// Row `row` of the values of page t (this head's 128 columns).
+// Two teams of 4 warps take the pages of a segment in turn, a thread one row of the query tile (its TMEM lane)
+// with a maximum, a sum and 128 sums of its own; the teams' results are joined at the segment's end. While one
+// team waits for the tensor core the other one computes.
 template <bool kF32>
 UOCR_DEV const char* value_row(const ChunkArgs& a, const Walk& w, int t, int row) {
     constexpr int kElt = kF32 ? 4 : 2;
@@ -424,12 +414,12 @@ UOCR_DEV uint32_t seen_mask(int c0, int hi, int lo, int pre) {
 template <bool kF32>
 __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging, const ChunkParts& parts, int g) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int team = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = s.tmem + ((uint32_t)(warp & 3) << 21);  // lane field: bits 16 up, 32 lanes a warp
     const float factor = fabsf(a.scale) * kLog2e;  // the scale's sign is in the query operand
     float qscale = 0.f;
     bool alive = true;
-    const uint32_t pair_bar = kPairBar + (warp & 3), tid = threadIdx.x;
+    const uint32_t tid = threadIdx.x;
     auto chunk = [&](int row, int c) { return staging + row * 128 + ((c ^ (row & 7)) << 4); };
 
     // The query rows of a segment into TMEM. A row is read by 8 threads, 16 bytes each, and turned into its halves
@@ -492,10 +482,10 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
             uint32_t y[16];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const uint4 v = *reinterpret_cast<const uint4*>(chunk(row, half * 4 + c));
+                const uint4 v = *reinterpret_cast<const uint4*>(chunk(row, team * 4 + c));
                 y[4 * c] = v.x, y[4 * c + 1] = v.y, y[4 * c + 2] = v.z, y[4 * c + 3] = v.w;
             }
-            const uint32_t to = lanes + kColQ + (kF32 ? half * 64 + i * 16 : i * 32 + half * 16);
+            const uint32_t to = lanes + kColQ + (kF32 ? team * 64 + i * 16 : i * 32 + team * 16);
             tmem_st<8>(to, y);
             tmem_st<8>(to + 8, y + 8);
         }
@@ -506,228 +496,239 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
         if (lane == 0) mbar_arrive(&s.q_full);
     };
 
-    uint64_t acc[32];  // 64 sums, in pairs
-    float m = 0.f, l = 0.f, alpha = 1.f;
-
-    // acc = acc * alpha + (P V of unit u), and the values of page t that were kept out of it
-    auto add_pv = [&](const Walk& w, uint32_t u, int t, bool live, int pos) __attribute__((always_inline)) {
-        if (alive && !wait(s, &s.pv_full, u & 1)) alive = false;
-        if (alive && live) {
-            tc_fence_after();
-            const float f = kF32 ? s.vmeta[u & 7].scale : 1.f;
-            uint32_t x[64];
-            tmem_ld64(lanes + kColPv + half * 64, x);
-            const uint64_t a2 = pair(alpha, alpha), f2 = pair(f, f);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                uint64_t v = pair(x[2 * i], x[2 * i + 1]);
-                acc[i] = fma2(acc[i], a2, kF32 ? mul2(v, f2) : v);
-            }
-            const uint4 vb = *reinterpret_cast<const uint4*>(s.vmeta[u & 7].bad);
-            if (vb.x | vb.y | vb.z | vb.w) {
-                for (int q = 0; q < kPageRows; ++q) {
-                    if (!(s.vmeta[u & 7].bad[q >> 5] >> (q & 31) & 1)) continue;
-                    const int r = t * kPageRows + q;
-                    const bool seen = r <= pos && (a.window <= 0 || r > pos - a.window || r < w.r.prefix);
-                    if (!seen) continue;
-                    const char* p = value_row<kF32>(a, w, t, q) + half * (kF32 ? 256 : 128);
-                    auto odd = [](float v) { return odd_f32(__float_as_uint(v)) ? v : 0.f; };
-#pragma unroll
-                    for (int d = 0; d < 32; ++d) {
-                        float v0, v1;
-                        if constexpr (kF32) {
-                            const float2 v = reinterpret_cast<const float2*>(p)[d];
-                            v0 = v.x, v1 = v.y;
-                        } else {
-                            const uint32_t v = reinterpret_cast<const uint32_t*>(p)[d];
-                            v0 = bf16lo(v), v1 = bf16hi(v);
-                        }
-                        acc[d] = add2(acc[d], pair(odd(v0), odd(v1)));
-                    }
-                }
-            }
-            tc_fence_before();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.pv_free);
-    };
+    uint64_t acc[64];  // 128 sums, in pairs
+    float m = -INFINITY, l = 0.f, alpha = 1.f;
+    bool run = false;
 
     // The scores of unit u to weights: the running maximum and sum, P in the scores' place; masked: the row does not
     // see all of the page.
-    float alpha_next = 1.f;
-    bool run = false;
-    auto softmax = [&](const Walk& w, uint32_t u, uint32_t sa, bool masked, int pos, int c0) __attribute__((always_inline)) {
-        uint32_t x[64];
-        float top = -INFINITY;
-        if (run) {
-            tmem_ld64(sa, x);
-            if constexpr (kF32) {  // 1 / scale of each column's key
-                const float* ks = &s.kscale[u & 7][half * 64];
+    auto softmax = [&](const Walk& w, uint32_t u, bool masked, int pos, int c0) __attribute__((always_inline)) {
+        const uint32_t sa = lanes + kColS + (u & 1) * 128;
+        const int lo = a.window > 0 ? pos - a.window + 1 - c0 : -kPageRows;
+        uint32_t x[32];
+        auto scores = [&](int c) __attribute__((always_inline)) {  // 32 columns, times 1 / scale of each one's key
+            tmem_ld_32x32b_x32(sa + c * 32, x);
+            tmem_wait_ld_tie(x);
+            if constexpr (kF32) {
+                const float* ks = &s.kscale[u & 7][c * 32];
 #pragma unroll
-                for (int i = 0; i < 64; i += 4) {
+                for (int i = 0; i < 32; i += 4) {
                     const float4 k4 = *reinterpret_cast<const float4*>(ks + i);
                     unpair(mul2(pair(x[i], x[i + 1]), pair(k4.x, k4.y)), x[i], x[i + 1]);
                     unpair(mul2(pair(x[i + 2], x[i + 3]), pair(k4.z, k4.w)), x[i + 2], x[i + 3]);
                 }
             }
             if (masked) {
-                asm volatile("");  // a branch, not 64 selects on every page
-                const int lo = a.window > 0 ? pos - a.window + 1 - c0 : -kPageRows;
+                asm volatile("");  // a branch, not 32 selects on every page
+                const uint32_t mask = seen_mask(c * 32, pos - c0, lo, w.r.prefix - c0);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const uint32_t mask = seen_mask(half * 64 + c * 32, pos - c0, lo, w.r.prefix - c0);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (!(mask >> i & 1)) x[c * 32 + i] = 0xFF800000u;
-                }
+                for (int i = 0; i < 32; ++i)
+                    if (!(mask >> i & 1)) x[i] = 0xFF800000u;
             }
-            float top2 = -INFINITY;
+        };
+        float top = -INFINITY, top2 = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+            scores(c);
 #pragma unroll
-            for (int i = 0; i < 64; i += 4) {
+            for (int i = 0; i < 32; i += 4) {
                 top = fmaxf(fmaxf(top, __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
                 top2 = fmaxf(fmaxf(top2, __uint_as_float(x[i + 2])), __uint_as_float(x[i + 3]));
             }
-            top = fmaxf(top, top2) * qscale;
         }
-        s.xmax[u & 1][half][row] = top;
-        named_bar_sync(pair_bar, 64);
-        top = fmaxf(top, s.xmax[u & 1][half ^ 1][row]);
-        const float mn = fmaxf(m, top);
-        alpha_next = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
+        const float mn = fmaxf(m, fmaxf(top, top2) * qscale);
+        alpha = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
         m = mn;
         const float shift = (mn == -INFINITY ? 0.f : mn) - (kF32 ? 14.f : 0.f);
-        if (run) {
-            const uint64_t q2 = pair(qscale, qscale), s2 = pair(-shift, -shift);
-            uint64_t sum2[2] = {0, 0};
+        const uint64_t q2 = pair(qscale, qscale), s2 = pair(-shift, -shift);
+        uint64_t sum2[2] = {0, 0};
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+            scores(c);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int h = 0; h < 2; ++h) {
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     uint32_t p0, p1;
-                    unpair(fma2(pair(x[c * 16 + 2 * i], x[c * 16 + 2 * i + 1]), q2, s2), p0, p1);
+                    unpair(fma2(pair(x[h * 16 + 2 * i], x[h * 16 + 2 * i + 1]), q2, s2), p0, p1);
                     const float e0 = exp2_fast(__uint_as_float(p0)), e1 = exp2_fast(__uint_as_float(p1));
                     sum2[i & 1] = add2(sum2[i & 1], pair(e0, e1));
                     if constexpr (kF32) split2(e0, e1, hi[i], lo[i]);
                     else hi[i] = pack_bf16(e0, e1);
                 }
                 // in the place of the 16 scores just read
-                tmem_st<8>(sa + c * 16, hi);
-                if constexpr (kF32) tmem_st<8>(sa + c * 16 + 8, lo);
+                tmem_st<8>(sa + c * 32 + h * 16, hi);
+                if constexpr (kF32) tmem_st<8>(sa + c * 32 + h * 16 + 8, lo);
             }
-            uint32_t u0, u1;
-            unpair(add2(sum2[0], sum2[1]), u0, u1);
-            l = l * alpha_next + (__uint_as_float(u0) + __uint_as_float(u1));
-            tmem_wait_st();
-            tc_fence_before();
+        }
+        uint32_t u0, u1;
+        unpair(add2(sum2[0], sum2[1]), u0, u1);
+        l = l * alpha + (__uint_as_float(u0) + __uint_as_float(u1));
+        tmem_wait_st();
+        tc_fence_before();
+    };
+
+    // acc = acc * alpha + (P V of unit u), and the values of page t that were kept out of it
+    auto add_pv = [&](const Walk& w, uint32_t u, int t, int pos) __attribute__((always_inline)) {
+        const float f = kF32 ? s.vmeta[u & 7].scale : 1.f;
+        const uint64_t a2 = pair(alpha, alpha), f2 = pair(f, f);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            uint32_t x[32];
+            tmem_ld_32x32b_x32(lanes + kColPv + c * 32, x);
+            tmem_wait_ld_tie(x);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint64_t v = pair(x[2 * i], x[2 * i + 1]);
+                acc[c * 16 + i] = fma2(acc[c * 16 + i], a2, kF32 ? mul2(v, f2) : v);
+            }
+        }
+        tc_fence_before();
+        const uint4 vb = *reinterpret_cast<const uint4*>(s.vmeta[u & 7].bad);
+        if (vb.x | vb.y | vb.z | vb.w) {
+            for (int q = 0; q < kPageRows; ++q) {
+                if (!(s.vmeta[u & 7].bad[q >> 5] >> (q & 31) & 1)) continue;
+                const int r = t * kPageRows + q;
+                const bool seen = r <= pos && (a.window <= 0 || r > pos - a.window || r < w.r.prefix);
+                if (!seen) continue;
+                const char* p = value_row<kF32>(a, w, t, q);
+                auto odd = [](float v) { return odd_f32(__float_as_uint(v)) ? v : 0.f; };
+#pragma unroll
+                for (int d = 0; d < 64; ++d) {
+                    float v0, v1;
+                    if constexpr (kF32) {
+                        const float2 v = reinterpret_cast<const float2*>(p)[d];
+                        v0 = v.x, v1 = v.y;
+                    } else {
+                        const uint32_t v = reinterpret_cast<const uint32_t*>(p)[d];
+                        v0 = bf16lo(v), v1 = bf16hi(v);
+                    }
+                    acc[d] = add2(acc[d], pair(odd(v0), odd(v1)));
+                }
+            }
         }
     };
 
     Walk& w = s.walk[warp];
     Walk& done = s.done[warp];
-    bool more = w.begin(a, s.run, g, kTile);
+    bool more = w.begin(a, s.run, g, kTile, kLead);
     __syncwarp();
     int state[2] = {0, 0}, place[4] = {0, 0, 0, 0};
     uint32_t unit0 = 0;
-    if (more) load_query(w);
-    while (more) {
+    for (bool first = true; more; first = false) {
+        if (first) load_query(w);
         const int R = w.qt * kTile + row, rows = w.r.n * g - w.qt * kTile;  // valid rows of the tile
         const bool live = (warp & 3) * 32 < rows;                           // this warp has some
         const int pos = w.r.start + R / g;
         m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) acc[i] = 0;
-        for (int j = 0; j < w.n; ++j) {
-            const uint32_t u = unit0 + j, buf = u & 1;
+        for (int i = 0; i < 64; ++i) acc[i] = 0;
+        const int n = w.n, j0 = (team ^ unit0) & 1;  // this team's pages: units of its parity
+        for (int j = j0; j < n; j += 2) {
+            const uint32_t u = unit0 + j;
             const int t = w.t.page(w.j + j), c0 = t * kPageRows;
-            if (alive && !wait(s, &s.s_full[buf], (u >> 1) & 1)) alive = false;
+            if (alive && !wait(s, &s.s_full[u & 1], (u >> 1) & 1)) alive = false;
             tc_fence_after();
             run = alive && live;
-            const uint32_t sa = lanes + kColS + buf * 128 + half * 64;
             // does every row of the tile see the whole page?
             const bool all = c0 + kPageRows - 1 <= w.t.first_pos &&
                              (a.window <= 0 || c0 > w.t.last_pos - a.window || c0 + kPageRows <= w.r.prefix);
-            softmax(w, u, sa, !all, pos, c0);
+            if (run) softmax(w, u, !all, pos, c0);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s.p_full[buf]);
-            if (j > 0) add_pv(w, u - 1, w.t.page(w.j + j - 1), live, pos);
-            alpha = alpha_next;
+            if (lane == 0) mbar_arrive(&s.p_full[u & 1]);
+            if (j + 2 < n) {
+                if (alive && !wait(s, &s.pv_full[u & 1], (u >> 1) & 1)) alive = false;
+                tc_fence_after();
+                if (alive && live) add_pv(w, u, t, pos);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.pv_free[u & 1]);
+            }
         }
-        const uint32_t last = unit0 + w.n - 1;
-        unit0 += w.n;
+        // both teams have read the segment's scores (load_query's first barrier): its query makes room for the next
+        const uint32_t last = unit0 + (n - 1 - ((n - 1 - j0) & 1));  // this team's last unit, if n > j0
+        unit0 += n;
         done = w;
         __syncwarp();
-        more = w.next(a, g, kTile);
+        more = w.next(a, g, kTile, kLead);
         __syncwarp();
-        if (more) load_query(w);  // every score of the finished segment has been read: its query is free
-        add_pv(done, last, done.t.page(done.j + done.n - 1), live, pos);
-        s.xsum[half][row] = l;
-        named_bar_sync(pair_bar, 64);
-        const float total = s.xsum[0][row] + s.xsum[1][row];
-        named_bar_sync(pair_bar, 64);
-        const bool mine = row < rows;
-        if (!alive) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) acc[i] = pair(NAN, NAN);
+        if (more) load_query(w);
+        if (n > j0) {
+            if (alive && !wait(s, &s.pv_full[last & 1], (last >> 1) & 1)) alive = false;
+            tc_fence_after();
+            if (alive && live) add_pv(done, last, done.t.page(done.j + (int)(last + n - unit0)), pos);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.pv_free[last & 1]);
         }
-        if (done.whole()) {
-            // rows of the tile to rows of out by way of shared memory: 64 bytes of each half a round
-            const float inv = 1.f / total;
-            const uint64_t inv2 = pair(inv, inv);
-            constexpr int kElt = kF32 ? 4 : 2, kRounds = kF32 ? 4 : 2;
-            const int row8 = tid >> 3, c8 = tid & 7;
+        // the two teams' results: out = (f0 acc0 + f1 acc1) / (f0 l0 + f1 l1), f = 2^(m - max m)
+        s.xmax[team][row] = m, s.xsum[team][row] = l;
+        named_bar_sync(kTeamBar, 32 * kTeamWarps);
+        const float M = fmaxf(m, s.xmax[team ^ 1][row]);
+        auto weight = [&](float mt) { return mt == -INFINITY ? 0.f : exp2_fast(mt - M); };
+        const float total = s.xsum[0][row] * weight(s.xmax[0][row]) + s.xsum[1][row] * weight(s.xmax[1][row]);
+        const bool whole = done.whole();
+        float f = m == -INFINITY && l == 0.f ? 0.f : weight(m);
+        if (whole) f *= 1.f / total;
+        if (!alive) f = NAN;
+        const uint64_t f2 = pair(f, f);
+        const int slot = done.j == 0 ? 1 : 0;
+        float* part = parts.slots + ((size_t)blockIdx.x * 2 + slot) * slot_floats(kTile);
+        constexpr int kElt = kF32 ? 4 : 2;
+        const int row8 = tid >> 3, c8 = tid & 7;
 #pragma unroll
-            for (int i = 0; i < kRounds; ++i) {
-                named_bar_sync(kTeamBar, 32 * kTeamWarps);
+        for (int i = 0; i < 4; ++i) {  // 32 columns a round, by way of shared memory: team 1's part, then the sums
+            if (team == 1) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t y[8];
+                for (int c = 0; c < 8; ++c) {
                     uint4 v;
-                    if constexpr (kF32) {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) unpair(mul2(acc[i * 8 + c * 2 + e], inv2), y[2 * e], y[2 * e + 1]);
-                        v = make_uint4(y[0], y[1], y[2], y[3]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) unpair(mul2(acc[i * 16 + c * 4 + e], inv2), y[2 * e], y[2 * e + 1]);
-                        auto two = [&](int k) { return pack_bf16(__uint_as_float(y[k]), __uint_as_float(y[k + 1])); };
-                        v = make_uint4(two(0), two(2), two(4), two(6));
-                    }
-                    *reinterpret_cast<uint4*>(chunk(row, half * 4 + c)) = v;
+                    unpair(mul2(acc[i * 16 + 2 * c], f2), v.x, v.y);
+                    unpair(mul2(acc[i * 16 + 2 * c + 1], f2), v.z, v.w);
+                    *reinterpret_cast<uint4*>(chunk(row, c)) = v;
                 }
-                named_bar_sync(kTeamBar, 32 * kTeamWarps);
+            }
+            named_bar_sync(kTeamBar, 32 * kTeamWarps);
+            if (team == 0) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    uint4 v = *reinterpret_cast<const uint4*>(chunk(row, c));
+                    unpair(fma2(acc[i * 16 + 2 * c], f2, pair(v.x, v.y)), v.x, v.y);
+                    unpair(fma2(acc[i * 16 + 2 * c + 1], f2, pair(v.z, v.w)), v.z, v.w);
+                    if (whole) {
+                        *reinterpret_cast<uint4*>(chunk(row, c)) = v;
+                    } else if (row < rows) {
+                        float* o = part + (i * 32 + c * 4) * kTile + row;
+                        o[0] = __uint_as_float(v.x), o[kTile] = __uint_as_float(v.y);
+                        o[2 * kTile] = __uint_as_float(v.z), o[3 * kTile] = __uint_as_float(v.w);
+                    }
+                }
+            }
+            named_bar_sync(kTeamBar, 32 * kTeamWarps);
+            if (whole) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int rr = k * 32 + row8, T = done.qt * kTile + rr;
-                    if (rr < rows)
-                        *reinterpret_cast<uint4*>(static_cast<char*>(a.out) +
-                                                  ((size_t)(done.r.lo + T / g) * a.heads + (a.head0 + done.head) * g + T % g) *
-                                                      (kDim * kElt) +
-                                                  (c8 >> 2) * (64 * kElt) + i * 64 + (c8 & 3) * 16) =
-                            *reinterpret_cast<const uint4*>(chunk(rr, c8));
+                    if (rr >= rows) continue;
+                    const uint4 v = *reinterpret_cast<const uint4*>(chunk(rr, c8));
+                    char* o = static_cast<char*>(a.out) +
+                              (((size_t)(done.r.lo + T / g) * a.heads + (a.head0 + done.head) * g + T % g) * kDim + i * 32 + c8 * 4) * kElt;
+                    if constexpr (kF32) *reinterpret_cast<uint4*>(o) = v;
+                    else *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(__uint_as_float(v.x), __uint_as_float(v.y)),
+                                                                   pack_bf16(__uint_as_float(v.z), __uint_as_float(v.w)));
                 }
             }
-        } else {
-            const int slot = done.j == 0 ? 1 : 0;
-            float* part = parts.slots + ((size_t)blockIdx.x * 2 + slot) * slot_floats(kTile);
-            if (mine) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    uint32_t y0, y1;
-                    unpair(acc[i], y0, y1);
-                    part[(half * 64 + 2 * i) * kTile + row] = __uint_as_float(y0);
-                    part[(half * 64 + 2 * i + 1) * kTile + row] = __uint_as_float(y1);
-                }
-                if (half == 0) {
-                    part[kDim * kTile + row] = m;
-                    part[(kDim + 1) * kTile + row] = total;
-                }
+            named_bar_sync(kTeamBar, 32 * kTeamWarps);
+        }
+        if (!whole) {
+            if (team == 0 && row < rows) {
+                part[kDim * kTile + row] = M;
+                part[(kDim + 1) * kTile + row] = total;
             }
             state[slot] = slot == 0 && done.j + done.n == done.t.count ? 2 : 1;
-            if (slot == 1) place[0] = done.r.lo, place[1] = done.qt * kTile, place[2] = min(rows, kTile), place[3] = a.head0 + done.head;
+            if (slot == 1)
+                place[0] = done.r.lo, place[1] = done.qt * kTile, place[2] = min(rows, kTile), place[3] = a.head0 + done.head;
         }
     }
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         int* o = parts.info + blockIdx.x * kInfoInts;
         o[0] = state[0], o[1] = state[1];
         for (int i = 0; i < 4; ++i) o[2 + i] = place[i];
@@ -743,14 +744,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs 
     const int g = a.heads / a.kv_heads;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&s.s_full[i], 1), mbar_init(&s.p_full[i], kTeamWarps);
-        mbar_init(&s.pv_full, 1), mbar_init(&s.pv_free, kTeamWarps), mbar_init(&s.q_full, kTeamWarps), mbar_init(&s.drain, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&s.s_full[i], 1), mbar_init(&s.p_full[i], kTeamWarps / 2), mbar_init(&s.pv_full[i], 1),
+                                    mbar_init(&s.pv_free[i], kTeamWarps / 2);
+        mbar_init(&s.q_full, kTeamWarps), mbar_init(&s.drain, 1);
         fence_mbar_init();
         s.abort = 0;
     }
     if (warp == kTeamWarps) tmem_alloc(&s.tmem, 512);
     tc_fence_before();
-    find_run(a, s.run, reinterpret_cast<long long*>(ring), g, kTile);
+    find_run(a, s.run, reinterpret_cast<long long*>(ring), g, kTile, kLead);
     tc_fence_after();
     pdl_launch_dependents();
     if (warp < kTeamWarps) {

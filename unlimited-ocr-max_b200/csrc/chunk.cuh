@@ -63,35 +63,39 @@ UOCR_DEV Tile tile_at(const ChunkArgs& a, const Request& r, int qt, int g, int t
     return t;
 }
 
-// A CTA's run: its units, and where they begin (heads are counted from the pass's first).
+// A CTA's run of the call's work: its length, and where it begins (heads are counted from the pass's first). Work is
+// counted in pages; a tile and head counts `lead` more in front of its pages, for what a CTA does once for it
+// (its queries, its results), so that a run of many short tiles takes no longer than one of a few long ones.
 struct Run {
-    int left, b, qt, head, j;
+    int left, b, qt, head, x;
 };
 
 // The walk over a CTA's units, a segment (pages of one tile and head) at a time; every warp walks by
 // itself.
 struct Walk {
     int b, qt, head, j, n, tiles;  // segment: pages j .. j + n - 1 of the tile's
-    int left;                      // units behind this segment
+    int left;                      // of the run, behind this segment
     Request r;
     Tile t;
-    UOCR_DEV void enter(const ChunkArgs& a, int g, int tile) {
+    // at x of the segment's tile and head; false: the run ends in front of its pages
+    UOCR_DEV bool enter(const ChunkArgs& a, int g, int tile, int lead, int x) {
         t = tile_at(a, r, qt, g, tile);
-        n = min(t.count - j, left);
-        left -= n;
+        const int end = min(x + left, t.count + lead);
+        j = max(x - lead, 0);
+        n = max(end - lead, 0) - j;
+        left -= end - x;
+        return n > 0;
     }
-    UOCR_DEV bool begin(const ChunkArgs& a, const Run& s, int g, int tile) {
+    UOCR_DEV bool begin(const ChunkArgs& a, const Run& s, int g, int tile, int lead) {
         left = s.left;
         if (left <= 0) return false;
-        b = s.b, qt = s.qt, head = s.head, j = s.j;
+        b = s.b, qt = s.qt, head = s.head;
         r = request_at(a, b);
         tiles = (r.n * g + tile - 1) / tile;
-        enter(a, g, tile);
-        return true;
+        return enter(a, g, tile, lead, s.x);
     }
-    UOCR_DEV bool next(const ChunkArgs& a, int g, int tile) {
+    UOCR_DEV bool next(const ChunkArgs& a, int g, int tile, int lead) {
         if (left <= 0) return false;
-        j = 0;
         if (++head == a.pass_heads) {
             head = 0;
             if (++qt >= tiles) {
@@ -103,8 +107,7 @@ struct Walk {
                 tiles = (r.n * g + tile - 1) / tile;
             }
         }
-        enter(a, g, tile);
-        return true;
+        return enter(a, g, tile, lead, 0);
     }
     UOCR_DEV bool whole() const { return j == 0 && n == t.count; }
 };
@@ -120,13 +123,13 @@ UOCR_DEV T warp_scan(T v, int lane) {  // inclusive
 }
 
 // All threads: this CTA's run of units. scratch: B long longs of shared memory.
-__device__ __noinline__ void find_run(const ChunkArgs& a, Run& run, long long* scratch, int g, int tile) {
+__device__ __noinline__ void find_run(const ChunkArgs& a, Run& run, long long* scratch, int g, int tile, int lead) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int b = warp; b < a.B; b += blockDim.x / 32) {
         const Request r = request_at(a, b);
         const int tiles = (r.n * g + tile - 1) / tile;
         long long sum = 0;
-        for (int qt = lane; qt < tiles; qt += 32) sum += tile_at(a, r, qt, g, tile).count;
+        for (int qt = lane; qt < tiles; qt += 32) sum += tile_at(a, r, qt, g, tile).count + lead;
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) scratch[b] = sum * a.pass_heads;
@@ -159,13 +162,13 @@ __device__ __noinline__ void find_run(const ChunkArgs& a, Run& run, long long* s
             const Request r = request_at(a, b);
             const int tiles = (r.n * g + tile - 1) / tile;
             for (int q0 = 0; q0 < tiles; q0 += 32) {
-                const int count = q0 + lane < tiles ? tile_at(a, r, q0 + lane, g, tile).count : 0;
+                const int count = q0 + lane < tiles ? tile_at(a, r, q0 + lane, g, tile).count + lead : 0;
                 const long long upto = before + warp_scan((long long)count * a.pass_heads, lane);
                 const uint32_t hit = __ballot_sync(0xffffffffu, upto > u0);
                 if (hit) {
                     if (lane == __ffs(hit) - 1) {
                         const long long in = u0 - (upto - (long long)count * a.pass_heads);
-                        run.b = b, run.qt = q0 + lane, run.head = (int)(in / count), run.j = (int)(in % count);
+                        run.b = b, run.qt = q0 + lane, run.head = (int)(in / count), run.x = (int)(in % count);
                     }
                     break;
                 }
