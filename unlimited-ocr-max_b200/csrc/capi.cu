@@ -312,7 +312,7 @@ int uocr_paged_decode_attention(const float* q, const float* k_new, const float*
 
 size_t uocr_paged_chunk_workspace_bytes(int64_t T, int64_t heads, int64_t kv_heads, int dtype, int64_t lut_cols, int64_t B) {
     if (T < 1 || B < 1 || B > uocr::kChunkMaxRequests || heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 1024 ||
-        T > (int64_t(1) << 30) / (heads / kv_heads) || lut_cols < 1 || lut_cols > (1 << 22) ||
+        T > (int64_t(1) << 30) / (heads / kv_heads) || lut_cols < 1 || lut_cols > (1 << 22) || B * lut_cols > (int64_t(1) << 30) ||
         (dtype != UOCR_DTYPE_F32 && dtype != UOCR_DTYPE_BF16))
         return 0;
     uocr::ChunkArgs a{};
@@ -344,6 +344,9 @@ int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, i
         lut_cols < 1 || lut_cols > (1 << 22))
         return fail(UOCR_EINVAL, "paged_chunk_attention: bad pool (pages %lld, layers %lld, layer %lld, lut_cols %lld)",
                     (long long)pages, (long long)layers, (long long)layer, (long long)lut_cols);
+    if (B * lut_cols > (int64_t(1) << 30))
+        return fail(UOCR_EUNSUPPORTED, "paged_chunk_attention: tables of %lld x %lld pages (this build: <= 2^30)", (long long)B,
+                    (long long)lut_cols);
     // a CTA counts its (query tile, head, page) units in 32 bits
     if ((T * (heads / kv_heads) / 128 + B) * kv_heads > (int64_t(1) << 38) / (lut_cols + T / 128 + 2))
         return fail(UOCR_EUNSUPPORTED, "paged_chunk_attention: T %lld over %lld pages a request is too much for one call",

@@ -56,33 +56,48 @@ constexpr int kStagingBytes = kTile * 128;  // a quarter (fp32) or half (bf16) o
 // TMEM columns
 constexpr uint32_t kColS = 0, kColPv = 256, kColQ = 384;
 
-// Beside a page's operands: 1 / scale of each row of k; of v, and which rows of it are not finite.
+// Beside a page's operands. Keys: 1 / scale of each row, and of all of them where they share one scale (else 0).
+// Values: 1 / scale, and which rows are not finite.
+struct alignas(16) KeyMeta {
+    float scale[kPageRows];
+    float all;
+    float pad[3];
+};
 struct alignas(16) ValueMeta {
     float scale;
     float pad[3];
     uint32_t bad[4];
 };
 struct alignas(16) PageMeta {
-    float kscale[kPageRows];
+    KeyMeta k;
     ValueMeta v;
 };
 
-// The operands of a pass, made by the first launch: page `p` of request b and head h (of the pass) at
-// index (b * lut_cols + p) * pass_heads + h: k, then v.
+// The operands of a pass, made by the first launch. Keys and values: page p of request b and head h (of the pass)
+// at index (b * lut_cols + p) * pass_heads + h, k, then v. Queries: tile t of request b at index
+// (query_base(b) + t) * pass_heads + h, 16 bytes of row r at (group * 128 + r) * 16 bytes as TMEM takes them (fp32: hi
+// halves in groups 0 to 15, lo halves in 16 to 31; bf16: 16 groups), and each row's 1 / scale times the
+// softmax's factor.
 struct Images {
     unsigned char* operands;
     PageMeta* meta;
+    unsigned char* queries;
+    float* qscale;
 };
+template <bool kF32>
+constexpr int kQueryBytes = kTile * kDim * (kF32 ? 4 : 2);
+// Tiles of the requests in front of b fit below: floor(x + y) + 1 >= floor(x) + ceil(y).
+UOCR_DEV int query_base(const Request& r, int b, int g) { return r.lo * g / kTile + b; }
 
 struct Shared {
-    alignas(16) float kscale[8][kPageRows];  // by unit
+    KeyMeta kmeta[8];  // by unit
     ValueMeta vmeta[8];
     uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], p_full[2], pv_full[2], pv_free[2], q_full, drain;
     uint32_t tmem;
     volatile int abort;
     Run run;
-    Walk walk[kThreads / 32], done[kTeamWarps];
-    float xmax[2][kTile], xsum[2][kTile], qscale[kTile];
+    Walk walk[kThreads / 32], now[kTeamWarps];
+    float xmax[2][kTile], xsum[2][kTile];
 };
 
 UOCR_DEV bool wait(Shared& s, uint64_t* bar, uint32_t parity) {
@@ -99,11 +114,6 @@ UOCR_DEV void umma_ts_f16(uint32_t d, uint32_t a, uint32_t desc_lo, uint32_t des
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
         "r"(a), "r"(desc_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
         : "memory");
-}
-UOCR_DEV bool elect_one() {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
-    return ok != 0;
 }
 // Shared-memory descriptors, 128-byte swizzle: 8-row groups 1024 bytes apart (the upper word); keys K-major (the
 // leading stride is not used), values MN-major, their 64-column blocks 16 KB apart.
@@ -169,14 +179,69 @@ UOCR_DEV uint32_t top_of(const uint4& x) {
     return max(max(x.x & 0x7FFFFFFFu, x.y & 0x7FFFFFFFu), max(x.z & 0x7FFFFFFFu, x.w & 0x7FFFFFFFu));
 }
 
-// A CTA per (page, head, request): its rows of k and v become operands, and its new rows are stored in the
-// pool. A warp takes 16 rows; a word (16 bytes of a thread) is one row of fp32 or two of bf16. Bound: HBM.
+// A query tile of head `head` (of the pass): 128 rows of q. A warp takes 16 rows.
+template <bool kF32>
+UOCR_DEV void query_operand(const ChunkArgs& a, const Images& im, int f, int head) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = a.heads / a.kv_heads;
+    int b = 0;
+    for (int hi = a.B - 1; b < hi;) {  // the last request whose tiles begin at f or below
+        const int mid = (b + hi + 1) / 2;
+        if (query_base(request_at(a, mid), mid, g) <= f) b = mid; else hi = mid - 1;
+    }
+    const Request r = request_at(a, b);
+    const int qt = f - query_base(r, b, g), rows = r.n * g - qt * kTile;
+    if (qt < 0 || rows <= 0) return;
+    const size_t index = (size_t)f * a.pass_heads + head;
+    unsigned char* out = im.queries + index * kQueryBytes<kF32>;
+    const float factor = fabsf(a.scale) * kLog2e;  // the scale's sign goes into the operand
+    constexpr int kElt = kF32 ? 4 : 2, kPer = kF32 ? 1 : 2, kWords = 16 / kPer;
+    uint4 x[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+        const int row = warp * 16 + i * kPer + (kF32 ? 0 : lane >> 4), R = qt * kTile + row;
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (row < rows)
+            x[i] = ldg_nc_v4(static_cast<const char*>(a.q) +
+                             ((r.lo + R / g) * a.q_ld + (size_t)((a.head0 + head) * g + R % g) * kDim) * kElt +
+                             (kF32 ? lane : lane & 15) * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+        const int row = warp * 16 + i * kPer + (kF32 ? 0 : lane >> 4);
+        if constexpr (kF32) {
+            auto finite = [](uint32_t e) { return (e & 0x7FFFFFFFu) < 0x7F800000u ? e & 0x7FFFFFFFu : 0u; };
+            const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(finite(x[i].x), finite(x[i].y)), max(finite(x[i].z), finite(x[i].w))));
+            const float up = a.scale < 0.f ? -scale_up(top) : scale_up(top);
+            uint2 hi, lo;
+            split2(__uint_as_float(x[i].x) * up, __uint_as_float(x[i].y) * up, hi.x, lo.x);
+            split2(__uint_as_float(x[i].z) * up, __uint_as_float(x[i].w) * up, hi.y, lo.y);
+            unsigned char* at = out + ((lane >> 1) * kTile + row) * 16 + (lane & 1) * 8;
+            *reinterpret_cast<uint2*>(at) = hi;
+            *reinterpret_cast<uint2*>(at + 16 * kTile * 16) = lo;
+            // never 0: a hidden score is -inf times this
+            if (lane == 0) im.qscale[index * kTile + row] = fmaxf(scale_down(top) * factor, 1e-37f);
+        } else {
+            const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+            *reinterpret_cast<uint4*>(out + ((lane & 15) * kTile + row) * 16) =
+                make_uint4(x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip);
+            if ((lane & 15) == 0) im.qscale[index * kTile + row] = fmaxf(factor, 1e-37f);
+        }
+    }
+}
+
+// A CTA per page (of a request's table) and head, then per query tile and head. Pages: their rows of k and v become
+// operands, and their new rows are stored in the pool. A warp takes 16 rows; a word (16 bytes of a thread) is one
+// row of fp32 or two of bf16. Bound: HBM.
 template <bool kF32>
 __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Images im) {
     pdl_launch_dependents();
     constexpr int kElt = kF32 ? 4 : 2, kPer = kF32 ? 1 : 2, kWords = 16 / kPer;
     __shared__ uint32_t tops[8], bads[8];
-    const int page = blockIdx.x, b = blockIdx.z, head = a.head0 + blockIdx.y;
+    if (blockIdx.x >= (unsigned)(a.B * a.lut_cols)) {
+        query_operand<kF32>(a, im, blockIdx.x - a.B * a.lut_cols, blockIdx.y);
+        return;
+    }
+    const int b = blockIdx.x / a.lut_cols, page = blockIdx.x % a.lut_cols, head = a.head0 + blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = a.heads / a.kv_heads;
     const Request r = request_at(a, b);
     if (r.n == 0) return;
@@ -210,6 +275,7 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
             }
         }
         float up = 1.f;
+        uint32_t my_top = 0, page_top = 0;  // fp32, k: lane i has the largest magnitude of row i
         if (v) {
             // values that are not finite leave the operand; fp32: one scale for the page, whose rows are summed over
             uint32_t top = 0, bad = 0;
@@ -240,6 +306,7 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
                 }
                 if (kF32) top = __reduce_max_sync(0xffffffffu, top);
             }
+            __syncthreads();  // tops may still be read
             if (lane == 0) tops[warp] = top, bads[warp] = bad;
             __syncthreads();
             if (kF32) {
@@ -248,27 +315,39 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
                 if (threadIdx.x == 0) meta.v.scale = scale_down(top);
             }
             if (threadIdx.x < 4) meta.v.bad[threadIdx.x] = bads[2 * threadIdx.x] | bads[2 * threadIdx.x + 1] << 16;
+        } else if (kF32) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                uint32_t top = __reduce_max_sync(0xffffffffu, top_of(x[i]));
+                if (top >= 0x7F800000u) {  // rare: the row's scores become NaN; it sets no scale
+                    uint32_t m = 0;
+                    auto mark = [&](uint32_t& e) {
+                        if (odd_f32(e)) e = 0x7FFFFFFFu;
+                        else m = max(m, e & 0x7FFFFFFFu);
+                    };
+                    mark(x[i].x), mark(x[i].y), mark(x[i].z), mark(x[i].w);
+                    top = __reduce_max_sync(0xffffffffu, m);
+                }
+                if (lane == i) my_top = top;
+            }
+            page_top = __reduce_max_sync(0xffffffffu, my_top);
+            if (lane == 0) tops[warp] = page_top;
+            __syncthreads();
+            page_top = __reduce_max_sync(0xffffffffu, tops[lane & 7]);
+            // A row within 2^10 of the page's largest takes the page's scale (its halves still hold 2^-29 of it);
+            // others have their own.
+            const bool near = my_top == 0 || (my_top >> 23) + 10 >= page_top >> 23;
+            if (near) my_top = page_top;
+            const bool all = __syncthreads_and(near || lane >= 16);
+            if (lane < 16) meta.k.scale[warp * 16 + lane] = scale_down(my_top);
+            if (threadIdx.x == 0) meta.k.all = all ? scale_down(page_top) : 0.f;
         }
         unsigned char* out = im.operands + (index * 2 + v) * kOperandBytes<kF32>;
-        uint32_t my_top = 0;  // lane i: the largest magnitude of row i of k
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
             const int row = row0 + i * kPer;
             if constexpr (kF32) {
-                if (!v) {
-                    uint32_t top = __reduce_max_sync(0xffffffffu, top_of(x[i]));
-                    if (top >= 0x7F800000u) {  // rare: its scores become NaN; it sets no scale
-                        uint32_t m = 0;
-                        auto mark = [&](uint32_t& e) {
-                            if (odd_f32(e)) e = 0x7FFFFFFFu;
-                            else m = max(m, e & 0x7FFFFFFFu);
-                        };
-                        mark(x[i].x), mark(x[i].y), mark(x[i].z), mark(x[i].w);
-                        top = __reduce_max_sync(0xffffffffu, m);
-                    }
-                    if (lane == i) my_top = top;
-                    up = scale_up(top);
-                }
+                if (!v) up = scale_up(__shfl_sync(0xffffffffu, my_top, i));
                 uint2 hi, lo;
                 split2(__uint_as_float(x[i].x) * up, __uint_as_float(x[i].y) * up, hi.x, lo.x);
                 split2(__uint_as_float(x[i].z) * up, __uint_as_float(x[i].w) * up, hi.y, lo.y);
@@ -280,7 +359,6 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
                 *reinterpret_cast<uint4*>(out + ((lane >> 3) & 1) * 16384 + row * 128 + (((lane & 7) ^ (row & 7)) << 4)) = x[i];
             }
         }
-        if (kF32 && !v && lane < 16) meta.kscale[warp * 16 + lane] = scale_down(my_top);
     }
 }
 
@@ -296,12 +374,12 @@ __device__ void copy_role(const ChunkArgs& a, Shared& s, unsigned char* ring, co
         const uint32_t u = (unit0 + j) & 7;
         const PageMeta& meta = im.meta[index];
         if (!mbar_wait(&s.empty[stage], phase ^ 1, nullptr)) return false;
-        const uint32_t extra = v ? sizeof(ValueMeta) : kF32 ? sizeof(meta.kscale) : 0;
+        const uint32_t extra = v ? sizeof(ValueMeta) : kF32 ? sizeof(KeyMeta) : 0;
         mbar_arrive_expect_tx(&s.full[stage], kOperandBytes<kF32> + extra);
         bulk_g2s(ring + stage * kOperandBytes<kF32>, im.operands + (index * 2 + v) * kOperandBytes<kF32>, kOperandBytes<kF32>,
                  &s.full[stage]);
         if (v) bulk_g2s(&s.vmeta[u], &meta.v, sizeof(ValueMeta), &s.full[stage]);
-        else if (kF32) bulk_g2s(s.kscale[u], meta.kscale, sizeof(meta.kscale), &s.full[stage]);
+        else if (kF32) bulk_g2s(&s.kmeta[u], &meta.k, sizeof(KeyMeta), &s.full[stage]);
         ++issued;
         if (++stage == kStages<kF32>) stage = 0, phase ^= 1;
         return true;
@@ -326,45 +404,42 @@ __device__ void copy_role(const ChunkArgs& a, Shared& s, unsigned char* ring, co
 }
 
 // ---- the issuing warp -------------------------------------------------------------------------
+// One thread: between two products' last and first MMA the tensor core waits for it.
 template <bool kF32>
 __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int g) {
     const uint32_t tmem = s.tmem, base = smem_addr(ring);
     uint32_t stage = 0, phase = 0, unit0 = 0, seg = 0;
     Walk& w = s.walk[kTeamWarps];
+    auto ready = [&](uint64_t* bar, uint32_t parity) {
+        if (mbar_wait(bar, parity, nullptr)) return true;
+        s.abort = 1;
+        return false;
+    };
     // one operand: its MMAs issued (D = sum over the products of A's halves and the operand's, 16 of the summed
     // dimension at a time), its stage given back, the result announced
     auto product = [&](uint32_t d, uint32_t ta, uint32_t a_step, uint32_t a_lo, uint32_t kind, uint32_t b_step2, uint32_t b_step8,
                        uint32_t id, uint64_t* done) {
-        if (!wait(s, &s.full[stage], phase)) return false;
+        if (!ready(&s.full[stage], phase)) return false;
         tc_fence_after();
-        if (elect_one()) {
-            const uint32_t b = desc_lo(base + stage * kOperandBytes<kF32>, kind);
+        const uint32_t b = desc_lo(base + stage * kOperandBytes<kF32>, kind);
 #pragma unroll
-            for (int p = kF32 ? 0 : 2; p < 3; ++p) {  // lo x hi, hi x lo, hi x hi
+        for (int p = kF32 ? 0 : 2; p < 3; ++p) {  // lo x hi, hi x lo, hi x hi
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    umma_ts_f16(d, ta + i * a_step + (p == 0 ? a_lo : 0),
-                                b + (i & 3) * b_step2 + (i >> 2) * b_step8 + (p == 1 ? 32768 >> 4 : 0), kDescHi, id,
-                                p != (kF32 ? 0 : 2) || i != 0);
-            }
-            umma_commit(&s.empty[stage]);
-            umma_commit(done);
+            for (int i = 0; i < 8; ++i)
+                umma_ts_f16(d, ta + i * a_step + (p == 0 ? a_lo : 0),
+                            b + (i & 3) * b_step2 + (i >> 2) * b_step8 + (p == 1 ? 32768 >> 4 : 0), kDescHi, id,
+                            p != (kF32 ? 0 : 2) || i != 0);
         }
-        __syncwarp();
+        umma_commit(&s.empty[stage]);
+        umma_commit(done);
         if (++stage == kStages<kF32>) stage = 0, phase ^= 1;
         return true;
     };
     auto run = [&] {
-        auto next = [&](bool first) {
-            __syncwarp();
-            const bool more = first ? w.begin(a, s.run, g, kTile, kLead) : w.next(a, g, kTile, kLead);
-            __syncwarp();
-            return more;
-        };
-        for (bool more = next(true); more; more = next(false), ++seg) {
-            if (!wait(s, &s.q_full, seg & 1)) return;
-            tc_fence_after();
+        for (bool more = w.begin(a, s.run, g, kTile, kLead); more; more = w.next(a, g, kTile, kLead), ++seg) {
             const int n = w.n;
+            if (!ready(&s.q_full, seg & 1)) return;
+            tc_fence_after();
             for (int jj = 0; jj <= n; ++jj) {
                 if (jj < n) {  // S = Q K^T: 16 dimensions of K are 32 bytes of a row, 64 a block
                     const uint32_t u = unit0 + jj;
@@ -374,8 +449,8 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
                 }
                 if (jj >= 1) {  // P V: 16 rows of V are 2048 bytes of both its blocks
                     const uint32_t u = unit0 + jj - 1;
-                    if (!wait(s, &s.p_full[u & 1], (u >> 1) & 1)) return;
-                    if (u > 0 && !wait(s, &s.pv_free[(u - 1) & 1], ((u - 1) >> 1) & 1)) return;
+                    if (!ready(&s.p_full[u & 1], (u >> 1) & 1)) return;
+                    if (u > 0 && !ready(&s.pv_free[(u - 1) & 1], ((u - 1) >> 1) & 1)) return;
                     if (!product(tmem + kColPv, tmem + kColS + (u & 1) * 128, 16, 8, kDescValues, 2048 >> 4, 8192 >> 4,
                                  idesc<kF32>(true), &s.pv_full[u & 1]))
                         return;
@@ -386,9 +461,8 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
     };
     run();
     // every MMA of this CTA has finished before its TMEM is freed
-    if (elect_one()) umma_commit(&s.drain);
-    __syncwarp();
-    mbar_wait_warp(&s.drain, 0, nullptr, nullptr);
+    umma_commit(&s.drain);
+    mbar_wait(&s.drain, 0, nullptr);
 }
 
 // ---- the softmax warps ------------------------------------------------------------------------
@@ -412,84 +486,33 @@ UOCR_DEV uint32_t seen_mask(int c0, int hi, int lo, int pre) {
 }
 
 template <bool kF32>
-__device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging, const ChunkParts& parts, int g) {
+__device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging, const Images& im, const ChunkParts& parts, int g) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int team = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = s.tmem + ((uint32_t)(warp & 3) << 21);  // lane field: bits 16 up, 32 lanes a warp
-    const float factor = fabsf(a.scale) * kLog2e;  // the scale's sign is in the query operand
     float qscale = 0.f;
     bool alive = true;
     const uint32_t tid = threadIdx.x;
     auto chunk = [&](int row, int c) { return staging + row * 128 + ((c ^ (row & 7)) << 4); };
 
-    // The query rows of a segment into TMEM. A row is read by 8 threads, 16 bytes each, and turned into its halves
-    // there (qscale: 1 / its scale, times the softmax's factor); by way of shared memory, a quarter of the row at a
-    // time (bf16: a half), it comes to the threads of its lane.
+    // A segment's queries into TMEM (team 0 the hi halves, team 1 the lo ones; bf16: half the dimensions each), once
+    // both teams have read the last one's scores.
     auto load_query = [&](const Walk& w) __attribute__((always_inline)) {
-        constexpr int kElt = kF32 ? 4 : 2, kRounds = kF32 ? 4 : 2;
-        uint4 x[kRounds][4];
-        const int row8 = tid >> 3, c8 = tid & 7, rows = w.r.n * g - w.qt * kTile;
+        const size_t index = (size_t)(query_base(w.r, w.b, g) + w.qt) * a.pass_heads + w.head;
+        const uint4* p = reinterpret_cast<const uint4*>(im.queries + index * kQueryBytes<kF32>) + team * (kF32 ? 16 : 8) * kTile + row;
+        named_bar_sync(kTeamBar, 32 * kTeamWarps);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int rr = k * 32 + row8, R = w.qt * kTile + rr;
-            const char* p = static_cast<const char*>(a.q) +
-                            ((size_t)(w.r.lo + (rr < rows ? R / g : 0)) * a.q_ld +
-                             (size_t)((a.head0 + w.head) * g + (rr < rows ? R % g : 0)) * kDim) * kElt + c8 * 16;
+        for (int h = 0; h < (kF32 ? 2 : 1); ++h) {
+            uint32_t x[32];
 #pragma unroll
-            for (int i = 0; i < kRounds; ++i)
-                x[i][k] = rr < rows ? *reinterpret_cast<const uint4*>(p + i * 128) : make_uint4(0, 0, 0, 0);
-        }
-        if constexpr (kF32) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                uint32_t m = 0;
-                auto take = [&](uint32_t e) {
-                    e &= 0x7FFFFFFFu;
-                    m = max(m, e < 0x7F800000u ? e : 0u);
-                };
-#pragma unroll
-                for (int i = 0; i < 4; ++i) take(x[i][k].x), take(x[i][k].y), take(x[i][k].z), take(x[i][k].w);
-#pragma unroll
-                for (int o = 4; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                // never 0: a hidden score is -inf times this
-                if (c8 == 0) s.qscale[k * 32 + row8] = fmaxf(scale_down(m) * factor, 1e-37f);
-                const float up = a.scale < 0.f ? -scale_up(m) : scale_up(m);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint4 y;  // two words of hi halves, two of lo halves
-                    split2(__uint_as_float(x[i][k].x) * up, __uint_as_float(x[i][k].y) * up, y.x, y.z);
-                    split2(__uint_as_float(x[i][k].z) * up, __uint_as_float(x[i][k].w) * up, y.y, y.w);
-                    x[i][k] = y;
-                }
+            for (int i = 0; i < 8; ++i) {
+                const uint4 v = ldg_nc_v4(p + (h * 8 + i) * kTile);
+                x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tmem_st<8>(lanes + kColQ + team * (kF32 ? 64 : 32) + h * 32 + i * 8, x + 8 * i);
         }
-#pragma unroll
-        for (int i = 0; i < kRounds; ++i) {
-            named_bar_sync(kTeamBar, 32 * kTeamWarps);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int rr = k * 32 + row8;
-                if constexpr (kF32) {  // chunks 0-3 of the row: hi halves, 4-7: lo halves
-                    *reinterpret_cast<uint2*>(chunk(rr, c8 >> 1) + (c8 & 1) * 8) = make_uint2(x[i][k].x, x[i][k].y);
-                    *reinterpret_cast<uint2*>(chunk(rr, 4 + (c8 >> 1)) + (c8 & 1) * 8) = make_uint2(x[i][k].z, x[i][k].w);
-                } else {
-                    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-                    *reinterpret_cast<uint4*>(chunk(rr, c8)) =
-                        make_uint4(x[i][k].x ^ flip, x[i][k].y ^ flip, x[i][k].z ^ flip, x[i][k].w ^ flip);
-                }
-            }
-            named_bar_sync(kTeamBar, 32 * kTeamWarps);
-            uint32_t y[16];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const uint4 v = *reinterpret_cast<const uint4*>(chunk(row, team * 4 + c));
-                y[4 * c] = v.x, y[4 * c + 1] = v.y, y[4 * c + 2] = v.z, y[4 * c + 3] = v.w;
-            }
-            const uint32_t to = lanes + kColQ + (kF32 ? team * 64 + i * 16 : i * 32 + team * 16);
-            tmem_st<8>(to, y);
-            tmem_st<8>(to + 8, y + 8);
-        }
-        qscale = kF32 ? s.qscale[row] : fmaxf(factor, 1e-37f);
+        qscale = __ldg(im.qscale + index * kTile + row);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -498,7 +521,6 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
 
     uint64_t acc[64];  // 128 sums, in pairs
     float m = -INFINITY, l = 0.f, alpha = 1.f;
-    bool run = false;
 
     // The scores of unit u to weights: the running maximum and sum, P in the scores' place; masked: the row does not
     // see all of the page.
@@ -506,11 +528,16 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
         const uint32_t sa = lanes + kColS + (u & 1) * 128;
         const int lo = a.window > 0 ? pos - a.window + 1 - c0 : -kPageRows;
         uint32_t x[32];
-        auto scores = [&](int c) __attribute__((always_inline)) {  // 32 columns, times 1 / scale of each one's key
+        // keys of one scale: it goes into the factor; else 1 / scale of each one's key (a branch, rarely taken)
+        const float all = kF32 ? s.kmeta[u & 7].all : 1.f;
+        const bool own_scales = all == 0.f;
+        const float factor = own_scales ? qscale : fmaxf(qscale * all, 1e-37f);
+        auto scores = [&](int c) __attribute__((always_inline)) {  // 32 columns
             tmem_ld_32x32b_x32(sa + c * 32, x);
             tmem_wait_ld_tie(x);
-            if constexpr (kF32) {
-                const float* ks = &s.kscale[u & 7][c * 32];
+            if (kF32 && own_scales) {
+                asm volatile("");
+                const float* ks = &s.kmeta[u & 7].scale[c * 32];
 #pragma unroll
                 for (int i = 0; i < 32; i += 4) {
                     const float4 k4 = *reinterpret_cast<const float4*>(ks + i);
@@ -536,11 +563,11 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
                 top2 = fmaxf(fmaxf(top2, __uint_as_float(x[i + 2])), __uint_as_float(x[i + 3]));
             }
         }
-        const float mn = fmaxf(m, fmaxf(top, top2) * qscale);
+        const float mn = fmaxf(m, fmaxf(top, top2) * factor);
         alpha = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
         m = mn;
         const float shift = (mn == -INFINITY ? 0.f : mn) - (kF32 ? 14.f : 0.f);
-        const uint64_t q2 = pair(qscale, qscale), s2 = pair(-shift, -shift);
+        const uint64_t q2 = pair(factor, factor), s2 = pair(-shift, -shift);
         uint64_t sum2[2] = {0, 0};
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -611,78 +638,82 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
     };
 
     Walk& w = s.walk[warp];
-    Walk& done = s.done[warp];
+    Walk& now = s.now[warp];  // the segment at work, while w is one ahead
     bool more = w.begin(a, s.run, g, kTile, kLead);
     __syncwarp();
     int state[2] = {0, 0}, place[4] = {0, 0, 0, 0};
     uint32_t unit0 = 0;
-    for (bool first = true; more; first = false) {
-        if (first) load_query(w);
-        const int R = w.qt * kTile + row, rows = w.r.n * g - w.qt * kTile;  // valid rows of the tile
-        const bool live = (warp & 3) * 32 < rows;                           // this warp has some
-        const int pos = w.r.start + R / g;
+    if (more) load_query(w);
+    while (more) {
+        now = w;
+        __syncwarp();
+        const int R = now.qt * kTile + row, rows = now.r.n * g - now.qt * kTile;  // valid rows of the tile
+        const bool live = (warp & 3) * 32 < rows;                                 // this warp has some
+        const int pos = now.r.start + R / g;
         m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[i] = 0;
-        const int n = w.n, j0 = (team ^ unit0) & 1;  // this team's pages: units of its parity
-        for (int j = j0; j < n; j += 2) {
-            const uint32_t u = unit0 + j;
-            const int t = w.t.page(w.j + j), c0 = t * kPageRows;
-            if (alive && !wait(s, &s.s_full[u & 1], (u >> 1) & 1)) alive = false;
-            tc_fence_after();
-            run = alive && live;
-            // does every row of the tile see the whole page?
-            const bool all = c0 + kPageRows - 1 <= w.t.first_pos &&
-                             (a.window <= 0 || c0 > w.t.last_pos - a.window || c0 + kPageRows <= w.r.prefix);
-            if (run) softmax(w, u, !all, pos, c0);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.p_full[u & 1]);
-            if (j + 2 < n) {
+        const int n = now.n, j0 = (team ^ unit0) & 1;  // this team's pages: units of its parity
+        for (int j = j0;; j += 2) {
+            if (j >= n) {  // the next segment's queries, while the last products run
+                more = w.next(a, g, kTile, kLead);
+                __syncwarp();
+                if (more) load_query(w);
+            }
+            if (j > j0) {  // the sums of this team's page before
+                const uint32_t u = unit0 + j - 2;
                 if (alive && !wait(s, &s.pv_full[u & 1], (u >> 1) & 1)) alive = false;
                 tc_fence_after();
-                if (alive && live) add_pv(w, u, t, pos);
+                if (alive && live) add_pv(now, u, now.t.page(now.j + j - 2), pos);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s.pv_free[u & 1]);
             }
-        }
-        // both teams have read the segment's scores (load_query's first barrier): its query makes room for the next
-        const uint32_t last = unit0 + (n - 1 - ((n - 1 - j0) & 1));  // this team's last unit, if n > j0
-        unit0 += n;
-        done = w;
-        __syncwarp();
-        more = w.next(a, g, kTile, kLead);
-        __syncwarp();
-        if (more) load_query(w);
-        if (n > j0) {
-            if (alive && !wait(s, &s.pv_full[last & 1], (last >> 1) & 1)) alive = false;
+            if (j >= n) break;
+            const uint32_t u = unit0 + j;
+            const int c0 = now.t.page(now.j + j) * kPageRows;
+            if (alive && !wait(s, &s.s_full[u & 1], (u >> 1) & 1)) alive = false;
             tc_fence_after();
-            if (alive && live) add_pv(done, last, done.t.page(done.j + (int)(last + n - unit0)), pos);
+            // does every row of the tile see the whole page?
+            const bool all = c0 + kPageRows - 1 <= now.t.first_pos &&
+                             (a.window <= 0 || c0 > now.t.last_pos - a.window || c0 + kPageRows <= now.r.prefix);
+            if (alive && live) softmax(now, u, !all, pos, c0);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s.pv_free[last & 1]);
+            if (lane == 0) mbar_arrive(&s.p_full[u & 1]);
         }
+        unit0 += n;
         // the two teams' results: out = (f0 acc0 + f1 acc1) / (f0 l0 + f1 l1), f = 2^(m - max m)
         s.xmax[team][row] = m, s.xsum[team][row] = l;
         named_bar_sync(kTeamBar, 32 * kTeamWarps);
         const float M = fmaxf(m, s.xmax[team ^ 1][row]);
         auto weight = [&](float mt) { return mt == -INFINITY ? 0.f : exp2_fast(mt - M); };
         const float total = s.xsum[0][row] * weight(s.xmax[0][row]) + s.xsum[1][row] * weight(s.xmax[1][row]);
-        const bool whole = done.whole();
+        const bool whole = now.whole();
         float f = m == -INFINITY && l == 0.f ? 0.f : weight(m);
         if (whole) f *= 1.f / total;
         if (!alive) f = NAN;
         const uint64_t f2 = pair(f, f);
-        const int slot = done.j == 0 ? 1 : 0;
+        const int slot = now.j == 0 ? 1 : 0;
         float* part = parts.slots + ((size_t)blockIdx.x * 2 + slot) * slot_floats(kTile);
         constexpr int kElt = kF32 ? 4 : 2;
         const int row8 = tid >> 3, c8 = tid & 7;
+        char* to[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // 32 columns a round, by way of shared memory: team 1's part, then the sums
+        for (int k = 0; k < 4; ++k) {
+            const int T = now.qt * kTile + k * 32 + row8;
+            to[k] = static_cast<char*>(a.out) +
+                    (((size_t)(now.r.lo + T / g) * a.heads + (a.head0 + now.head) * g + T % g) * kDim + c8 * 4) * kElt;
+        }
+        float* part_at = part + row;
+        // 32 columns a round, by way of shared memory: team 1's part, then the sums (a loop: run once a tile, its
+        // instructions come from far)
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
             if (team == 1) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     uint4 v;
-                    unpair(mul2(acc[i * 16 + 2 * c], f2), v.x, v.y);
-                    unpair(mul2(acc[i * 16 + 2 * c + 1], f2), v.z, v.w);
+                    unpair(mul2(acc[2 * c], f2), v.x, v.y);
+                    unpair(mul2(acc[2 * c + 1], f2), v.z, v.w);
                     *reinterpret_cast<uint4*>(chunk(row, c)) = v;
                 }
             }
@@ -691,12 +722,12 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     uint4 v = *reinterpret_cast<const uint4*>(chunk(row, c));
-                    unpair(fma2(acc[i * 16 + 2 * c], f2, pair(v.x, v.y)), v.x, v.y);
-                    unpair(fma2(acc[i * 16 + 2 * c + 1], f2, pair(v.z, v.w)), v.z, v.w);
+                    unpair(fma2(acc[2 * c], f2, pair(v.x, v.y)), v.x, v.y);
+                    unpair(fma2(acc[2 * c + 1], f2, pair(v.z, v.w)), v.z, v.w);
                     if (whole) {
                         *reinterpret_cast<uint4*>(chunk(row, c)) = v;
                     } else if (row < rows) {
-                        float* o = part + (i * 32 + c * 4) * kTile + row;
+                        float* o = part_at + c * 4 * kTile;
                         o[0] = __uint_as_float(v.x), o[kTile] = __uint_as_float(v.y);
                         o[2 * kTile] = __uint_as_float(v.z), o[3 * kTile] = __uint_as_float(v.w);
                     }
@@ -706,16 +737,17 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
             if (whole) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int rr = k * 32 + row8, T = done.qt * kTile + rr;
-                    if (rr >= rows) continue;
-                    const uint4 v = *reinterpret_cast<const uint4*>(chunk(rr, c8));
-                    char* o = static_cast<char*>(a.out) +
-                              (((size_t)(done.r.lo + T / g) * a.heads + (a.head0 + done.head) * g + T % g) * kDim + i * 32 + c8 * 4) * kElt;
-                    if constexpr (kF32) *reinterpret_cast<uint4*>(o) = v;
-                    else *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16(__uint_as_float(v.x), __uint_as_float(v.y)),
-                                                                   pack_bf16(__uint_as_float(v.z), __uint_as_float(v.w)));
+                    if (k * 32 + row8 >= rows) continue;
+                    const uint4 v = *reinterpret_cast<const uint4*>(chunk(k * 32 + row8, c8));
+                    if constexpr (kF32) *reinterpret_cast<uint4*>(to[k]) = v;
+                    else *reinterpret_cast<uint2*>(to[k]) = make_uint2(pack_bf16(__uint_as_float(v.x), __uint_as_float(v.y)),
+                                                                       pack_bf16(__uint_as_float(v.z), __uint_as_float(v.w)));
+                    to[k] += 32 * kElt;
                 }
             }
+            part_at += 32 * kTile;
+#pragma unroll
+            for (int k = 0; k < 48; ++k) acc[k] = acc[k + 16];
             named_bar_sync(kTeamBar, 32 * kTeamWarps);
         }
         if (!whole) {
@@ -723,9 +755,9 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
                 part[kDim * kTile + row] = M;
                 part[(kDim + 1) * kTile + row] = total;
             }
-            state[slot] = slot == 0 && done.j + done.n == done.t.count ? 2 : 1;
+            state[slot] = slot == 0 && now.j + now.n == now.t.count ? 2 : 1;
             if (slot == 1)
-                place[0] = done.r.lo, place[1] = done.qt * kTile, place[2] = min(rows, kTile), place[3] = a.head0 + done.head;
+                place[0] = now.r.lo, place[1] = now.qt * kTile, place[2] = min(rows, kTile), place[3] = a.head0 + now.head;
         }
     }
     if (tid == 0) {
@@ -757,10 +789,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs 
     pdl_launch_dependents();
     if (warp < kTeamWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTeamRegs));
-        team_role<kF32>(a, s, ring + kStages<kF32> * kOperandBytes<kF32>, parts, g);
+        pdl_wait_prior_grid();
+        team_role<kF32>(a, s, ring + kStages<kF32> * kOperandBytes<kF32>, im, parts, g);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (warp == kTeamWarps) {
+        if (threadIdx.x == 32 * kTeamWarps) {
             mma_role<kF32>(a, s, ring, g);
         } else if (threadIdx.x == 32 * (kTeamWarps + 1)) {
             fence_proxy_async_smem();  // the ring was find_run's scratch
@@ -768,6 +801,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs 
             copy_role<kF32>(a, s, ring, im, g);
         }
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -832,13 +866,16 @@ cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
+// Query tiles of the call, at most (query_base).
+int query_tiles(const ChunkArgs& a) { return (int)((long long)a.T * (a.heads / a.kv_heads) / kTile) + a.B; }
+
 template <bool kF32>
 cudaError_t launch(const ChunkArgs& a, const Images& im, const ChunkParts& parts, cudaStream_t st) {
     const size_t smem = (size_t)kStages<kF32> * kOperandBytes<kF32> + kStagingBytes + 1024;
     auto kernel = chunk_attention_kernel<kF32>;
     cudaError_t err = ensure_smem_optin(reinterpret_cast<const void*>(kernel), smem);
     if (err != cudaSuccess) return err;
-    chunk_operands_kernel<kF32><<<dim3(a.lut_cols, a.pass_heads, a.B), 256, 0, st>>>(a, im);
+    chunk_operands_kernel<kF32><<<dim3(a.B * a.lut_cols + query_tiles(a), a.pass_heads), 256, 0, st>>>(a, im);
     err = cudaGetLastError();
     if (err != cudaSuccess) return err;
     err = launch_dependent(kernel, dim3(parts.ctas), kThreads, smem, st, a, im, parts);
@@ -846,14 +883,18 @@ cudaError_t launch(const ChunkArgs& a, const Images& im, const ChunkParts& parts
     return launch_chunk_join(a, parts, st);
 }
 
-// Bytes of a page's operands and their meta data, one head.
-size_t image_bytes(bool bf16) { return 2 * (size_t)(bf16 ? kOperandBytes<false> : kOperandBytes<true>) + sizeof(PageMeta); }
+// Operands and what lies beside them, of one page or query tile and one head.
+size_t page_bytes(const ChunkArgs& a) { return 2 * (size_t)(a.bf16 ? kOperandBytes<false> : kOperandBytes<true>) + sizeof(PageMeta); }
+size_t query_bytes(const ChunkArgs& a) { return (a.bf16 ? kQueryBytes<false> : kQueryBytes<true>) + kTile * sizeof(float); }
+// The operands of one KV head.
+size_t head_bytes(const ChunkArgs& a) {
+    return (size_t)a.B * a.lut_cols * page_bytes(a) + (size_t)query_tiles(a) * query_bytes(a);
+}
 
 // The KV heads of one pass: their operands stay within 1 GiB (one head at least); a call with more takes several.
 constexpr size_t kPassBytes = size_t(1) << 30;
 int heads_of_pass(const ChunkArgs& a) {
-    const size_t head = (size_t)a.B * a.lut_cols * image_bytes(a.bf16);
-    return (int)std::max<size_t>(1, std::min<size_t>(a.kv_heads, kPassBytes / head));
+    return (int)std::max<size_t>(1, std::min<size_t>(a.kv_heads, kPassBytes / head_bytes(a)));
 }
 
 size_t parts_bytes(int sms, int tile) {
@@ -869,7 +910,7 @@ cudaError_t launch_chunk_join(const ChunkArgs& a, const ChunkParts& p, cudaStrea
 }
 
 size_t chunk_workspace_bytes(const ChunkArgs& a, int sms) {
-    return parts_bytes(sms, kTile) + (size_t)a.B * a.lut_cols * heads_of_pass(a) * image_bytes(a.bf16);
+    return parts_bytes(sms, kTile) + head_bytes(a) * heads_of_pass(a);
 }
 
 cudaError_t launch_chunk_attention(const ChunkArgs& args, void* ws, int sms, cudaStream_t st) {
@@ -879,9 +920,12 @@ cudaError_t launch_chunk_attention(const ChunkArgs& args, void* ws, int sms, cud
     ChunkParts parts{reinterpret_cast<float*>(w + ((size_t)sms * kInfoInts * 4 + 255) / 256 * 256), reinterpret_cast<int*>(w), sms,
                      kTile};
     const int heads = heads_of_pass(a);
+    const size_t pages = (size_t)a.B * a.lut_cols * heads, tiles = (size_t)query_tiles(a) * heads;
     Images im;
     im.operands = reinterpret_cast<unsigned char*>(w + parts_bytes(sms, kTile));
-    im.meta = reinterpret_cast<PageMeta*>(im.operands + (size_t)a.B * a.lut_cols * heads * (image_bytes(a.bf16) - sizeof(PageMeta)));
+    im.queries = im.operands + pages * (page_bytes(a) - sizeof(PageMeta));
+    im.meta = reinterpret_cast<PageMeta*>(im.queries + tiles * (query_bytes(a) - kTile * sizeof(float)));
+    im.qscale = reinterpret_cast<float*>(im.meta + pages);
     for (a.head0 = 0; a.head0 < a.kv_heads; a.head0 += heads) {
         a.pass_heads = std::min(heads, a.kv_heads - a.head0);
         const cudaError_t err = a.bf16 ? launch<false>(a, im, parts, st) : launch<true>(a, im, parts, st);
