@@ -909,7 +909,17 @@ cudaError_t launch_chunk_join(const ChunkArgs& a, const ChunkParts& p, cudaStrea
     return launch_dependent(a.bf16 ? chunk_join_kernel<false> : chunk_join_kernel<true>, grid, 256, 0, st, a, p);
 }
 
+// Rows of a query tile: 1, 2, 4 or 8 where a request has up to 8 (token, head) rows of a KV head on average
+// (chunk_rows.cu: bound by the cache's bytes), else 128 (tensor cores).
+static int tile_rows(const ChunkArgs& a) {
+    const long long rows = (long long)a.T * (a.heads / a.kv_heads);
+    for (int t = 1; t <= 8; t *= 2)
+        if (rows <= (long long)t * a.B) return t;
+    return kTile;
+}
+
 size_t chunk_workspace_bytes(const ChunkArgs& a, int sms) {
+    if (tile_rows(a) < kTile) return parts_bytes(sms, tile_rows(a));
     return parts_bytes(sms, kTile) + head_bytes(a) * heads_of_pass(a);
 }
 
@@ -918,7 +928,11 @@ cudaError_t launch_chunk_attention(const ChunkArgs& args, void* ws, int sms, cud
     if (a.B <= 0 || a.T <= 0) return cudaSuccess;
     char* w = static_cast<char*>(ws);
     ChunkParts parts{reinterpret_cast<float*>(w + ((size_t)sms * kInfoInts * 4 + 255) / 256 * 256), reinterpret_cast<int*>(w), sms,
-                     kTile};
+                     tile_rows(a)};
+    if (parts.tile < kTile) {
+        a.head0 = 0, a.pass_heads = a.kv_heads;
+        return launch_chunk_rows(a, parts, st);
+    }
     const int heads = heads_of_pass(a);
     const size_t pages = (size_t)a.B * a.lut_cols * heads, tiles = (size_t)query_tiles(a) * heads;
     Images im;
