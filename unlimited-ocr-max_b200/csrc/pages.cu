@@ -43,28 +43,96 @@ struct CompactArgs {
     char* pool;
     const int32_t *src_lut, *dst_lut, *keep, *keep_len;
     int pages, planes, row_bytes, src_cols, dst_cols, max_keep;
+    int lanes;   // words (16 bytes) of a row that a CTA moves: a power of two, at most 64
+    int slices;  // CTAs across a row
 };
 
-// New row i of request b is its old row keep[b][i], in every plane. One CTA per request and plane
-// walks the request's rows upwards in groups: a group is read, then (after a barrier) written. The
-// kept rows ascend, so keep[i] >= i, and a group's writes (rows below its end) touch no source of a
-// later group (keep[i'] >= i' >= the group's end): the compaction may be in place.
-__global__ void __launch_bounds__(256) compact_rows_kernel(CompactArgs a) {
-    const int b = blockIdx.y, plane = blockIdx.x;
+constexpr int kMoveThreads = 256;
+constexpr int kMoveUnroll = 8;  // words of a thread in flight: 32 KB per CTA
+
+// New row i of request b is its old row keep[b][i], in every plane. The kept rows ascend, so keep[i] >= i; rows up to
+// the first that changes place stay. A CTA moves `lanes` words of a plane's rows, in groups: a group is read, then
+// (after a barrier) written. Its writes (rows below the group's end) touch no source of a later group
+// (keep[i'] >= i' >= that end), so walking upwards compacts in place; with a slice and plane to itself the
+// CTA needs no order against others. Where no row to move lies below the rows written (keep[first] >= n), or the
+// tables share no page, the groups are independent and the rows are dealt to `splits` CTAs. Bound: HBM (each moved
+// row read and written once).
+__global__ void __launch_bounds__(kMoveThreads) compact_rows_kernel(CompactArgs a, int splits) {
+    __shared__ long long from[2][kMoveThreads * kMoveUnroll / 16], to[2][kMoveThreads * kMoveUnroll / 16];
+    __shared__ int first_shared;
+    const int b = blockIdx.z, plane = blockIdx.y, slice = blockIdx.x % a.slices, split = blockIdx.x / a.slices;
+    const int tid = threadIdx.x;
     const int n = min(min(max(a.keep_len[b], 0), a.max_keep), a.dst_cols * kPageRows);
-    const int words = a.row_bytes / 16;
     const int32_t* keep = a.keep + (size_t)b * a.max_keep;
-    for (int i = 0; i < n; ++i) {
-        const int k = keep[i];
-        if (k < 0 || k >= a.src_cols * kPageRows) continue;  // the same for every thread
-        const int from = a.src_lut[(size_t)b * a.src_cols + k / kPageRows];
-        const int to = a.dst_lut[(size_t)b * a.dst_cols + i / kPageRows];
-        if ((unsigned)from >= (unsigned)a.pages || (unsigned)to >= (unsigned)a.pages) continue;
-        const size_t fo = (((size_t)from * a.planes + plane) * kPageRows + k % kPageRows) * a.row_bytes;
-        const size_t to_ = (((size_t)to * a.planes + plane) * kPageRows + i % kPageRows) * a.row_bytes;
-        if (fo == to_) continue;
-        for (int w = threadIdx.x; w < words; w += blockDim.x)  // a thread reads and writes its own words only
-            reinterpret_cast<uint4*>(a.pool + to_)[w] = reinterpret_cast<const uint4*>(a.pool + fo)[w];
+    const int32_t* src = a.src_lut + (size_t)b * a.src_cols;
+    const int32_t* dst = a.dst_lut + (size_t)b * a.dst_cols;
+    // the first row that changes place
+    if (tid == 0) first_shared = n;
+    __syncthreads();
+    for (int i0 = 0; i0 < n; i0 += kMoveThreads) {
+        const int i = i0 + tid;
+        const bool moves = i < n && (keep[i] != i || i >= a.src_cols * kPageRows || src[i / kPageRows] != dst[i / kPageRows]);
+        if (moves) atomicMin(&first_shared, i);
+        if (__syncthreads_or(moves)) break;
+    }
+    const int first = first_shared;
+    if (first >= n) return;
+    int begin = first, end = n;
+    bool ordered = false;
+    if (keep[first] < n) {  // a row to move may be one that is written: do the tables share a page?
+        const int used = (n + kPageRows - 1) / kPageRows;
+        bool shared = src == dst;
+        for (int c = tid; !shared && c < a.src_cols; c += kMoveThreads) {
+            const int page = src[c];
+            for (int k = first / kPageRows; k < used; ++k) shared |= dst[k] == page;
+        }
+        ordered = __syncthreads_or(shared);
+    }
+    const int per = kMoveThreads / a.lanes, group = per * kMoveUnroll;  // rows at a time, rows of a group
+    if (ordered) {
+        if (split) return;
+    } else {
+        const int groups = (n - first + group - 1) / group, share = (groups + splits - 1) / splits * group;
+        begin = first + split * share, end = min(n, begin + share);
+        if (begin >= end) return;
+    }
+    const int word = slice * a.lanes + tid % a.lanes, row = tid / a.lanes;
+    const bool live = word < a.row_bytes / 16;
+    char* base = a.pool + (size_t)plane * kPageRows * a.row_bytes + (size_t)word * 16;
+    // where the rows of the group at i0 lie (-1: not moved)
+    auto locate = [&](int i0, int buf) {
+        for (int r = tid; r < group; r += kMoveThreads) {
+            const int i = i0 + r, k = i < end ? keep[i] : -1;
+            long long f = -1, t = -1;
+            if (k >= 0 && k < a.src_cols * kPageRows) {
+                const int p = src[k / kPageRows], q = dst[i / kPageRows];
+                if ((unsigned)p < (unsigned)a.pages && (unsigned)q < (unsigned)a.pages) {
+                    f = ((long long)p * a.planes * kPageRows + k % kPageRows) * a.row_bytes;
+                    t = ((long long)q * a.planes * kPageRows + i % kPageRows) * a.row_bytes;
+                    if (f == t) f = -1;
+                }
+            }
+            from[buf][r] = f, to[buf][r] = t;
+        }
+    };
+    locate(begin, 0);
+    __syncthreads();
+    int buf = 0;
+    for (int i0 = begin; i0 < end; i0 += group, buf ^= 1) {
+        uint4 v[kMoveUnroll];
+#pragma unroll
+        for (int u = 0; u < kMoveUnroll; ++u) {
+            const long long f = from[buf][u * per + row];
+            if (live && f >= 0) v[u] = *reinterpret_cast<const uint4*>(base + f);
+        }
+        if (i0 + group < end) locate(i0 + group, buf ^ 1);
+        __syncthreads();  // the group has been read, and the next one's rows are located
+#pragma unroll
+        for (int u = 0; u < kMoveUnroll; ++u) {
+            const int r = u * per + row;
+            if (live && from[buf][r] >= 0) *reinterpret_cast<uint4*>(base + to[buf][r]) = v[u];
+        }
+        __syncthreads();  // from and to of this group are free again
     }
 }
 
@@ -87,8 +155,16 @@ cudaError_t launch_compact_rows(void* pool, int pages, int layers, int row_bytes
                                 const int32_t* keep_len, int B, cudaStream_t st) {
     if (B <= 0 || max_keep <= 0) return cudaSuccess;
     CompactArgs a{static_cast<char*>(pool), src_lut, dst_lut, keep, keep_len, pages, 2 * layers, row_bytes, src_cols,
-                  dst_cols, max_keep};
-    compact_rows_kernel<<<dim3(2 * layers, B), 256, 0, st>>>(a);
+                  dst_cols, max_keep, 0, 0};
+    const int words = row_bytes / 16;
+    a.lanes = 16;
+    while (a.lanes < 64 && a.lanes < words) a.lanes *= 2;
+    a.slices = (words + a.lanes - 1) / a.lanes;
+    // enough CTAs to fill the GPU several times over, none with less than a group
+    const int group = kMoveThreads / a.lanes * kMoveUnroll;
+    const long long others = (long long)a.slices * a.planes * B, wanted = (148 * 16 + others - 1) / others;
+    const int splits = (int)std::max<long long>(1, std::min<long long>(wanted, (max_keep + group - 1) / group));
+    compact_rows_kernel<<<dim3(a.slices * splits, a.planes, B), kMoveThreads, 0, st>>>(a, splits);
     return cudaGetLastError();
 }
 

@@ -277,12 +277,12 @@ def _pool_dims(op: str, kv_pool: torch.Tensor) -> tuple[int, int, int, int]:
     """(pages, layers, heads, bytes of a row) of a page pool, which is used in place."""
     if kv_pool.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"{op}: the pool must be fp32 or bf16, got {kv_pool.dtype}")
-    if kv_pool.dim() != 6 or kv_pool.shape[1] != 2 or kv_pool.shape[3] != 128 or kv_pool.shape[5] != 128:
-        raise ValueError(f"{op}: the pool must be [pages, 2, layers, 128, heads, 128], got {tuple(kv_pool.shape)}")
+    shape = kv_pool.shape
+    if len(shape) != 6 or shape[1] != 2 or shape[3] != 128 or shape[5] != 128:
+        raise ValueError(f"{op}: the pool must be [pages, 2, layers, 128, heads, 128], got {tuple(shape)}")
     if not kv_pool.is_contiguous():
         raise ValueError(f"{op}: the pool must be contiguous (it is written in place)")
-    pages, _, layers, _, heads, dim = kv_pool.shape
-    return pages, layers, heads, heads * dim * kv_pool.element_size()
+    return shape[0], shape[2], shape[4], shape[4] * 128 * kv_pool.itemsize
 
 
 def _index(op: str, t: torch.Tensor, name: str, shape: tuple[int, ...]) -> torch.Tensor:
@@ -292,12 +292,31 @@ def _index(op: str, t: torch.Tensor, name: str, shape: tuple[int, ...]) -> torch
     return t
 
 
-def _extent(t: torch.Tensor) -> tuple[int, int]:
-    """The byte range that a tensor's elements lie in."""
-    if t.numel() == 0:
-        return t.data_ptr(), t.data_ptr()
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t [T, heads, 128]`` and the distance of its rows, each row's heads one run on 16 bytes (else a copy)."""
+    T, heads, _ = t.shape
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, heads * 128
+    ld, between, within = t.stride()
+    if within == 1 and (heads == 1 or between == 128) and t.data_ptr() % 16 == 0:
+        if T <= 1:
+            return t, heads * 128
+        if ld >= heads * 128 and ld * t.itemsize % 16 == 0:
+            return t, ld
+    return t.clone(memory_format=torch.contiguous_format), heads * 128
+
+
+#: workspace bytes of the calls seen, by what they depend on
+_CHUNK_WS: dict[tuple, int] = {}
+
+
+def _on_device(t: torch.Tensor, call) -> None:
+    """``call(stream)`` with ``t``'s device current, on its current stream."""
+    if torch.cuda.current_device() == t.device.index:
+        check(call(_stream(t)))
+    else:
+        with torch.cuda.device(t.device):
+            check(call(_stream(t)))
 
 
 def paged_chunk_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, kv_pool: torch.Tensor, layer: int,
@@ -316,11 +335,17 @@ def paged_chunk_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Ten
     only those with ``r > p - window`` or ``r < prefix[b]`` (int32 ``[B]``; None: 0). ``out [T, heads, 128]``
     (contiguous, overlapping no input) is returned; its rows in no request keep what they held. All index
     tensors are on the device, and nothing synchronises; the workspace is the call's own, so calls may run
-    on several streams and be captured. The result is deterministic.
+    on several streams and be captured. The result is deterministic. ``T * heads / kv_heads`` against the
+    number of requests decides the form: up to 8 rows a request and KV head are computed straight from the
+    cache, more on the tensor cores (fp32 values then to 2^-38 of the largest finite one of their page).
     """
     op = "paged_chunk_attention"
-    extra = [t for t in (prefix, out) if t is not None]
-    _need_cuda(op, q, k_new, v_new, kv_pool, lut, row_offsets, start, *extra)
+    tensors = [q, k_new, v_new, kv_pool, lut, row_offsets, start]
+    if prefix is not None:
+        tensors.append(prefix)
+    if out is not None:
+        tensors.append(out)
+    _need_cuda(op, *tensors)
     pages, layers, kv_heads, _ = _pool_dims(op, kv_pool)
     dt = kv_pool.dtype
     for name, t in (("q", q), ("k_new", k_new), ("v_new", v_new)):
@@ -337,41 +362,47 @@ def paged_chunk_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Ten
     if lut.dim() != 2:
         raise ValueError(f"{op}: lut must be [B, cols], got {tuple(lut.shape)}")
     lut = lut.contiguous()
-    B = lut.shape[0]
+    B, cols = lut.shape
     row_offsets = _index(op, row_offsets, "row_offsets", (B + 1,))
     start = _index(op, start, "start", (B,))
     if prefix is not None:
         prefix = _index(op, prefix, "prefix", (B,))
-    step = 16 // dt.itemsize
-
-    def rows(t):  # a row's heads are read as one run; rows may lie apart
-        whole = t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == 128)
-        if whole and (T <= 1 or (t.stride(0) >= t.shape[1] * 128 and t.stride(0) % step == 0)) and t.data_ptr() % 16 == 0:
-            return t, (t.stride(0) if T > 1 else t.shape[1] * 128)
-        t = t.clone(memory_format=torch.contiguous_format)
-        return t, t.shape[1] * 128
-
-    q, q_ld = rows(q)
-    k_new, k_ld = rows(k_new)
-    v_new, v_ld = rows(v_new)
+    q, q_ld = _rows(q)
+    k_new, k_ld = _rows(k_new)
+    v_new, v_ld = _rows(v_new)
     if out is None:
         out = torch.empty((T, heads, 128), dtype=dt, device=q.device)
     elif out.dtype != dt or out.shape != (T, heads, 128) or not out.is_contiguous():
         raise ValueError(f"{op}: out must be a contiguous {dt} tensor of shape {(T, heads, 128)}")
-    else:
-        lo, hi = _extent(out)
-        for name, t in (("q", q), ("k_new", k_new), ("v_new", v_new), ("the pool", kv_pool)):
-            a, z = _extent(t)
-            if a < hi and lo < z:
-                raise ValueError(f"{op}: out overlaps {name}")
-    with torch.cuda.device(q.device):
-        need = load().uocr_paged_chunk_workspace_bytes(T, heads, kv_heads, 1 if dt == torch.bfloat16 else 0, lut.shape[1], B)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        check(load().uocr_paged_chunk_attention(
-            q.data_ptr(), q_ld, k_new.data_ptr(), k_ld, v_new.data_ptr(), v_ld, T, heads, kv_heads, dim,
-            1 if dt == torch.bfloat16 else 0, kv_pool.data_ptr(), pages, layers, layer, lut.data_ptr(), lut.shape[1],
-            row_offsets.data_ptr(), start.data_ptr(), B, float(scale), int(window),
-            0 if prefix is None else prefix.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(q)))
+    size = dt.itemsize
+    at = {"q": q.data_ptr(), "k_new": k_new.data_ptr(), "v_new": v_new.data_ptr(), "the pool": kv_pool.data_ptr()}
+    pool_at, out_at = at["the pool"], out.data_ptr()
+    pool_end, out_end = pool_at + kv_pool.numel() * size, out_at + T * heads * 128 * size
+    for name, ld, width in (("q", q_ld, heads), ("k_new", k_ld, kv_heads), ("v_new", v_ld, kv_heads)):
+        a, z = at[name], at[name] + ((T - 1) * ld + width * 128) * size
+        if T and a < out_end and out_at < z:
+            raise ValueError(f"{op}: out overlaps {name}")
+        if T and a < pool_end and pool_at < z:
+            raise ValueError(f"{op}: {name} overlaps the pool")
+    if T and pool_at < out_end and out_at < pool_end:
+        raise ValueError(f"{op}: out overlaps the pool")
+    kind = 1 if dt == torch.bfloat16 else 0
+    scale, window, lib = float(scale), int(window), load()
+
+    def call(stream):
+        key = (T, heads, kv_heads, kind, cols, B, kv_pool.device)
+        need = _CHUNK_WS.get(key)
+        if need is None:
+            if len(_CHUNK_WS) > 4096:
+                _CHUNK_WS.clear()
+            need = _CHUNK_WS[key] = lib.uocr_paged_chunk_workspace_bytes(T, heads, kv_heads, kind, cols, B)
+        ws = torch.empty(need, dtype=torch.uint8, device=kv_pool.device)
+        return lib.uocr_paged_chunk_attention(
+            at["q"], q_ld, at["k_new"], k_ld, at["v_new"], v_ld, T, heads, kv_heads, dim, kind, pool_at, pages, layers, layer,
+            lut.data_ptr(), cols, row_offsets.data_ptr(), start.data_ptr(), B, scale, window,
+            None if prefix is None else prefix.data_ptr(), out_at, ws.data_ptr(), need, stream)
+
+    _on_device(kv_pool, call)
     return out
 
 
@@ -387,9 +418,9 @@ def copy_pages(kv_pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, *, r
     dst = _index(op, dst, "dst", tuple(src.shape))
     if rows is not None:
         rows = _index(op, rows, "rows", tuple(src.shape))
-    with torch.cuda.device(kv_pool.device):
-        check(load().uocr_copy_pages(kv_pool.data_ptr(), pages, layers, row_bytes, src.data_ptr(), dst.data_ptr(),
-                                     0 if rows is None else rows.data_ptr(), src.shape[0], _stream(kv_pool)))
+    _on_device(kv_pool, lambda stream: load().uocr_copy_pages(
+        kv_pool.data_ptr(), pages, layers, row_bytes, src.data_ptr(), dst.data_ptr(),
+        0 if rows is None else rows.data_ptr(), src.shape[0], stream))
 
 
 def compact_rows(kv_pool: torch.Tensor, src_lut: torch.Tensor, dst_lut: torch.Tensor, keep: torch.Tensor,
@@ -409,7 +440,6 @@ def compact_rows(kv_pool: torch.Tensor, src_lut: torch.Tensor, dst_lut: torch.Te
     B = keep_len.shape[0]
     if src_lut.shape[0] != B or dst_lut.shape[0] != B or keep.shape[0] != B:
         raise ValueError(f"{op}: src_lut, dst_lut, keep and keep_len disagree on the number of requests")
-    with torch.cuda.device(kv_pool.device):
-        check(load().uocr_compact_rows(kv_pool.data_ptr(), pages, layers, row_bytes, src_lut.data_ptr(), src_lut.shape[1],
-                                       dst_lut.data_ptr(), dst_lut.shape[1], keep.data_ptr(), keep.shape[1],
-                                       keep_len.data_ptr(), B, _stream(kv_pool)))
+    _on_device(kv_pool, lambda stream: load().uocr_compact_rows(
+        kv_pool.data_ptr(), pages, layers, row_bytes, src_lut.data_ptr(), src_lut.shape[1], dst_lut.data_ptr(),
+        dst_lut.shape[1], keep.data_ptr(), keep.shape[1], keep_len.data_ptr(), B, stream))
