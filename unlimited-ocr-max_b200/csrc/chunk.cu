@@ -38,7 +38,7 @@ namespace {
 
 constexpr int kTile = 128;      // (token, head) rows of a query tile
 constexpr int kLead = 6;        // what a tile costs beside its pages
-constexpr int kTeamWarps = 8;   // softmax; then a warpgroup of the issuing warp, the copying warp and two idle ones
+constexpr int kTeamWarps = 8;   // softmax; then a warpgroup: the warps that issue Q K^T, copy, issue P V, and an idle one
 constexpr int kThreads = 32 * (kTeamWarps + 4);
 constexpr int kLaunchRegs = 168, kTeamRegs = 216, kOtherRegs = 72;  // a thread
 static_assert(kTeamWarps * kTeamRegs + 4 * kOtherRegs <= (kTeamWarps + 4) * kLaunchRegs, "a split of the launch's registers");
@@ -56,21 +56,13 @@ constexpr int kStagingBytes = kTile * 128;  // a quarter (fp32) or half (bf16) o
 // TMEM columns
 constexpr uint32_t kColS = 0, kColPv = 256, kColQ = 384;
 
-// Beside a page's operands. Keys: 1 / scale of each row, and of all of them where they share one scale (else 0).
-// Values: 1 / scale, and which rows are not finite.
-struct alignas(16) KeyMeta {
-    float scale[kPageRows];
-    float all;
-    float pad[3];
-};
-struct alignas(16) ValueMeta {
-    float scale;
-    float pad[3];
-    uint32_t bad[4];
-};
+// Beside a page's operands: 1 / scale of each row of k, and of all of them where they share one (else 0); 1 / scale of
+// v, and which rows of v are not finite. bf16 has the last of these only.
 struct alignas(16) PageMeta {
-    KeyMeta k;
-    ValueMeta v;
+    float keys[kPageRows];
+    float all_keys, values;
+    float pad[2];
+    uint32_t bad[4];
 };
 
 // The operands of a pass, made by the first launch. Keys and values: page p of request b and head h (of the pass)
@@ -90,14 +82,14 @@ constexpr int kQueryBytes = kTile * kDim * (kF32 ? 4 : 2);
 UOCR_DEV int query_base(const Request& r, int b, int g) { return r.lo * g / kTile + b; }
 
 struct Shared {
-    KeyMeta kmeta[8];  // by unit
-    ValueMeta vmeta[8];
-    uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], p_full[2], pv_full[2], pv_free[2], q_full, drain;
+    PageMeta meta[8];  // by unit
+    uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], p_full[2], pv_full[2], pv_free, q_full, drain[2];
+    uint32_t fresh[2];
     uint32_t tmem;
     volatile int abort;
     Run run;
     Walk walk[kThreads / 32], now[kTeamWarps];
-    float xmax[2][kTile], xsum[2][kTile];
+    float xmax[2][2][kTile], xsum[2][kTile];
 };
 
 UOCR_DEV bool wait(Shared& s, uint64_t* bar, uint32_t parity) {
@@ -133,6 +125,19 @@ UOCR_DEV void tmem_st<8>(uint32_t addr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
+}
+// 64 columns into x, complete on return (the waits mark x as written by them: no use moves in front of them).
+UOCR_DEV void tmem_ld64(uint32_t addr, uint32_t (&x)[64]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]), "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]), "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31])
+                 : "r"(addr + 0));
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(x[32]), "=r"(x[33]), "=r"(x[34]), "=r"(x[35]), "=r"(x[36]), "=r"(x[37]), "=r"(x[38]), "=r"(x[39]), "=r"(x[40]), "=r"(x[41]), "=r"(x[42]), "=r"(x[43]), "=r"(x[44]), "=r"(x[45]), "=r"(x[46]), "=r"(x[47]), "=r"(x[48]), "=r"(x[49]), "=r"(x[50]), "=r"(x[51]), "=r"(x[52]), "=r"(x[53]), "=r"(x[54]), "=r"(x[55]), "=r"(x[56]), "=r"(x[57]), "=r"(x[58]), "=r"(x[59]), "=r"(x[60]), "=r"(x[61]), "=r"(x[62]), "=r"(x[63])
+                 : "r"(addr + 32));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]), "+r"(x[9]), "+r"(x[10]), "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15]) : : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[16]), "+r"(x[17]), "+r"(x[18]), "+r"(x[19]), "+r"(x[20]), "+r"(x[21]), "+r"(x[22]), "+r"(x[23]), "+r"(x[24]), "+r"(x[25]), "+r"(x[26]), "+r"(x[27]), "+r"(x[28]), "+r"(x[29]), "+r"(x[30]), "+r"(x[31]) : : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[32]), "+r"(x[33]), "+r"(x[34]), "+r"(x[35]), "+r"(x[36]), "+r"(x[37]), "+r"(x[38]), "+r"(x[39]), "+r"(x[40]), "+r"(x[41]), "+r"(x[42]), "+r"(x[43]), "+r"(x[44]), "+r"(x[45]), "+r"(x[46]), "+r"(x[47]) : : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[48]), "+r"(x[49]), "+r"(x[50]), "+r"(x[51]), "+r"(x[52]), "+r"(x[53]), "+r"(x[54]), "+r"(x[55]), "+r"(x[56]), "+r"(x[57]), "+r"(x[58]), "+r"(x[59]), "+r"(x[60]), "+r"(x[61]), "+r"(x[62]), "+r"(x[63]) : : "memory");
 }
 // Two fp32 operations an instruction (each rounded as its scalar form).
 UOCR_DEV uint64_t pair(uint32_t x, uint32_t y) {
@@ -312,9 +317,9 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
             if (kF32) {
                 top = __reduce_max_sync(0xffffffffu, tops[lane & 7]);
                 up = scale_up(top);
-                if (threadIdx.x == 0) meta.v.scale = scale_down(top);
+                if (threadIdx.x == 0) meta.values = scale_down(top);
             }
-            if (threadIdx.x < 4) meta.v.bad[threadIdx.x] = bads[2 * threadIdx.x] | bads[2 * threadIdx.x + 1] << 16;
+            if (threadIdx.x < 4) meta.bad[threadIdx.x] = bads[2 * threadIdx.x] | bads[2 * threadIdx.x + 1] << 16;
         } else if (kF32) {
 #pragma unroll
             for (int i = 0; i < kWords; ++i) {
@@ -339,8 +344,8 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
             const bool near = my_top == 0 || (my_top >> 23) + 10 >= page_top >> 23;
             if (near) my_top = page_top;
             const bool all = __syncthreads_and(near || lane >= 16);
-            if (lane < 16) meta.k.scale[warp * 16 + lane] = scale_down(my_top);
-            if (threadIdx.x == 0) meta.k.all = all ? scale_down(page_top) : 0.f;
+            if (lane < 16) meta.keys[warp * 16 + lane] = scale_down(my_top);
+            if (threadIdx.x == 0) meta.all_keys = all ? scale_down(page_top) : 0.f;
         }
         unsigned char* out = im.operands + (index * 2 + v) * kOperandBytes<kF32>;
 #pragma unroll
@@ -374,12 +379,13 @@ __device__ void copy_role(const ChunkArgs& a, Shared& s, unsigned char* ring, co
         const uint32_t u = (unit0 + j) & 7;
         const PageMeta& meta = im.meta[index];
         if (!mbar_wait(&s.empty[stage], phase ^ 1, nullptr)) return false;
-        const uint32_t extra = v ? sizeof(ValueMeta) : kF32 ? sizeof(KeyMeta) : 0;
-        mbar_arrive_expect_tx(&s.full[stage], kOperandBytes<kF32> + extra);
+        constexpr uint32_t kSkip = kF32 ? 0 : offsetof(PageMeta, all_keys), kMetaBytes = sizeof(PageMeta) - kSkip;
+        mbar_arrive_expect_tx(&s.full[stage], kOperandBytes<kF32> + (v ? 0 : kMetaBytes));
         bulk_g2s(ring + stage * kOperandBytes<kF32>, im.operands + (index * 2 + v) * kOperandBytes<kF32>, kOperandBytes<kF32>,
                  &s.full[stage]);
-        if (v) bulk_g2s(&s.vmeta[u], &meta.v, sizeof(ValueMeta), &s.full[stage]);
-        else if (kF32) bulk_g2s(&s.kmeta[u], &meta.k, sizeof(KeyMeta), &s.full[stage]);
+        if (!v)
+            bulk_g2s(reinterpret_cast<char*>(&s.meta[u]) + kSkip, reinterpret_cast<const char*>(&meta) + kSkip, kMetaBytes,
+                     &s.full[stage]);
         ++issued;
         if (++stage == kStages<kF32>) stage = 0, phase ^= 1;
         return true;
@@ -404,71 +410,86 @@ __device__ void copy_role(const ChunkArgs& a, Shared& s, unsigned char* ring, co
 }
 
 // ---- the issuing warp -------------------------------------------------------------------------
-// One thread: between two products' last and first MMA the tensor core waits for it.
-template <bool kF32>
-__device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int g) {
-    const uint32_t tmem = s.tmem, base = smem_addr(ring);
-    uint32_t stage = 0, phase = 0, unit0 = 0, seg = 0;
-    Walk& w = s.walk[kTeamWarps];
+// Two warps, one thread each: S = Q K^T and P V. While one waits for its next operand or looks at its barriers, the
+// other's MMAs keep the tensor core busy. Operand i of a CTA lies in stage i % kStages; K(j) of a segment is operand
+// 2 j - 1 (K(0): 0) of the segment's 2 n, V(j) operand 2 j + 2 (V(n - 1): 2 n - 1).
+template <bool kF32, bool kValues>
+__device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int g, Walk& w) {
+    const uint32_t base = smem_addr(ring);
     auto ready = [&](uint64_t* bar, uint32_t parity) {
         if (mbar_wait(bar, parity, nullptr)) return true;
         s.abort = 1;
         return false;
     };
-    // one operand: its MMAs issued (D = sum over the products of A's halves and the operand's, 16 of the summed
-    // dimension at a time), its stage given back, the result announced
-    auto product = [&](uint32_t d, uint32_t ta, uint32_t a_step, uint32_t a_lo, uint32_t kind, uint32_t b_step2, uint32_t b_step8,
-                       uint32_t id, uint64_t* done) {
-        if (!ready(&s.full[stage], phase)) return false;
+    // 16 dimensions of K are 32 bytes of a row, 64 a block; 16 rows of V are 2048 bytes of both its blocks
+    constexpr uint32_t a_step = kValues ? 16 : 8, a_lo = kValues ? 8 : 64;
+    constexpr uint32_t b_step2 = kValues ? 2048 >> 4 : 32 >> 4, b_step8 = kValues ? 8192 >> 4 : 16384 >> 4;
+    auto product = [&](uint32_t op, uint32_t buf, uint32_t accumulate, uint64_t* done) {
+        const uint32_t stage = op % kStages<kF32>;
+        if (!ready(&s.full[stage], op / kStages<kF32> & 1)) return false;
         tc_fence_after();
-        const uint32_t b = desc_lo(base + stage * kOperandBytes<kF32>, kind);
+        const uint32_t b = desc_lo(base + stage * kOperandBytes<kF32>, kValues ? kDescValues : kDescKeys);
+        const uint32_t scores = kColS + buf * 128, d = kValues ? kColPv : scores, ta = kValues ? scores : kColQ;
 #pragma unroll
         for (int p = kF32 ? 0 : 2; p < 3; ++p) {  // lo x hi, hi x lo, hi x hi
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 umma_ts_f16(d, ta + i * a_step + (p == 0 ? a_lo : 0),
-                            b + (i & 3) * b_step2 + (i >> 2) * b_step8 + (p == 1 ? 32768 >> 4 : 0), kDescHi, id,
-                            p != (kF32 ? 0 : 2) || i != 0);
+                            b + (i & 3) * b_step2 + (i >> 2) * b_step8 + (p == 1 ? 32768 >> 4 : 0), kDescHi, idesc<kF32>(kValues),
+                            p != (kF32 ? 0 : 2) || i != 0 ? 1u : accumulate);
         }
         umma_commit(&s.empty[stage]);
         umma_commit(done);
-        if (++stage == kStages<kF32>) stage = 0, phase ^= 1;
         return true;
     };
     auto run = [&] {
+        uint32_t unit0 = 0, seg = 0, sums = 0;  // sums: begun so far in TMEM
         for (bool more = w.begin(a, s.run, g, kTile, kLead); more; more = w.next(a, g, kTile, kLead), ++seg) {
             const int n = w.n;
-            if (!ready(&s.q_full, seg & 1)) return;
-            tc_fence_after();
-            for (int jj = 0; jj <= n; ++jj) {
-                if (jj < n) {  // S = Q K^T: 16 dimensions of K are 32 bytes of a row, 64 a block
-                    const uint32_t u = unit0 + jj;
-                    if (!product(tmem + kColS + (u & 1) * 128, tmem + kColQ, 8, 64, kDescKeys, 32 >> 4, 16384 >> 4,
-                                 idesc<kF32>(false), &s.s_full[u & 1]))
-                        return;
-                }
-                if (jj >= 1) {  // P V: 16 rows of V are 2048 bytes of both its blocks
-                    const uint32_t u = unit0 + jj - 1;
-                    if (!ready(&s.p_full[u & 1], (u >> 1) & 1)) return;
-                    if (u > 0 && !ready(&s.pv_free[(u - 1) & 1], ((u - 1) >> 1) & 1)) return;
-                    if (!product(tmem + kColPv, tmem + kColS + (u & 1) * 128, 16, 8, kDescValues, 2048 >> 4, 8192 >> 4,
-                                 idesc<kF32>(true), &s.pv_full[u & 1]))
-                        return;
+            if (!kValues) {
+                if (!ready(&s.q_full, seg & 1)) return;
+                tc_fence_after();
+            }
+            for (int j = 0; j < n; ++j) {
+                const uint32_t u = unit0 + j, buf = u & 1;
+                if (kValues) {
+                    if (!ready(&s.p_full[buf], (u >> 1) & 1)) return;
+                    const uint32_t fresh = s.fresh[buf];  // a new sum, once the last one has been taken
+                    if (fresh && sums++ && !ready(&s.pv_free, (sums - 2) & 1)) return;
+                    if (!product(2 * unit0 + (j == n - 1 ? 2 * n - 1 : 2 * j + 2), buf, fresh ^ 1, &s.pv_full[buf])) return;
+                } else {
+                    if (u > 1 && !ready(&s.pv_full[buf], ((u - 2) >> 1) & 1)) return;  // the weights in this buffer are used
+                    if (!product(2 * unit0 + (j == 0 ? 0 : 2 * j - 1), buf, 0, &s.s_full[buf])) return;
                 }
             }
             unit0 += n;
         }
     };
-    run();
-    // every MMA of this CTA has finished before its TMEM is freed
-    umma_commit(&s.drain);
-    mbar_wait(&s.drain, 0, nullptr);
+    if (s.tmem == 0) run();
+    else s.abort = 1;  // never: all 512 columns are ours
+    // this warp's MMAs have finished before the CTA's TMEM is freed
+    umma_commit(&s.drain[kValues]);
+    mbar_wait(&s.drain[kValues], 0, nullptr);
 }
 
 // ---- the softmax warps ------------------------------------------------------------------------
-// Two teams of 4 warps take the pages of a segment in turn, a thread one row of the query tile (its TMEM lane)
-// with a maximum, a sum and 128 sums of its own; the teams' results are joined at the segment's end. While one
-// team waits for the tensor core the other one computes.
+// Two threads per row of the query tile (its TMEM lane): columns and dimensions [64 half, 64 half + 64) each. A row's
+// weights are 2^(score - m) with m its maximum when the sum in TMEM was begun: while no score of the tile exceeds its
+// row's m by more than 7, the tensor core adds page after page into that sum; then, or after kSumPages pages, the
+// threads take it into their registers (fp32, round to nearest; the tensor core's own additions truncate, which is why an
+// fp32 sum is short) and m becomes the maximum. fp32: the weights are 2^4 larger, and by the page's value scale over
+// the sum's where that is within 2^4: at most 2^15, and their halves resolve 2^-25.
+template <bool kF32>
+constexpr int kSumPages = kF32 ? 2 : 16;
+constexpr float kHeadroom = 7.f;
+UOCR_DEV bool any_of_team(bool v) {  // a barrier of the softmax warps
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r)
+                 : "r"((uint32_t)v), "r"(kTeamBar), "r"(32 * kTeamWarps)
+                 : "memory");
+    return r != 0;
+}
 template <bool kF32>
 UOCR_DEV const char* value_row(const ChunkArgs& a, const Walk& w, int t, int row) {
     constexpr int kElt = kF32 ? 4 : 2;
@@ -488,18 +509,18 @@ UOCR_DEV uint32_t seen_mask(int c0, int hi, int lo, int pre) {
 template <bool kF32>
 __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging, const Images& im, const ChunkParts& parts, int g) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int team = warp >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t lanes = s.tmem + ((uint32_t)(warp & 3) << 21);  // lane field: bits 16 up, 32 lanes a warp
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM address: lane from bit 16 up, 32 lanes a warp; columns from 0
     float qscale = 0.f;
     bool alive = true;
     const uint32_t tid = threadIdx.x;
     auto chunk = [&](int row, int c) { return staging + row * 128 + ((c ^ (row & 7)) << 4); };
 
-    // A segment's queries into TMEM (team 0 the hi halves, team 1 the lo ones; bf16: half the dimensions each), once
-    // both teams have read the last one's scores.
+    // A segment's queries into TMEM (half 0 of the threads the hi halves, half 1 the lo ones; bf16: half the dimensions
+    // each), once all have read the last one's scores.
     auto load_query = [&](const Walk& w) __attribute__((always_inline)) {
         const size_t index = (size_t)(query_base(w.r, w.b, g) + w.qt) * a.pass_heads + w.head;
-        const uint4* p = reinterpret_cast<const uint4*>(im.queries + index * kQueryBytes<kF32>) + team * (kF32 ? 16 : 8) * kTile + row;
+        const uint4* p = reinterpret_cast<const uint4*>(im.queries + index * kQueryBytes<kF32>) + half * (kF32 ? 16 : 8) * kTile + row;
         named_bar_sync(kTeamBar, 32 * kTeamWarps);
 #pragma unroll
         for (int h = 0; h < (kF32 ? 2 : 1); ++h) {
@@ -510,7 +531,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
                 x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_st<8>(lanes + kColQ + team * (kF32 ? 64 : 32) + h * 32 + i * 8, x + 8 * i);
+            for (int i = 0; i < 4; ++i) tmem_st<8>(lanes + kColQ + half * (kF32 ? 64 : 32) + h * 32 + i * 8, x + 8 * i);
         }
         qscale = __ldg(im.qscale + index * kTile + row);
         tmem_wait_st();
@@ -519,120 +540,49 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
         if (lane == 0) mbar_arrive(&s.q_full);
     };
 
-    uint64_t acc[64];  // 128 sums, in pairs
-    float m = -INFINITY, l = 0.f, alpha = 1.f;
+    uint64_t acc[32];  // 64 sums, in pairs
+    float m = -INFINITY, l = 0.f;
 
-    // The scores of unit u to weights: the running maximum and sum, P in the scores' place; masked: the row does not
-    // see all of the page.
-    auto softmax = [&](const Walk& w, uint32_t u, bool masked, int pos, int c0) __attribute__((always_inline)) {
-        const uint32_t sa = lanes + kColS + (u & 1) * 128;
-        const int lo = a.window > 0 ? pos - a.window + 1 - c0 : -kPageRows;
-        uint32_t x[32];
-        // keys of one scale: it goes into the factor; else 1 / scale of each one's key (a branch, rarely taken)
-        const float all = kF32 ? s.kmeta[u & 7].all : 1.f;
-        const bool own_scales = all == 0.f;
-        const float factor = own_scales ? qscale : fmaxf(qscale * all, 1e-37f);
-        auto scores = [&](int c) __attribute__((always_inline)) {  // 32 columns
-            tmem_ld_32x32b_x32(sa + c * 32, x);
-            tmem_wait_ld_tie(x);
-            if (kF32 && own_scales) {
-                asm volatile("");
-                const float* ks = &s.kmeta[u & 7].scale[c * 32];
+    // The sum in TMEM into acc (unit u its last page's), with its values' scale
+    auto take_sum = [&](uint32_t u, float scale, bool live) __attribute__((always_inline)) {
+        if (alive && !wait(s, &s.pv_full[u & 1], (u >> 1) & 1)) alive = false;
+        tc_fence_after();
+        if (alive && live) {
+            const uint64_t f2 = pair(scale, scale);
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    const float4 k4 = *reinterpret_cast<const float4*>(ks + i);
-                    unpair(mul2(pair(x[i], x[i + 1]), pair(k4.x, k4.y)), x[i], x[i + 1]);
-                    unpair(mul2(pair(x[i + 2], x[i + 3]), pair(k4.z, k4.w)), x[i + 2], x[i + 3]);
-                }
-            }
-            if (masked) {
-                asm volatile("");  // a branch, not 32 selects on every page
-                const uint32_t mask = seen_mask(c * 32, pos - c0, lo, w.r.prefix - c0);
+            for (int c = 0; c < 2; ++c) {
+                uint32_t x[32];
+                tmem_ld_32x32b_x32(lanes + kColPv + half * 64 + c * 32, x);
+                tmem_wait_ld_tie(x);
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (!(mask >> i & 1)) x[i] = 0xFF800000u;
+                for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fma2(pair(x[2 * i], x[2 * i + 1]), f2, acc[c * 16 + i]);
             }
-        };
-        float top = -INFINITY, top2 = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-            scores(c);
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                top = fmaxf(fmaxf(top, __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
-                top2 = fmaxf(fmaxf(top2, __uint_as_float(x[i + 2])), __uint_as_float(x[i + 3]));
-            }
+            tc_fence_before();
         }
-        const float mn = fmaxf(m, fmaxf(top, top2) * factor);
-        alpha = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
-        m = mn;
-        const float shift = (mn == -INFINITY ? 0.f : mn) - (kF32 ? 14.f : 0.f);
-        const uint64_t q2 = pair(factor, factor), s2 = pair(-shift, -shift);
-        uint64_t sum2[2] = {0, 0};
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-            scores(c);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t hi[8], lo[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    uint32_t p0, p1;
-                    unpair(fma2(pair(x[h * 16 + 2 * i], x[h * 16 + 2 * i + 1]), q2, s2), p0, p1);
-                    const float e0 = exp2_fast(__uint_as_float(p0)), e1 = exp2_fast(__uint_as_float(p1));
-                    sum2[i & 1] = add2(sum2[i & 1], pair(e0, e1));
-                    if constexpr (kF32) split2(e0, e1, hi[i], lo[i]);
-                    else hi[i] = pack_bf16(e0, e1);
-                }
-                // in the place of the 16 scores just read
-                tmem_st<8>(sa + c * 32 + h * 16, hi);
-                if constexpr (kF32) tmem_st<8>(sa + c * 32 + h * 16 + 8, lo);
-            }
-        }
-        uint32_t u0, u1;
-        unpair(add2(sum2[0], sum2[1]), u0, u1);
-        l = l * alpha + (__uint_as_float(u0) + __uint_as_float(u1));
-        tmem_wait_st();
-        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.pv_free);
     };
 
-    // acc = acc * alpha + (P V of unit u), and the values of page t that were kept out of it
-    auto add_pv = [&](const Walk& w, uint32_t u, int t, int pos) __attribute__((always_inline)) {
-        const float f = kF32 ? s.vmeta[u & 7].scale : 1.f;
-        const uint64_t a2 = pair(alpha, alpha), f2 = pair(f, f);
+    // The values of page t that are not finite and were kept out of its operand
+    auto add_bad = [&](const Walk& w, uint32_t u, int t, int pos) __attribute__((always_inline)) {
+        for (int q = 0; q < kPageRows; ++q) {
+            if (!(s.meta[u & 7].bad[q >> 5] >> (q & 31) & 1)) continue;
+            const int r = t * kPageRows + q;
+            const bool seen = r <= pos && (a.window <= 0 || r > pos - a.window || r < w.r.prefix);
+            if (!seen) continue;
+            const char* p = value_row<kF32>(a, w, t, q) + half * (kF32 ? 256 : 128);
+            auto odd = [](float v) { return odd_f32(__float_as_uint(v)) ? v : 0.f; };
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            uint32_t x[32];
-            tmem_ld_32x32b_x32(lanes + kColPv + c * 32, x);
-            tmem_wait_ld_tie(x);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const uint64_t v = pair(x[2 * i], x[2 * i + 1]);
-                acc[c * 16 + i] = fma2(acc[c * 16 + i], a2, kF32 ? mul2(v, f2) : v);
-            }
-        }
-        tc_fence_before();
-        const uint4 vb = *reinterpret_cast<const uint4*>(s.vmeta[u & 7].bad);
-        if (vb.x | vb.y | vb.z | vb.w) {
-            for (int q = 0; q < kPageRows; ++q) {
-                if (!(s.vmeta[u & 7].bad[q >> 5] >> (q & 31) & 1)) continue;
-                const int r = t * kPageRows + q;
-                const bool seen = r <= pos && (a.window <= 0 || r > pos - a.window || r < w.r.prefix);
-                if (!seen) continue;
-                const char* p = value_row<kF32>(a, w, t, q);
-                auto odd = [](float v) { return odd_f32(__float_as_uint(v)) ? v : 0.f; };
-#pragma unroll
-                for (int d = 0; d < 64; ++d) {
-                    float v0, v1;
-                    if constexpr (kF32) {
-                        const float2 v = reinterpret_cast<const float2*>(p)[d];
-                        v0 = v.x, v1 = v.y;
-                    } else {
-                        const uint32_t v = reinterpret_cast<const uint32_t*>(p)[d];
-                        v0 = bf16lo(v), v1 = bf16hi(v);
-                    }
-                    acc[d] = add2(acc[d], pair(odd(v0), odd(v1)));
+            for (int d = 0; d < 32; ++d) {
+                float v0, v1;
+                if constexpr (kF32) {
+                    const float2 v = reinterpret_cast<const float2*>(p)[d];
+                    v0 = v.x, v1 = v.y;
+                } else {
+                    const uint32_t v = reinterpret_cast<const uint32_t*>(p)[d];
+                    v0 = bf16lo(v), v1 = bf16hi(v);
                 }
+                acc[d] = add2(acc[d], pair(odd(v0), odd(v1)));
             }
         }
     };
@@ -653,88 +603,148 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
         m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[i] = 0;
-        const int n = now.n, j0 = (team ^ unit0) & 1;  // this team's pages: units of its parity
-        for (int j = j0;; j += 2) {
-            if (j >= n) {  // the next segment's queries, while the last products run
+        const int n = now.n;
+        float sum_scale = 1.f;  // of the sum in TMEM
+        int sum_pages = 0;
+        for (int j = 0;; ++j) {
+            if (j == n) {  // the next segment's queries, while the last products run
                 more = w.next(a, g, kTile, kLead);
                 __syncwarp();
                 if (more) load_query(w);
+                break;
             }
-            if (j > j0) {  // the sums of this team's page before
-                const uint32_t u = unit0 + j - 2;
-                if (alive && !wait(s, &s.pv_full[u & 1], (u >> 1) & 1)) alive = false;
-                tc_fence_after();
-                if (alive && live) add_pv(now, u, now.t.page(now.j + j - 2), pos);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s.pv_free[u & 1]);
-            }
-            if (j >= n) break;
-            const uint32_t u = unit0 + j;
+            const uint32_t u = unit0 + j, sa = lanes + kColS + (u & 1) * 128 + half * 64;
             const int c0 = now.t.page(now.j + j) * kPageRows;
             if (alive && !wait(s, &s.s_full[u & 1], (u >> 1) & 1)) alive = false;
             tc_fence_after();
+            const bool run = alive && live;
             // does every row of the tile see the whole page?
             const bool all = c0 + kPageRows - 1 <= now.t.first_pos &&
                              (a.window <= 0 || c0 > now.t.last_pos - a.window || c0 + kPageRows <= now.r.prefix);
-            if (alive && live) softmax(now, u, !all, pos, c0);
+            // keys of one scale: it goes into the factor; else 1 / scale of each one's key (a branch, rarely taken)
+            const PageMeta& pm = s.meta[u & 7];
+            const float all_keys = kF32 ? pm.all_keys : 1.f, factor = kF32 && all_keys != 0.f ? fmaxf(qscale * all_keys, 1e-37f) : qscale;
+            uint32_t x[64];
+            float top = -INFINITY;
+            if (run) {
+                tmem_ld64(sa, x);
+                if (kF32 && all_keys == 0.f) {
+                    asm volatile("");
+#pragma unroll
+                    for (int i = 0; i < 64; i += 4) {
+                        const float4 k4 = *reinterpret_cast<const float4*>(pm.keys + half * 64 + i);
+                        unpair(mul2(pair(x[i], x[i + 1]), pair(k4.x, k4.y)), x[i], x[i + 1]);
+                        unpair(mul2(pair(x[i + 2], x[i + 3]), pair(k4.z, k4.w)), x[i + 2], x[i + 3]);
+                    }
+                }
+                if (!all) {
+                    asm volatile("");  // a branch, not 64 selects on every page
+                    const int lo = a.window > 0 ? pos - a.window + 1 - c0 : -kPageRows;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const uint32_t mask = seen_mask(half * 64 + c * 32, pos - c0, lo, now.r.prefix - c0);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (!(mask >> i & 1)) x[c * 32 + i] = 0xFF800000u;
+                    }
+                }
+                float top2 = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 64; i += 4) {
+                    top = fmaxf(fmaxf(top, __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
+                    top2 = fmaxf(fmaxf(top2, __uint_as_float(x[i + 2])), __uint_as_float(x[i + 3]));
+                }
+                top = fmaxf(top, top2) * factor;
+            }
+            s.xmax[u & 1][half][row] = top;
+            bool fresh = any_of_team(top > m + kHeadroom);
+            int shift = 0;  // of the page's value scale against the sum's, in powers of 2
+            if (kF32) {
+                shift = (int)(__float_as_uint(pm.values) >> 23) - (int)(__float_as_uint(sum_scale) >> 23);
+                fresh |= shift > 4 || shift < -4;
+            }
+            fresh |= j == 0 || sum_pages == kSumPages<kF32>;
+            if (fresh) {
+                if (j > 0) take_sum(u - 1, sum_scale, live);
+                const float mn = fmaxf(m, fmaxf(top, s.xmax[u & 1][half ^ 1][row]));
+                const float keep = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
+                if (__any_sync(0xffffffffu, keep != 1.f)) {
+                    const uint64_t k2 = pair(keep, keep);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) acc[i] = mul2(acc[i], k2);
+                    l *= keep;
+                }
+                m = mn;
+                if (kF32) sum_scale = pm.values;
+                shift = 0, sum_pages = 0;
+            }
+            ++sum_pages;
+            if (run) {
+                const float base = (kF32 ? 4.f + (float)shift : 0.f) - (m == -INFINITY ? 0.f : m);
+                const uint64_t q2 = pair(factor, factor), s2 = pair(base, base);
+                uint64_t sum2[2] = {0, 0};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint32_t p0, p1;
+                        unpair(fma2(pair(x[c * 16 + 2 * i], x[c * 16 + 2 * i + 1]), q2, s2), p0, p1);
+                        const float e0 = exp2_fast(__uint_as_float(p0)), e1 = exp2_fast(__uint_as_float(p1));
+                        sum2[i & 1] = add2(sum2[i & 1], pair(e0, e1));
+                        if constexpr (kF32) split2(e0, e1, hi[i], lo[i]);
+                        else hi[i] = pack_bf16(e0, e1);
+                    }
+                    // in the place of the 16 scores
+                    tmem_st<8>(sa + c * 16, hi);
+                    if constexpr (kF32) tmem_st<8>(sa + c * 16 + 8, lo);
+                }
+                uint32_t u0, u1;
+                unpair(add2(sum2[0], sum2[1]), u0, u1);
+                l += (__uint_as_float(u0) + __uint_as_float(u1)) * (kF32 ? __uint_as_float((uint32_t)(127 - shift) << 23) : 1.f);
+                tmem_wait_st();
+                tc_fence_before();
+            }
+            if (lane == 0) s.fresh[u & 1] = fresh;
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.p_full[u & 1]);
+            const uint4 bad = *reinterpret_cast<const uint4*>(pm.bad);
+            if (bad.x | bad.y | bad.z | bad.w) add_bad(now, u, now.t.page(now.j + j), pos);
         }
+        take_sum(unit0 + n - 1, sum_scale, live);
         unit0 += n;
-        // the two teams' results: out = (f0 acc0 + f1 acc1) / (f0 l0 + f1 l1), f = 2^(m - max m)
-        s.xmax[team][row] = m, s.xsum[team][row] = l;
+        // rows of the tile to rows of out by way of shared memory, 64 bytes (fp32: 16 columns) of each half a round; or
+        // to the workspace, column by column
+        s.xsum[half][row] = l;
         named_bar_sync(kTeamBar, 32 * kTeamWarps);
-        const float M = fmaxf(m, s.xmax[team ^ 1][row]);
-        auto weight = [&](float mt) { return mt == -INFINITY ? 0.f : exp2_fast(mt - M); };
-        const float total = s.xsum[0][row] * weight(s.xmax[0][row]) + s.xsum[1][row] * weight(s.xmax[1][row]);
+        const float total = s.xsum[0][row] + s.xsum[1][row];
         const bool whole = now.whole();
-        float f = m == -INFINITY && l == 0.f ? 0.f : weight(m);
-        if (whole) f *= 1.f / total;
-        if (!alive) f = NAN;
+        const float f = !alive ? NAN : whole ? 1.f / total : 1.f;
         const uint64_t f2 = pair(f, f);
         const int slot = now.j == 0 ? 1 : 0;
         float* part = parts.slots + ((size_t)blockIdx.x * 2 + slot) * slot_floats(kTile);
-        constexpr int kElt = kF32 ? 4 : 2;
-        const int row8 = tid >> 3, c8 = tid & 7;
-        char* to[4];
+        if (whole) {
+            constexpr int kElt = kF32 ? 4 : 2;
+            const int row8 = tid >> 3, c8 = tid & 7;
+            char* to[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int T = now.qt * kTile + k * 32 + row8;
-            to[k] = static_cast<char*>(a.out) +
-                    (((size_t)(now.r.lo + T / g) * a.heads + (a.head0 + now.head) * g + T % g) * kDim + c8 * 4) * kElt;
-        }
-        float* part_at = part + row;
-        // 32 columns a round, by way of shared memory: team 1's part, then the sums (a loop: run once a tile, its
-        // instructions come from far)
+            for (int k = 0; k < 4; ++k) {
+                const int T = now.qt * kTile + k * 32 + row8;
+                to[k] = static_cast<char*>(a.out) +
+                        (((size_t)(now.r.lo + T / g) * a.heads + (a.head0 + now.head) * g + T % g) * kDim + (c8 >> 2) * 64 + (c8 & 3) * 4) *
+                            kElt;
+            }
+            // a loop: run once a tile, its instructions come from far
 #pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-            if (team == 1) {
+            for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
+                for (int c = 0; c < 4; ++c) {
                     uint4 v;
                     unpair(mul2(acc[2 * c], f2), v.x, v.y);
                     unpair(mul2(acc[2 * c + 1], f2), v.z, v.w);
-                    *reinterpret_cast<uint4*>(chunk(row, c)) = v;
+                    *reinterpret_cast<uint4*>(chunk(row, half * 4 + c)) = v;
                 }
-            }
-            named_bar_sync(kTeamBar, 32 * kTeamWarps);
-            if (team == 0) {
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    uint4 v = *reinterpret_cast<const uint4*>(chunk(row, c));
-                    unpair(fma2(acc[2 * c], f2, pair(v.x, v.y)), v.x, v.y);
-                    unpair(fma2(acc[2 * c + 1], f2, pair(v.z, v.w)), v.z, v.w);
-                    if (whole) {
-                        *reinterpret_cast<uint4*>(chunk(row, c)) = v;
-                    } else if (row < rows) {
-                        float* o = part_at + c * 4 * kTile;
-                        o[0] = __uint_as_float(v.x), o[kTile] = __uint_as_float(v.y);
-                        o[2 * kTile] = __uint_as_float(v.z), o[3 * kTile] = __uint_as_float(v.w);
-                    }
-                }
-            }
-            named_bar_sync(kTeamBar, 32 * kTeamWarps);
-            if (whole) {
+                named_bar_sync(kTeamBar, 32 * kTeamWarps);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     if (k * 32 + row8 >= rows) continue;
@@ -742,17 +752,25 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
                     if constexpr (kF32) *reinterpret_cast<uint4*>(to[k]) = v;
                     else *reinterpret_cast<uint2*>(to[k]) = make_uint2(pack_bf16(__uint_as_float(v.x), __uint_as_float(v.y)),
                                                                        pack_bf16(__uint_as_float(v.z), __uint_as_float(v.w)));
-                    to[k] += 32 * kElt;
+                    to[k] += 16 * kElt;
                 }
-            }
-            part_at += 32 * kTile;
 #pragma unroll
-            for (int k = 0; k < 48; ++k) acc[k] = acc[k + 16];
-            named_bar_sync(kTeamBar, 32 * kTeamWarps);
+                for (int k = 0; k < 24; ++k) acc[k] = acc[k + 8];
+                named_bar_sync(kTeamBar, 32 * kTeamWarps);
+            }
+        } else if (row < rows) {
+            float* o = part + half * 64 * kTile + row;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                uint32_t y0, y1;
+                unpair(mul2(acc[i], f2), y0, y1);
+                o[2 * i * kTile] = __uint_as_float(y0), o[(2 * i + 1) * kTile] = __uint_as_float(y1);
+            }
         }
+        named_bar_sync(kTeamBar, 32 * kTeamWarps);
         if (!whole) {
-            if (team == 0 && row < rows) {
-                part[kDim * kTile + row] = M;
+            if (half == 0 && row < rows) {
+                part[kDim * kTile + row] = m;
                 part[(kDim + 1) * kTile + row] = total;
             }
             state[slot] = slot == 0 && now.j + now.n == now.t.count ? 2 : 1;
@@ -776,9 +794,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs 
     const int g = a.heads / a.kv_heads;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&s.s_full[i], 1), mbar_init(&s.p_full[i], kTeamWarps / 2), mbar_init(&s.pv_full[i], 1),
-                                    mbar_init(&s.pv_free[i], kTeamWarps / 2);
-        mbar_init(&s.q_full, kTeamWarps), mbar_init(&s.drain, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&s.s_full[i], 1), mbar_init(&s.p_full[i], kTeamWarps), mbar_init(&s.pv_full[i], 1);
+        mbar_init(&s.pv_free, kTeamWarps), mbar_init(&s.q_full, kTeamWarps), mbar_init(&s.drain[0], 1), mbar_init(&s.drain[1], 1);
         fence_mbar_init();
         s.abort = 0;
     }
@@ -794,7 +811,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs 
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (threadIdx.x == 32 * kTeamWarps) {
-            mma_role<kF32>(a, s, ring, g);
+            mma_role<kF32, false>(a, s, ring, g, s.walk[kTeamWarps]);
+        } else if (threadIdx.x == 32 * (kTeamWarps + 2)) {
+            mma_role<kF32, true>(a, s, ring, g, s.walk[kTeamWarps + 2]);
         } else if (threadIdx.x == 32 * (kTeamWarps + 1)) {
             fence_proxy_async_smem();  // the ring was find_run's scratch
             pdl_wait_prior_grid();
