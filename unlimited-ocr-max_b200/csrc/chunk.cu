@@ -38,7 +38,7 @@ namespace {
 
 constexpr int kTile = 128;      // (token, head) rows of a query tile
 constexpr int kLead = 6;        // what a tile costs beside its pages
-constexpr int kTeamWarps = 8;   // softmax; then a warpgroup: the warps that issue Q K^T, copy, issue P V, and an idle one
+constexpr int kTeamWarps = 8;   // softmax; then a warpgroup: the issuing warp, the copying warp and two idle ones
 constexpr int kThreads = 32 * (kTeamWarps + 4);
 constexpr int kLaunchRegs = 168, kTeamRegs = 216, kOtherRegs = 72;  // a thread
 static_assert(kTeamWarps * kTeamRegs + 4 * kOtherRegs <= (kTeamWarps + 4) * kLaunchRegs, "a split of the launch's registers");
@@ -49,7 +49,7 @@ constexpr int kOperandBytes = kF32 ? 65536 : 32768;
 template <bool kF32>
 constexpr int kStages = kF32 ? 3 : 6;  // of operands in shared memory
 constexpr int kMaxStages = 6;
-constexpr uint32_t kTeamBar = 1;
+constexpr uint32_t kTeamBar = 1, kPairBar = 2;  // all softmax warps; the two warps of 32 rows (kPairBar + 0..3)
 constexpr int kStagingBytes = kTile * 128;  // a quarter (fp32) or half (bf16) of a tile's rows, between the row-wise and the
                                             // lane-wise order; 16-byte chunks swizzled by the row
 
@@ -83,8 +83,7 @@ UOCR_DEV int query_base(const Request& r, int b, int g) { return r.lo * g / kTil
 
 struct Shared {
     PageMeta meta[8];  // by unit
-    uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], p_full[2], pv_full[2], pv_free, q_full, drain[2];
-    uint32_t fresh[2];
+    uint64_t full[kMaxStages], empty[kMaxStages], s_full[2], p_full[2], pv_full[2], pv_free, q_full, drain;
     uint32_t tmem;
     volatile int abort;
     Run run;
@@ -92,20 +91,39 @@ struct Shared {
     float xmax[2][2][kTile], xsum[2][kTile];
 };
 
+// A whole warp's bounded wait: one lane polls (32 lanes' polls take several times as long), the others follow.
 UOCR_DEV bool wait(Shared& s, uint64_t* bar, uint32_t parity) {
-    if (mbar_wait_warp(bar, parity, &s.abort, nullptr)) return true;
-    s.abort = 1;
-    return false;
+    uint32_t ok = 1;
+    if ((threadIdx.x & 31) == 0 && !mbar_try_wait(bar, parity)) {
+        const uint64_t t0 = global_timer_ns();
+        while (ok && !mbar_try_wait(bar, parity)) ok = !s.abort && global_timer_ns() - t0 <= kWaitBudgetNs;
+        if (!ok) s.abort = 1;
+    }
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
 // ---- tensor-core operands ---------------------------------------------------------------------
-// D[tmem] (+)= A[tmem] * B[smem], kind::f16, one thread issues. The descriptor's upper word is a constant.
-UOCR_DEV void umma_ts_f16(uint32_t d, uint32_t a, uint32_t desc_lo, uint32_t desc_hi, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] * B[smem], kind::f16, where `me` (one lane of a converged warp: the operands stay in uniform
+// registers, from which the tensor core takes them). The descriptor's upper word is a constant.
+UOCR_DEV void umma_ts_f16(uint32_t me, uint32_t d, uint32_t a, uint32_t desc_lo, uint32_t desc_hi, uint32_t idesc,
+                          uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-        "r"(a), "r"(desc_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\tsetp.ne.b32 e, %6, 0;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(desc_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate), "r"(me)
         : "memory");
+}
+UOCR_DEV void umma_commit_if(uint32_t me, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+        "r"(me)
+        : "memory");
+}
+UOCR_DEV uint32_t elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok;
 }
 // Shared-memory descriptors, 128-byte swizzle: 8-row groups 1024 bytes apart (the upper word); keys K-major (the
 // leading stride is not used), values MN-major, their 64-column blocks 16 KB apart.
@@ -409,87 +427,100 @@ __device__ void copy_role(const ChunkArgs& a, Shared& s, unsigned char* ring, co
     }
 }
 
+// Pages whose products are added in TMEM.
+template <bool kF32>
+constexpr int kSumPages = kF32 ? 1 : 16;
+
 // ---- the issuing warp -------------------------------------------------------------------------
-// Two warps, one thread each: S = Q K^T and P V. While one waits for its next operand or looks at its barriers, the
-// other's MMAs keep the tensor core busy. Operand i of a CTA lies in stage i % kStages; K(j) of a segment is operand
-// 2 j - 1 (K(0): 0) of the segment's 2 n, V(j) operand 2 j + 2 (V(n - 1): 2 n - 1).
-template <bool kF32, bool kValues>
-__device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int g, Walk& w) {
-    const uint32_t base = smem_addr(ring);
-    auto ready = [&](uint64_t* bar, uint32_t parity) {
-        if (mbar_wait(bar, parity, nullptr)) return true;
-        s.abort = 1;
-        return false;
+// One warp, converged, one lane of which issues. A page's P V and the scores of the page after the next are issued as one
+// run of MMAs, in whose middle the tensor core waits for nothing: the scores go where the weights lay, and MMAs run
+// in the order in which they are issued. Meanwhile the softmax warps have the page between them.
+template <bool kF32>
+__device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int g) {
+    const uint32_t base = smem_addr(ring), me = elect_one();
+    Walk& w = s.walk[kTeamWarps];
+    uint32_t stage = 0, phase = 0, unit0 = 0, seg = 0, sums = 0;  // sums: begun so far in TMEM
+    auto look = [&](uint64_t* bar, uint32_t parity) { return mbar_try_wait(bar, parity); };
+    // the operand `ahead` of the next one
+    auto full = [&](uint32_t ahead) {
+        const bool wraps = stage + ahead >= kStages<kF32>;
+        return look(&s.full[wraps ? stage + ahead - kStages<kF32> : stage + ahead], phase ^ (wraps ? 1 : 0));
     };
-    // 16 dimensions of K are 32 bytes of a row, 64 a block; 16 rows of V are 2048 bytes of both its blocks
-    constexpr uint32_t a_step = kValues ? 16 : 8, a_lo = kValues ? 8 : 64;
-    constexpr uint32_t b_step2 = kValues ? 2048 >> 4 : 32 >> 4, b_step8 = kValues ? 8192 >> 4 : 16384 >> 4;
-    auto product = [&](uint32_t op, uint32_t buf, uint32_t accumulate, uint64_t* done) {
-        const uint32_t stage = op % kStages<kF32>;
-        if (!ready(&s.full[stage], op / kStages<kF32> & 1)) return false;
-        tc_fence_after();
-        const uint32_t b = desc_lo(base + stage * kOperandBytes<kF32>, kValues ? kDescValues : kDescKeys);
-        const uint32_t scores = kColS + buf * 128, d = kValues ? kColPv : scores, ta = kValues ? scores : kColQ;
+    auto bounded = [&](auto&& all) {  // looks at all the barriers at once, until all are passed
+        if (__all_sync(0xffffffffu, all())) return true;
+        const uint64_t t0 = global_timer_ns();
+        while (!__all_sync(0xffffffffu, all())) {
+            if (__any_sync(0xffffffffu, s.abort || global_timer_ns() - t0 > kWaitBudgetNs)) {
+                s.abort = 1;
+                return false;
+            }
+        }
+        return true;
+    };
+    // the MMAs of the next operand: D = sum over the products of A's halves and the operand's, 16 of the summed dimension
+    // at a time; its stage given back, the result announced
+    auto product = [&](uint32_t d, uint32_t ta, uint32_t a_step, uint32_t a_lo, uint32_t kind, uint32_t b_step2, uint32_t b_step8,
+                       uint32_t id, uint32_t accumulate, uint64_t* done) __attribute__((always_inline)) {
+        const uint32_t b = desc_lo(base + stage * kOperandBytes<kF32>, kind);
 #pragma unroll
         for (int p = kF32 ? 0 : 2; p < 3; ++p) {  // lo x hi, hi x lo, hi x hi
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                umma_ts_f16(d, ta + i * a_step + (p == 0 ? a_lo : 0),
-                            b + (i & 3) * b_step2 + (i >> 2) * b_step8 + (p == 1 ? 32768 >> 4 : 0), kDescHi, idesc<kF32>(kValues),
+                umma_ts_f16(me, d, ta + i * a_step + (p == 0 ? a_lo : 0),
+                            b + (i & 3) * b_step2 + (i >> 2) * b_step8 + (p == 1 ? 32768 >> 4 : 0), kDescHi, id,
                             p != (kF32 ? 0 : 2) || i != 0 ? 1u : accumulate);
         }
-        umma_commit(&s.empty[stage]);
-        umma_commit(done);
-        return true;
+        umma_commit_if(me, &s.empty[stage]);
+        umma_commit_if(me, done);
+        if (++stage == kStages<kF32>) stage = 0, phase ^= 1;
     };
     auto run = [&] {
-        uint32_t unit0 = 0, seg = 0, sums = 0;  // sums: begun so far in TMEM
-        for (bool more = w.begin(a, s.run, g, kTile, kLead); more; more = w.next(a, g, kTile, kLead), ++seg) {
-            const int n = w.n;
-            if (!kValues) {
-                if (!ready(&s.q_full, seg & 1)) return;
-                tc_fence_after();
-            }
-            for (int j = 0; j < n; ++j) {
+        auto next = [&](bool first) {
+            __syncwarp();
+            const bool more = first ? w.begin(a, s.run, g, kTile, kLead) : w.next(a, g, kTile, kLead);
+            __syncwarp();
+            return __any_sync(0xffffffffu, more);
+        };
+        for (bool more = next(true); more; more = next(false), ++seg) {
+            const int n = __reduce_max_sync(0xffffffffu, w.n);
+            if (!bounded([&] { return look(&s.q_full, seg & 1); })) return;
+            for (int j = -2; j < n; ++j) {  // P V of page j, scores of page j + 2
                 const uint32_t u = unit0 + j, buf = u & 1;
-                if (kValues) {
-                    if (!ready(&s.p_full[buf], (u >> 1) & 1)) return;
-                    const uint32_t fresh = s.fresh[buf];  // a new sum, once the last one has been taken
-                    if (fresh && sums++ && !ready(&s.pv_free, (sums - 2) & 1)) return;
-                    if (!product(2 * unit0 + (j == n - 1 ? 2 * n - 1 : 2 * j + 2), buf, fresh ^ 1, &s.pv_full[buf])) return;
-                } else {
-                    if (u > 1 && !ready(&s.pv_full[buf], ((u - 2) >> 1) & 1)) return;  // the weights in this buffer are used
-                    if (!product(2 * unit0 + (j == 0 ? 0 : 2 * j - 1), buf, 0, &s.s_full[buf])) return;
-                }
+                const bool values = j >= 0, scores = j + 2 < n;
+                const bool fresh = values && j % kSumPages<kF32> == 0;  // a new sum, once the last one has been taken
+                const uint32_t taken = fresh ? sums++ : 0;
+                // 16 dimensions of K are 32 bytes of a row, 64 a block; 16 rows of V are 2048 bytes of both its blocks
+                if (!bounded([&] {
+                        return (!values || look(&s.p_full[buf], (u >> 1) & 1)) && (!(values || scores) || full(0)) &&
+                               (!(values && scores) || full(1)) && (taken == 0 || look(&s.pv_free, (taken - 1) & 1));
+                    }))
+                    return;
+                tc_fence_after();
+                if (values)
+                    product(kColPv, kColS + buf * 128, 16, 8, kDescValues, 2048 >> 4, 8192 >> 4, idesc<kF32>(true), !fresh,
+                            &s.pv_full[buf]);
+                if (scores)
+                    product(kColS + buf * 128, kColQ, 8, 64, kDescKeys, 32 >> 4, 16384 >> 4, idesc<kF32>(false), 0, &s.s_full[buf]);
             }
             unit0 += n;
         }
     };
     if (s.tmem == 0) run();
     else s.abort = 1;  // never: all 512 columns are ours
-    // this warp's MMAs have finished before the CTA's TMEM is freed
-    umma_commit(&s.drain[kValues]);
-    mbar_wait(&s.drain[kValues], 0, nullptr);
+    // the MMAs have finished before the CTA's TMEM is freed
+    umma_commit_if(me, &s.drain);
+    mbar_wait_warp(&s.drain, 0, nullptr, nullptr);
 }
 
 // ---- the softmax warps ------------------------------------------------------------------------
 // Two threads per row of the query tile (its TMEM lane): columns and dimensions [64 half, 64 half + 64) each. A row's
-// weights are 2^(score - m) with m its maximum when the sum in TMEM was begun: while no score of the tile exceeds its
-// row's m by more than 7, the tensor core adds page after page into that sum; then, or after kSumPages pages, the
-// threads take it into their registers (fp32, round to nearest; the tensor core's own additions truncate, which is why an
-// fp32 sum is short) and m becomes the maximum. fp32: the weights are 2^4 larger, and by the page's value scale over
-// the sum's where that is within 2^4: at most 2^15, and their halves resolve 2^-25.
-template <bool kF32>
-constexpr int kSumPages = kF32 ? 2 : 16;
-constexpr float kHeadroom = 7.f;
-UOCR_DEV bool any_of_team(bool v) {  // a barrier of the softmax warps
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(r)
-                 : "r"((uint32_t)v), "r"(kTeamBar), "r"(32 * kTeamWarps)
-                 : "memory");
-    return r != 0;
-}
+// weights are 2^(score - m); m is at most 7 below the row's maximum so far, and where a page exceeds that the row's
+// warps raise m and scale what they have. bf16: the tensor core adds the products of 16 pages in TMEM, which then come
+// into the threads' registers; fp32: of one page, for its own additions truncate (the threads' round to nearest:
+// 8.6e-7 off at 8192 rows, 1.2e-6 with two pages to a sum and no faster). The fp32 weights are 2^7 larger: at most
+// 2^14, and their halves resolve 2^-25.
+constexpr float kHeadroom = 7.f, kLift = 7.f;
+// Row `row` of the values of page t (this head's 128 columns).
 template <bool kF32>
 UOCR_DEV const char* value_row(const ChunkArgs& a, const Walk& w, int t, int row) {
     constexpr int kElt = kF32 ? 4 : 2;
@@ -514,6 +545,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
     float qscale = 0.f;
     bool alive = true;
     const uint32_t tid = threadIdx.x;
+    const uint32_t pair_bar = kPairBar + (warp & 3);
     auto chunk = [&](int row, int c) { return staging + row * 128 + ((c ^ (row & 7)) << 4); };
 
     // A segment's queries into TMEM (half 0 of the threads the hi halves, half 1 the lo ones; bf16: half the dimensions
@@ -543,24 +575,36 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
     uint64_t acc[32];  // 64 sums, in pairs
     float m = -INFINITY, l = 0.f;
 
-    // The sum in TMEM into acc (unit u its last page's), with its values' scale
-    auto take_sum = [&](uint32_t u, float scale, bool live) __attribute__((always_inline)) {
+    // acc = (acc + the sum in TMEM, unit u its last page's, times its values' scale) * keep; ends = false: the sum stays
+    // in TMEM, and it and acc become keep times as large.
+    auto take_sum = [&](uint32_t u, float scale, float keep, bool ends, bool live) __attribute__((always_inline)) {
         if (alive && !wait(s, &s.pv_full[u & 1], (u >> 1) & 1)) alive = false;
         tc_fence_after();
         if (alive && live) {
-            const uint64_t f2 = pair(scale, scale);
+            const uint64_t k2 = pair(keep, keep), f2 = ends ? pair(scale * keep, scale * keep) : 0;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t x[32];
                 tmem_ld_32x32b_x32(lanes + kColPv + half * 64 + c * 32, x);
                 tmem_wait_ld_tie(x);
+                if (ends) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fma2(pair(x[2 * i], x[2 * i + 1]), f2, acc[c * 16 + i]);
+                    for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fma2(pair(x[2 * i], x[2 * i + 1]), f2, mul2(acc[c * 16 + i], k2));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        acc[c * 16 + i] = mul2(acc[c * 16 + i], k2);
+                        unpair(mul2(pair(x[2 * i], x[2 * i + 1]), k2), x[2 * i], x[2 * i + 1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) tmem_st<8>(lanes + kColPv + half * 64 + c * 32 + i * 8, x + 8 * i);
+                }
             }
+            if (!ends) tmem_wait_st();
             tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s.pv_free);
+        if (ends && lane == 0) mbar_arrive(&s.pv_free);
     };
 
     // The values of page t that are not finite and were kept out of its operand
@@ -605,7 +649,6 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
         for (int i = 0; i < 64; ++i) acc[i] = 0;
         const int n = now.n;
         float sum_scale = 1.f;  // of the sum in TMEM
-        int sum_pages = 0;
         for (int j = 0;; ++j) {
             if (j == n) {  // the next segment's queries, while the last products run
                 more = w.next(a, g, kTile, kLead);
@@ -623,7 +666,8 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
                              (a.window <= 0 || c0 > now.t.last_pos - a.window || c0 + kPageRows <= now.r.prefix);
             // keys of one scale: it goes into the factor; else 1 / scale of each one's key (a branch, rarely taken)
             const PageMeta& pm = s.meta[u & 7];
-            const float all_keys = kF32 ? pm.all_keys : 1.f, factor = kF32 && all_keys != 0.f ? fmaxf(qscale * all_keys, 1e-37f) : qscale;
+            const float2 page = kF32 ? *reinterpret_cast<const float2*>(&pm.all_keys) : make_float2(1.f, 1.f);
+            const float all_keys = page.x, factor = kF32 && all_keys != 0.f ? fmaxf(qscale * all_keys, 1e-37f) : qscale;
             uint32_t x[64];
             float top = -INFINITY;
             if (run) {
@@ -657,43 +701,38 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
                 top = fmaxf(top, top2) * factor;
             }
             s.xmax[u & 1][half][row] = top;
-            bool fresh = any_of_team(top > m + kHeadroom);
-            int shift = 0;  // of the page's value scale against the sum's, in powers of 2
-            if (kF32) {
-                shift = (int)(__float_as_uint(pm.values) >> 23) - (int)(__float_as_uint(sum_scale) >> 23);
-                fresh |= shift > 4 || shift < -4;
-            }
-            fresh |= j == 0 || sum_pages == kSumPages<kF32>;
-            if (fresh) {
-                if (j > 0) take_sum(u - 1, sum_scale, live);
-                const float mn = fmaxf(m, fmaxf(top, s.xmax[u & 1][half ^ 1][row]));
-                const float keep = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
-                if (__any_sync(0xffffffffu, keep != 1.f)) {
-                    const uint64_t k2 = pair(keep, keep);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) acc[i] = mul2(acc[i], k2);
-                    l *= keep;
-                }
+            named_bar_sync(pair_bar, 64);
+            const float mn = fmaxf(m, fmaxf(top, s.xmax[u & 1][half ^ 1][row]));
+            float keep = 1.f;
+            const bool raised = __any_sync(0xffffffffu, mn > m + kHeadroom);  // the same in both warps of the rows
+            if (raised) {
+                keep = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
+                l *= keep;
                 m = mn;
-                if (kF32) sum_scale = pm.values;
-                shift = 0, sum_pages = 0;
             }
-            ++sum_pages;
+            const float old_scale = sum_scale;
+            sum_scale = page.y;
+            const bool fresh = j % kSumPages<kF32> == 0;  // a new sum in TMEM
             if (run) {
-                const float base = (kF32 ? 4.f + (float)shift : 0.f) - (m == -INFINITY ? 0.f : m);
+                const float base = (kF32 ? kLift : 0.f) - (m == -INFINITY ? 0.f : m);
                 const uint64_t q2 = pair(factor, factor), s2 = pair(base, base);
                 uint64_t sum2[2] = {0, 0};
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    uint32_t p0, p1;
+                    unpair(fma2(pair(x[2 * i], x[2 * i + 1]), q2, s2), p0, p1);
+                    x[2 * i] = __float_as_uint(exp2_fast(__uint_as_float(p0)));
+                    x[2 * i + 1] = __float_as_uint(exp2_fast(__uint_as_float(p1)));
+                }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t hi[8], lo[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        uint32_t p0, p1;
-                        unpair(fma2(pair(x[c * 16 + 2 * i], x[c * 16 + 2 * i + 1]), q2, s2), p0, p1);
-                        const float e0 = exp2_fast(__uint_as_float(p0)), e1 = exp2_fast(__uint_as_float(p1));
+                        const uint32_t e0 = x[c * 16 + 2 * i], e1 = x[c * 16 + 2 * i + 1];
                         sum2[i & 1] = add2(sum2[i & 1], pair(e0, e1));
-                        if constexpr (kF32) split2(e0, e1, hi[i], lo[i]);
-                        else hi[i] = pack_bf16(e0, e1);
+                        if constexpr (kF32) split2(__uint_as_float(e0), __uint_as_float(e1), hi[i], lo[i]);
+                        else hi[i] = pack_bf16(__uint_as_float(e0), __uint_as_float(e1));
                     }
                     // in the place of the 16 scores
                     tmem_st<8>(sa + c * 16, hi);
@@ -701,17 +740,18 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
                 }
                 uint32_t u0, u1;
                 unpair(add2(sum2[0], sum2[1]), u0, u1);
-                l += (__uint_as_float(u0) + __uint_as_float(u1)) * (kF32 ? __uint_as_float((uint32_t)(127 - shift) << 23) : 1.f);
+                l += __uint_as_float(u0) + __uint_as_float(u1);
                 tmem_wait_st();
                 tc_fence_before();
             }
-            if (lane == 0) s.fresh[u & 1] = fresh;
+            // the sum that ends here: its last product has run meanwhile
+            if (j > 0 && (fresh || raised)) take_sum(u - 1, old_scale, keep, fresh, live);
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.p_full[u & 1]);
             const uint4 bad = *reinterpret_cast<const uint4*>(pm.bad);
             if (bad.x | bad.y | bad.z | bad.w) add_bad(now, u, now.t.page(now.j + j), pos);
         }
-        take_sum(unit0 + n - 1, sum_scale, live);
+        take_sum(unit0 + n - 1, sum_scale, 1.f, true, live);
         unit0 += n;
         // rows of the tile to rows of out by way of shared memory, 64 bytes (fp32: 16 columns) of each half a round; or
         // to the workspace, column by column
@@ -790,12 +830,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs 
     extern __shared__ unsigned char raw[];
     __shared__ Shared s;
     unsigned char* ring = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int g = a.heads / a.kv_heads;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxStages; ++i) mbar_init(&s.full[i], 1), mbar_init(&s.empty[i], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&s.s_full[i], 1), mbar_init(&s.p_full[i], kTeamWarps), mbar_init(&s.pv_full[i], 1);
-        mbar_init(&s.pv_free, kTeamWarps), mbar_init(&s.q_full, kTeamWarps), mbar_init(&s.drain[0], 1), mbar_init(&s.drain[1], 1);
+        mbar_init(&s.pv_free, kTeamWarps), mbar_init(&s.q_full, kTeamWarps), mbar_init(&s.drain, 1);
         fence_mbar_init();
         s.abort = 0;
     }
@@ -810,10 +850,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs 
         team_role<kF32>(a, s, ring + kStages<kF32> * kOperandBytes<kF32>, im, parts, g);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (threadIdx.x == 32 * kTeamWarps) {
-            mma_role<kF32, false>(a, s, ring, g, s.walk[kTeamWarps]);
-        } else if (threadIdx.x == 32 * (kTeamWarps + 2)) {
-            mma_role<kF32, true>(a, s, ring, g, s.walk[kTeamWarps + 2]);
+        if (warp == kTeamWarps) {
+            mma_role<kF32>(a, s, ring, g);
         } else if (threadIdx.x == 32 * (kTeamWarps + 1)) {
             fence_proxy_async_smem();  // the ring was find_run's scratch
             pdl_wait_prior_grid();
