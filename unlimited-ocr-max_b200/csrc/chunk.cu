@@ -91,15 +91,21 @@ struct Shared {
     float xmax[2][2][kTile], xsum[2][kTile];
 };
 
-// A whole warp's bounded wait: one lane polls (32 lanes' polls take several times as long), the others follow.
+// Has the phase of `parity` completed? (No suspension, unlike try_wait.)
+UOCR_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(smem_addr(bar)), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+// A whole warp's bounded wait.
 UOCR_DEV bool wait(Shared& s, uint64_t* bar, uint32_t parity) {
-    uint32_t ok = 1;
-    if ((threadIdx.x & 31) == 0 && !mbar_try_wait(bar, parity)) {
-        const uint64_t t0 = global_timer_ns();
-        while (ok && !mbar_try_wait(bar, parity)) ok = !s.abort && global_timer_ns() - t0 <= kWaitBudgetNs;
-        if (!ok) s.abort = 1;
-    }
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+    if (mbar_wait_warp(bar, parity, &s.abort, nullptr)) return true;
+    s.abort = 1;
+    return false;
 }
 
 // ---- tensor-core operands ---------------------------------------------------------------------
@@ -440,7 +446,7 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
     const uint32_t base = smem_addr(ring), me = elect_one();
     Walk& w = s.walk[kTeamWarps];
     uint32_t stage = 0, phase = 0, unit0 = 0, seg = 0, sums = 0;  // sums: begun so far in TMEM
-    auto look = [&](uint64_t* bar, uint32_t parity) { return mbar_try_wait(bar, parity); };
+    auto look = [&](uint64_t* bar, uint32_t parity) { return mbar_test(bar, parity); };
     // the operand `ahead` of the next one
     auto full = [&](uint32_t ahead) {
         const bool wraps = stage + ahead >= kStages<kF32>;
@@ -647,7 +653,8 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
         m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[i] = 0;
-        const int n = now.n;
+        const int n = now.n, first_pos = now.t.first_pos, last_pos = now.t.last_pos, prefix = now.r.prefix;
+        const int head_pages = now.t.head_pages - now.j, tail_page = now.t.tail_page - head_pages;  // page of the segment's j
         float sum_scale = 1.f;  // of the sum in TMEM
         for (int j = 0;; ++j) {
             if (j == n) {  // the next segment's queries, while the last products run
@@ -657,16 +664,17 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
                 break;
             }
             const uint32_t u = unit0 + j, sa = lanes + kColS + (u & 1) * 128 + half * 64;
-            const int c0 = now.t.page(now.j + j) * kPageRows;
+            const int c0 = (j < head_pages ? now.j + j : j + tail_page) * kPageRows;
             if (alive && !wait(s, &s.s_full[u & 1], (u >> 1) & 1)) alive = false;
             tc_fence_after();
             const bool run = alive && live;
             // does every row of the tile see the whole page?
-            const bool all = c0 + kPageRows - 1 <= now.t.first_pos &&
-                             (a.window <= 0 || c0 > now.t.last_pos - a.window || c0 + kPageRows <= now.r.prefix);
+            const bool all = c0 + kPageRows - 1 <= first_pos &&
+                             (a.window <= 0 || c0 > last_pos - a.window || c0 + kPageRows <= prefix);
             // keys of one scale: it goes into the factor; else 1 / scale of each one's key (a branch, rarely taken)
             const PageMeta& pm = s.meta[u & 7];
             const float2 page = kF32 ? *reinterpret_cast<const float2*>(&pm.all_keys) : make_float2(1.f, 1.f);
+            const uint4 bad = *reinterpret_cast<const uint4*>(pm.bad);
             const float all_keys = page.x, factor = kF32 && all_keys != 0.f ? fmaxf(qscale * all_keys, 1e-37f) : qscale;
             uint32_t x[64];
             float top = -INFINITY;
@@ -686,7 +694,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
                     const int lo = a.window > 0 ? pos - a.window + 1 - c0 : -kPageRows;
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const uint32_t mask = seen_mask(half * 64 + c * 32, pos - c0, lo, now.r.prefix - c0);
+                        const uint32_t mask = seen_mask(half * 64 + c * 32, pos - c0, lo, prefix - c0);
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if (!(mask >> i & 1)) x[c * 32 + i] = 0xFF800000u;
@@ -748,8 +756,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
             if (j > 0 && (fresh || raised)) take_sum(u - 1, old_scale, keep, fresh, live);
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.p_full[u & 1]);
-            const uint4 bad = *reinterpret_cast<const uint4*>(pm.bad);
-            if (bad.x | bad.y | bad.z | bad.w) add_bad(now, u, now.t.page(now.j + j), pos);
+            if (bad.x | bad.y | bad.z | bad.w) add_bad(now, u, c0 / kPageRows, pos);
         }
         take_sum(unit0 + n - 1, sum_scale, 1.f, true, live);
         unit0 += n;
