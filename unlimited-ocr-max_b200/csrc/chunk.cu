@@ -37,7 +37,7 @@ namespace uocr {
 namespace {
 
 constexpr int kTile = 128;      // (token, head) rows of a query tile
-constexpr int kLead = 6;        // what a tile costs beside its pages
+constexpr int kLead = 3;        // what a tile costs beside its pages
 constexpr int kTeamWarps = 8;   // softmax; then a warpgroup: the issuing warp, the copying warp and two idle ones
 constexpr int kThreads = 32 * (kTeamWarps + 4);
 constexpr int kLaunchRegs = 168, kTeamRegs = 216, kOtherRegs = 72;  // a thread
@@ -50,8 +50,6 @@ template <bool kF32>
 constexpr int kStages = kF32 ? 3 : 6;  // of operands in shared memory
 constexpr int kMaxStages = 6;
 constexpr uint32_t kTeamBar = 1, kPairBar = 2;  // all softmax warps; the two warps of 32 rows (kPairBar + 0..3)
-constexpr int kStagingBytes = kTile * 128;  // a quarter (fp32) or half (bf16) of a tile's rows, between the row-wise and the
-                                            // lane-wise order; 16-byte chunks swizzled by the row
 
 // TMEM columns
 constexpr uint32_t kColS = 0, kColPv = 256, kColQ = 384;
@@ -544,7 +542,7 @@ UOCR_DEV uint32_t seen_mask(int c0, int hi, int lo, int pre) {
 }
 
 template <bool kF32>
-__device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging, const Images& im, const ChunkParts& parts, int g) {
+__device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const ChunkParts& parts, int g) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM address: lane from bit 16 up, 32 lanes a warp; columns from 0
@@ -552,26 +550,22 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
     bool alive = true;
     const uint32_t tid = threadIdx.x;
     const uint32_t pair_bar = kPairBar + (warp & 3);
-    auto chunk = [&](int row, int c) { return staging + row * 128 + ((c ^ (row & 7)) << 4); };
 
     // A segment's queries into TMEM (half 0 of the threads the hi halves, half 1 the lo ones; bf16: half the dimensions
     // each), once all have read the last one's scores.
     auto load_query = [&](const Walk& w) __attribute__((always_inline)) {
         const size_t index = (size_t)(query_base(w.r, w.b, g) + w.qt) * a.pass_heads + w.head;
         const uint4* p = reinterpret_cast<const uint4*>(im.queries + index * kQueryBytes<kF32>) + half * (kF32 ? 16 : 8) * kTile + row;
-        named_bar_sync(kTeamBar, 32 * kTeamWarps);
+        uint32_t x[kF32 ? 64 : 32];
 #pragma unroll
-        for (int h = 0; h < (kF32 ? 2 : 1); ++h) {
-            uint32_t x[32];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint4 v = ldg_nc_v4(p + (h * 8 + i) * kTile);
-                x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_st<8>(lanes + kColQ + half * (kF32 ? 64 : 32) + h * 32 + i * 8, x + 8 * i);
+        for (int i = 0; i < (kF32 ? 16 : 8); ++i) {
+            const uint4 v = ldg_nc_v4(p + i * kTile);
+            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
         }
         qscale = __ldg(im.qscale + index * kTile + row);
+        named_bar_sync(kTeamBar, 32 * kTeamWarps);
+#pragma unroll
+        for (int i = 0; i < (kF32 ? 8 : 4); ++i) tmem_st<8>(lanes + kColQ + half * (kF32 ? 64 : 32) + i * 8, x + 8 * i);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -638,7 +632,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
     };
 
     Walk& w = s.walk[warp];
-    Walk& now = s.now[warp];  // the segment at work, while w is one ahead
+    Walk& now = s.now[warp];  // the segment at work
     bool more = w.begin(a, s.run, g, kTile, kLead);
     __syncwarp();
     int state[2] = {0, 0}, place[4] = {0, 0, 0, 0};
@@ -653,13 +647,13 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
         m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[i] = 0;
+        more = w.next(a, g, kTile, kLead);  // w is one ahead from here on
+        __syncwarp();
         const int n = now.n, first_pos = now.t.first_pos, last_pos = now.t.last_pos, prefix = now.r.prefix;
         const int head_pages = now.t.head_pages - now.j, tail_page = now.t.tail_page - head_pages;  // page of the segment's j
         float sum_scale = 1.f;  // of the sum in TMEM
         for (int j = 0;; ++j) {
             if (j == n) {  // the next segment's queries, while the last products run
-                more = w.next(a, g, kTile, kLead);
-                __syncwarp();
                 if (more) load_query(w);
                 break;
             }
@@ -760,52 +754,35 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
         }
         take_sum(unit0 + n - 1, sum_scale, 1.f, true, live);
         unit0 += n;
-        // rows of the tile to rows of out by way of shared memory, 64 bytes (fp32: 16 columns) of each half a round; or
-        // to the workspace, column by column
+        // to out, or column by column to the workspace
         s.xsum[half][row] = l;
-        named_bar_sync(kTeamBar, 32 * kTeamWarps);
+        named_bar_sync(pair_bar, 64);
         const float total = s.xsum[0][row] + s.xsum[1][row];
         const bool whole = now.whole();
         const float f = !alive ? NAN : whole ? 1.f / total : 1.f;
         const uint64_t f2 = pair(f, f);
         const int slot = now.j == 0 ? 1 : 0;
         float* part = parts.slots + ((size_t)blockIdx.x * 2 + slot) * slot_floats(kTile);
-        if (whole) {
-            constexpr int kElt = kF32 ? 4 : 2;
-            const int row8 = tid >> 3, c8 = tid & 7;
-            char* to[4];
+        if (whole && row < rows) {
+            const size_t at = ((size_t)(now.r.lo + R / g) * a.heads + (a.head0 + now.head) * g + R % g) * kDim + half * 64;
+            auto two = [&](int i) {
+                uint32_t y0, y1;
+                unpair(mul2(acc[i], f2), y0, y1);
+                return pack_bf16(__uint_as_float(y0), __uint_as_float(y1));
+            };
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int T = now.qt * kTile + k * 32 + row8;
-                to[k] = static_cast<char*>(a.out) +
-                        (((size_t)(now.r.lo + T / g) * a.heads + (a.head0 + now.head) * g + T % g) * kDim + (c8 >> 2) * 64 + (c8 & 3) * 4) *
-                            kElt;
-            }
-            // a loop: run once a tile, its instructions come from far
-#pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint4 v;
-                    unpair(mul2(acc[2 * c], f2), v.x, v.y);
-                    unpair(mul2(acc[2 * c + 1], f2), v.z, v.w);
-                    *reinterpret_cast<uint4*>(chunk(row, half * 4 + c)) = v;
+            for (int i = 0; i < (kF32 ? 16 : 8); ++i) {
+                uint4 v;
+                if constexpr (kF32) {
+                    unpair(mul2(acc[2 * i], f2), v.x, v.y);
+                    unpair(mul2(acc[2 * i + 1], f2), v.z, v.w);
+                    reinterpret_cast<uint4*>(static_cast<float*>(a.out) + at)[i] = v;
+                } else {
+                    v = make_uint4(two(4 * i), two(4 * i + 1), two(4 * i + 2), two(4 * i + 3));
+                    reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at)[i] = v;
                 }
-                named_bar_sync(kTeamBar, 32 * kTeamWarps);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (k * 32 + row8 >= rows) continue;
-                    const uint4 v = *reinterpret_cast<const uint4*>(chunk(k * 32 + row8, c8));
-                    if constexpr (kF32) *reinterpret_cast<uint4*>(to[k]) = v;
-                    else *reinterpret_cast<uint2*>(to[k]) = make_uint2(pack_bf16(__uint_as_float(v.x), __uint_as_float(v.y)),
-                                                                       pack_bf16(__uint_as_float(v.z), __uint_as_float(v.w)));
-                    to[k] += 16 * kElt;
-                }
-#pragma unroll
-                for (int k = 0; k < 24; ++k) acc[k] = acc[k + 8];
-                named_bar_sync(kTeamBar, 32 * kTeamWarps);
             }
-        } else if (row < rows) {
+        } else if (!whole && row < rows) {
             float* o = part + half * 64 * kTile + row;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
@@ -814,7 +791,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, unsigned char* staging,
                 o[2 * i * kTile] = __uint_as_float(y0), o[(2 * i + 1) * kTile] = __uint_as_float(y1);
             }
         }
-        named_bar_sync(kTeamBar, 32 * kTeamWarps);
+        named_bar_sync(pair_bar, 64);  // xsum is free again
         if (!whole) {
             if (half == 0 && row < rows) {
                 part[kDim * kTile + row] = m;
@@ -854,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs 
     if (warp < kTeamWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTeamRegs));
         pdl_wait_prior_grid();
-        team_role<kF32>(a, s, ring + kStages<kF32> * kOperandBytes<kF32>, im, parts, g);
+        team_role<kF32>(a, s, im, parts, g);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == kTeamWarps) {
@@ -883,27 +860,40 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a, ChunkParts
     const int ctas = p.ctas, tile = p.tile;
     const size_t slot = slot_floats(tile);
     const int c = blockIdx.x, g = a.heads / a.kv_heads;
-    const int* o = info + c * kInfoInts;
-    if (o[1] == 0) return;
-    const int lo = o[2], r0 = o[3], rows = o[4], head = o[5];
+    const int4 head4 = *reinterpret_cast<const int4*>(info + c * kInfoInts);      // states, lo, first row
+    const int2 tail2 = *reinterpret_cast<const int2*>(info + c * kInfoInts + 4);  // rows, head
+    if (head4.y == 0) return;
+    // one behind the last CTA of this tile: the states of 32 CTAs at a time
+    int end = c + 1;
+    for (;; end += 32) {
+        const int d = end + (threadIdx.x & 31);
+        const uint32_t last = __ballot_sync(0xffffffffu, d >= ctas || info[d * kInfoInts] != 1);
+        if (last) {
+            end = min(end + __ffs(last), ctas);
+            break;
+        }
+    }
+    const int lo = head4.z, r0 = head4.w, rows = tail2.x, head = tail2.y;
     // threads by row, then by 8 columns: few rows take few threads' time
     const int group = blockIdx.y * (256 / tile) + threadIdx.x / tile, row = threadIdx.x % tile, c0 = group * 8;
     if (row >= rows || group >= kDim / 8) return;
-    int end = c + 1;  // one behind the last CTA of this tile
-    while (end < ctas && info[end * kInfoInts] == 1) ++end;
-    end = min(end + 1, ctas);
-    float M = -INFINITY;
-    for (int d = c; d < end; ++d) M = fmaxf(M, slots[((size_t)d * 2 + (d == c)) * slot + kDim * tile + row]);
-    float l = 0.f, x[8];
+    // a running maximum, the next part on its way
+    float M = -INFINITY, l = 0.f, x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.f;
+#pragma unroll 4
     for (int d = c; d < end; ++d) {
         const float* part = slots + ((size_t)d * 2 + (d == c)) * slot;
-        const float md = part[kDim * tile + row];
-        const float f = md == -INFINITY ? 0.f : exp2_fast(md - M);  // a part in which the row sees nothing
-        l = fmaf(part[(kDim + 1) * tile + row], f, l);
+        const float md = part[kDim * tile + row], ld = part[(kDim + 1) * tile + row];
+        float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fmaf(part[(c0 + i) * tile + row], f, x[i]);
+        for (int i = 0; i < 8; ++i) y[i] = part[(c0 + i) * tile + row];
+        const float mn = fmaxf(M, md), base = mn == -INFINITY ? 0.f : mn;  // -inf: parts in which the row sees nothing
+        const float keep = exp2_fast(M - base), f = exp2_fast(md - base);
+        M = mn;
+        l = fmaf(ld, f, l * keep);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = fmaf(y[i], f, x[i] * keep);
     }
     const float inv = 1.f / l;
     const int R = r0 + row;
@@ -935,7 +925,7 @@ int query_tiles(const ChunkArgs& a) { return (int)((long long)a.T * (a.heads / a
 
 template <bool kF32>
 cudaError_t launch(const ChunkArgs& a, const Images& im, const ChunkParts& parts, cudaStream_t st) {
-    const size_t smem = (size_t)kStages<kF32> * kOperandBytes<kF32> + kStagingBytes + 1024;
+    const size_t smem = (size_t)kStages<kF32> * kOperandBytes<kF32> + 1024;
     auto kernel = chunk_attention_kernel<kF32>;
     cudaError_t err = ensure_smem_optin(reinterpret_cast<const void*>(kernel), smem);
     if (err != cudaSuccess) return err;
@@ -973,13 +963,15 @@ cudaError_t launch_chunk_join(const ChunkArgs& a, const ChunkParts& p, cudaStrea
     return launch_dependent(a.bf16 ? chunk_join_kernel<false> : chunk_join_kernel<true>, grid, 256, 0, st, a, p);
 }
 
-// Rows of a query tile: 1, 2, 4 or 8 where a request has up to 8 (token, head) rows of a KV head on average
-// (chunk_rows.cu: bound by the cache's bytes), else 128 (tensor cores).
+// Rows of a query tile: where a request has up to 8 (token, head) rows of a KV head on average, 1, 2, 4 or 8
+// (chunk_rows.cu: bound by the cache's bytes; twice the average less one, since the requests differ and a second
+// tile reads the cache again), else 128 (tensor cores).
 static int tile_rows(const ChunkArgs& a) {
     const long long rows = (long long)a.T * (a.heads / a.kv_heads);
-    for (int t = 1; t <= 8; t *= 2)
-        if (rows <= (long long)t * a.B) return t;
-    return kTile;
+    if (rows > 8ll * a.B) return kTile;
+    int t = 1;
+    while (t < 8 && 2 * rows - a.B > (long long)t * a.B) t *= 2;
+    return t;
 }
 
 size_t chunk_workspace_bytes(const ChunkArgs& a, int sms) {
