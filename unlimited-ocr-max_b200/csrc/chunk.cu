@@ -161,29 +161,6 @@ UOCR_DEV void tmem_ld64(uint32_t addr, uint32_t (&x)[64]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[32]), "+r"(x[33]), "+r"(x[34]), "+r"(x[35]), "+r"(x[36]), "+r"(x[37]), "+r"(x[38]), "+r"(x[39]), "+r"(x[40]), "+r"(x[41]), "+r"(x[42]), "+r"(x[43]), "+r"(x[44]), "+r"(x[45]), "+r"(x[46]), "+r"(x[47]) : : "memory");
     asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(x[48]), "+r"(x[49]), "+r"(x[50]), "+r"(x[51]), "+r"(x[52]), "+r"(x[53]), "+r"(x[54]), "+r"(x[55]), "+r"(x[56]), "+r"(x[57]), "+r"(x[58]), "+r"(x[59]), "+r"(x[60]), "+r"(x[61]), "+r"(x[62]), "+r"(x[63]) : : "memory");
 }
-// Two fp32 operations an instruction (each rounded as its scalar form).
-UOCR_DEV uint64_t pair(uint32_t x, uint32_t y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
-    return r;
-}
-UOCR_DEV uint64_t pair(float x, float y) { return pair(__float_as_uint(x), __float_as_uint(y)); }
-UOCR_DEV void unpair(uint64_t v, uint32_t& x, uint32_t& y) { asm("mov.b64 {%0, %1}, %2;" : "=r"(x), "=r"(y) : "l"(v)); }
-UOCR_DEV uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-UOCR_DEV uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-UOCR_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 UOCR_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // two values as fp16 halves: hi takes the upper 11 bits (exactly), lo the rest (rounded to 11 bits)
@@ -963,15 +940,15 @@ cudaError_t launch_chunk_join(const ChunkArgs& a, const ChunkParts& p, cudaStrea
     return launch_dependent(a.bf16 ? chunk_join_kernel<false> : chunk_join_kernel<true>, grid, 256, 0, st, a, p);
 }
 
-// Rows of a query tile: where a request has up to 8 (token, head) rows of a KV head on average, 1, 2, 4 or 8
+// Rows of a query tile: where a request has up to 8 (token, head) rows of a KV head on average, 1 to 8
 // (chunk_rows.cu: bound by the cache's bytes; twice the average less one, since the requests differ and a second
 // tile reads the cache again), else 128 (tensor cores).
 static int tile_rows(const ChunkArgs& a) {
     const long long rows = (long long)a.T * (a.heads / a.kv_heads);
     if (rows > 8ll * a.B) return kTile;
-    int t = 1;
-    while (t < 8 && 2 * rows - a.B > (long long)t * a.B) t *= 2;
-    return t;
+    for (int t : {1, 2, 3, 4, 6})
+        if (2 * rows - a.B <= (long long)t * a.B) return t;
+    return 8;
 }
 
 size_t chunk_workspace_bytes(const ChunkArgs& a, int sms) {

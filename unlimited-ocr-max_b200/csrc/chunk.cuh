@@ -194,5 +194,29 @@ UOCR_DEV float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two fp32 operations an instruction (each rounded as its scalar form).
+UOCR_DEV uint64_t pair(uint32_t x, uint32_t y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
+    return r;
+}
+UOCR_DEV uint64_t pair(float x, float y) { return pair(__float_as_uint(x), __float_as_uint(y)); }
+UOCR_DEV void unpair(uint64_t v, uint32_t& x, uint32_t& y) { asm("mov.b64 {%0, %1}, %2;" : "=r"(x), "=r"(y) : "l"(v)); }
+UOCR_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+UOCR_DEV uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+UOCR_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 }  // namespace
 }  // namespace uocr

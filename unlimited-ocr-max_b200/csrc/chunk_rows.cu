@@ -9,6 +9,8 @@
 // v lies in all 32 lanes, 4 columns each. While a page's scores are computed its values are on their way, and the next
 // page's keys while the values are summed: 64 KB of k and 64 KB of v a SM (fp32). The warps' results are joined
 // when a tile's run of pages ends, the runs' results by the joining launch.
+#include <type_traits>
+
 #include "chunk.cuh"
 
 namespace uocr {
@@ -22,8 +24,8 @@ struct Shared {
     Run run;
     Walk walk[kWarps];
     float4 q[2][NQ][kDim / 4];           // this segment's queries and the next one's, times scale log2(e)
-    float p[kWarps][16][NQ];             // a warp's weights; -0 for a row that is not seen
-    float sum[kWarps][NQ][kDim];
+    float2 p[kWarps][16][NQ];            // a warp's weights, twice each; -0 for a row that is not seen
+    alignas(16) float sum[kWarps][NQ][kDim];
     float m[kWarps][NQ], l[kWarps][NQ];
 };
 
@@ -32,7 +34,6 @@ UOCR_DEV float warp_max(float v) {
     asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
-UOCR_DEV uint2 ldg_stream2(const void* p) { return ldg_nc_v2(p); }
 
 // The words of a warp's 16 rows of a page. k: word (i, c) is row 4 i + lane / 8, 16 bytes lane % 8 + 8 c; v: word r is
 // row r, 4 columns of this lane.
@@ -73,29 +74,50 @@ UOCR_DEV Place place_of(const ChunkArgs& a, const Walk& w, int j, uint32_t id, i
 template <bool kF32>
 UOCR_DEV void load_keys(const ChunkArgs& a, const Place& p, int row0, int lane, Words<kF32>& x) {
     using W = Words<kF32>;
+    const int first = row0 + (lane >> 3);
     const size_t row_bytes = (size_t)a.kv_heads * (kDim * W::kElt);
+    const char* s = p.k_pool + first * row_bytes + (lane & 7) * 16;
+    if (p.cached >= kPageRows) {  // the whole page is cached: addresses by addition
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = row0 + 4 * i + (lane >> 3);
-        const char* s = (row < p.cached ? p.k_pool + row * row_bytes : p.k_new + row * (a.k_ld * W::kElt)) + (lane & 7) * 16;
+        for (int i = 0; i < 4; ++i, s += 4 * row_bytes)
 #pragma unroll
-        for (int c = 0; c < W::kChunks; ++c) x.k[i][c] = row < p.known ? ldg_nc_v4(s + c * 128) : make_uint4(0, 0, 0, 0);
+            for (int c = 0; c < W::kChunks; ++c) x.k[i][c] = ldg_nc_v4(s + c * 128);
+        return;
+    }
+    const long long ld = a.k_ld * W::kElt;
+    const char* f = p.k_new + first * ld + (lane & 7) * 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i, s += 4 * row_bytes, f += 4 * ld) {
+        const int row = first + 4 * i;
+        const char* from = row < p.cached ? s : f;
+#pragma unroll
+        for (int c = 0; c < W::kChunks; ++c) x.k[i][c] = row < p.known ? ldg_nc_v4(from + c * 128) : make_uint4(0, 0, 0, 0);
     }
 }
 template <bool kF32>
 UOCR_DEV void load_values(const ChunkArgs& a, const Place& p, int row0, int lane, Words<kF32>& x) {
     using W = Words<kF32>;
-    const size_t row_bytes = (size_t)a.kv_heads * (kDim * W::kElt);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int row = row0 + r;
-        const char* s = (row < p.cached ? p.v_pool + row * row_bytes : p.v_new + row * (a.v_ld * W::kElt)) + lane * (kF32 ? 16 : 8);
+    auto load = [&](int r, const char* from) {
         if constexpr (kF32) {
-            const uint4 v = row < p.known ? ldg_nc_v4(s) : make_uint4(0, 0, 0, 0);
+            const uint4 v = ldg_nc_v4(from);
             x.v[r][0] = make_uint2(v.x, v.y), x.v[r][1] = make_uint2(v.z, v.w);
         } else {
-            x.v[r][0] = row < p.known ? ldg_stream2(s) : make_uint2(0, 0);
+            x.v[r][0] = ldg_nc_v2(from);
         }
+    };
+    const size_t row_bytes = (size_t)a.kv_heads * (kDim * W::kElt);
+    const char* s = p.v_pool + row0 * row_bytes + lane * (kF32 ? 16 : 8);
+    if (p.cached >= kPageRows) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r, s += row_bytes) load(r, s);
+        return;
+    }
+    const long long ld = a.v_ld * W::kElt;
+    const char* f = p.v_new + row0 * ld + lane * (kF32 ? 16 : 8);
+#pragma unroll
+    for (int r = 0; r < 16; ++r, s += row_bytes, f += ld) {
+        x.v[r][0] = x.v[r][kF32 ? 1 : 0] = make_uint2(0, 0);
+        if (row0 + r < p.known) load(r, row0 + r < p.cached ? s : f);
     }
 }
 
@@ -157,9 +179,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(ChunkArgs a, Ch
     __syncthreads();
     for (int buf = 0; more; buf ^= 1) {
         float m[NQ], l[NQ];
-        float4 acc[NQ];
+        uint64_t acc[NQ][2];  // 4 columns, in pairs
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) m[j] = -INFINITY, l[j] = 0.f, acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < NQ; ++j) m[j] = -INFINITY, l[j] = 0.f, acc[j][0] = acc[j][1] = 0;
         const int n = w.n, qt = w.qt, head = w.head, lo = w.r.lo, start = w.r.start, prefix = w.r.prefix;
         const int rows = min(NQ, w.r.n * g - qt * NQ);
         const bool whole = w.whole(), begins = w.j == 0, ends = w.j + w.n == w.t.count;
@@ -176,28 +198,36 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(ChunkArgs a, Ch
             float sc[NQ];
 #pragma unroll
             for (int j = 0; j < NQ; ++j) {
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                uint64_t d2[4] = {0, 0, 0, 0};  // sums over even and odd dimensions
+                // (a constant index for every register: the loop over c is unrolled)
 #pragma unroll
                 for (int c = 0; c < W::kChunks; ++c) {
                     if constexpr (kF32) {
                         const float4 q = s.q[buf][j][(lane & 7) + 8 * c];
+                        const uint64_t q0 = pair(q.x, q.y), q1 = pair(q.z, q.w);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const uint4& k = x.k[i][c];
-                            d[i] = fmaf(q.x, __uint_as_float(k.x), d[i]), d[i] = fmaf(q.y, __uint_as_float(k.y), d[i]);
-                            d[i] = fmaf(q.z, __uint_as_float(k.z), d[i]), d[i] = fmaf(q.w, __uint_as_float(k.w), d[i]);
+                            d2[i] = fma2(q1, pair(k.z, k.w), fma2(q0, pair(k.x, k.y), d2[i]));
                         }
                     } else {
-                        const float4 q0 = s.q[buf][j][2 * ((lane & 7) + 8 * c)], q1 = s.q[buf][j][2 * ((lane & 7) + 8 * c) + 1];
+                        const float4 qa = s.q[buf][j][2 * ((lane & 7) + 8 * c)], qb = s.q[buf][j][2 * ((lane & 7) + 8 * c) + 1];
+                        const uint64_t q0 = pair(qa.x, qa.y), q1 = pair(qa.z, qa.w), q2 = pair(qb.x, qb.y), q3 = pair(qb.z, qb.w);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            float k[8];
-                            unpack_bf16x8(x.k[i][c], k);
-                            d[i] = fmaf(q0.x, k[0], d[i]), d[i] = fmaf(q0.y, k[1], d[i]), d[i] = fmaf(q0.z, k[2], d[i]);
-                            d[i] = fmaf(q0.w, k[3], d[i]), d[i] = fmaf(q1.x, k[4], d[i]), d[i] = fmaf(q1.y, k[5], d[i]);
-                            d[i] = fmaf(q1.z, k[6], d[i]), d[i] = fmaf(q1.w, k[7], d[i]);
+                            const uint4& k = x.k[i][c];
+                            auto two = [](uint32_t w) { return pair(w << 16, w & 0xFFFF0000u); };
+                            d2[i] = fma2(q1, two(k.y), fma2(q0, two(k.x), d2[i]));
+                            d2[i] = fma2(q3, two(k.w), fma2(q2, two(k.z), d2[i]));
                         }
                     }
+                }
+                float d[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t e, o;
+                    unpair(d2[i], e, o);
+                    d[i] = __uint_as_float(e) + __uint_as_float(o);
                 }
                 // 4 sums over 8 lanes: lanes with bit 2 take sums 2 and 3, with bit 1 the second of their two
                 const bool up2 = lane & 4, up1 = lane & 2;
@@ -230,8 +260,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(ChunkArgs a, Ch
                 const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m[j] - mn);
                 m[j] = mn;
                 l[j] = l[j] * alpha + p;
-                acc[j].x *= alpha, acc[j].y *= alpha, acc[j].z *= alpha, acc[j].w *= alpha;
-                if (!(lane & 1)) s.p[warp][mine][j] = seen ? p : -0.f;
+                const uint64_t a2 = pair(alpha, alpha);
+                acc[j][0] = mul2(acc[j][0], a2), acc[j][1] = mul2(acc[j][1], a2);
+                if (!(lane & 1)) s.p[warp][mine][j] = seen ? make_float2(p, p) : make_float2(-0.f, -0.f);
             }
             __syncwarp();
             if (stores) {  // the new rows of v
@@ -245,21 +276,23 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(ChunkArgs a, Ch
                     else *reinterpret_cast<uint2*>(o) = x.v[r][0];
                 }
             }
+            auto add_rows = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float4 v;
-                if constexpr (kF32)
-                    v = make_float4(__uint_as_float(x.v[r][0].x), __uint_as_float(x.v[r][0].y), __uint_as_float(x.v[r][1].x),
-                                    __uint_as_float(x.v[r][1].y));
-                else v = make_float4(bf16lo(x.v[r][0].x), bf16hi(x.v[r][0].x), bf16lo(x.v[r][0].y), bf16hi(x.v[r][0].y));
+                for (int r = 0; r < 16; ++r) {
+                    uint64_t v0, v1;
+                    if constexpr (kF32) v0 = pair(x.v[r][0].x, x.v[r][0].y), v1 = pair(x.v[r][1].x, x.v[r][1].y);
+                    else v0 = pair(x.v[r][0].x << 16, x.v[r][0].x & 0xFFFF0000u), v1 = pair(x.v[r][0].y << 16, x.v[r][0].y & 0xFFFF0000u);
 #pragma unroll
-                for (int j = 0; j < NQ; ++j) {
-                    const float p = s.p[warp][r][j];
-                    if (!all && __float_as_int(p) < 0) continue;  // not seen: whatever the row holds stays out
-                    acc[j].x = fmaf(p, v.x, acc[j].x), acc[j].y = fmaf(p, v.y, acc[j].y);
-                    acc[j].z = fmaf(p, v.z, acc[j].z), acc[j].w = fmaf(p, v.w, acc[j].w);
+                    for (int j = 0; j < NQ; ++j) {
+                        const float2 p = s.p[warp][r][j];
+                        if (decltype(masked)::value && __float_as_int(p.x) < 0) continue;  // not seen: whatever the row holds stays out
+                        const uint64_t p2 = pair(p.x, p.y);
+                        acc[j][0] = fma2(p2, v0, acc[j][0]), acc[j][1] = fma2(p2, v1, acc[j][1]);
+                    }
                 }
-            }
+            };
+            if (all) add_rows(std::false_type{});
+            else add_rows(std::true_type{});
             __syncwarp();
             pl = next;
         }
@@ -277,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(ChunkArgs a, Ch
 #pragma unroll
             for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
             if (lane == 0) s.m[warp][j] = m[j], s.l[warp][j] = t;
-            *reinterpret_cast<float4*>(&s.sum[warp][j][4 * lane]) = acc[j];
+            *reinterpret_cast<ulonglong2*>(&s.sum[warp][j][4 * lane]) = make_ulonglong2(acc[j][0], acc[j][1]);
         }
         if (more) load_query(buf ^ 1);
         __syncthreads();
@@ -338,7 +371,9 @@ cudaError_t launch_chunk_rows(const ChunkArgs& a, const ChunkParts& parts, cudaS
     switch (parts.tile) {
         case 1: return a.bf16 ? launch<false, 1>(a, parts, st) : launch<true, 1>(a, parts, st);
         case 2: return a.bf16 ? launch<false, 2>(a, parts, st) : launch<true, 2>(a, parts, st);
+        case 3: return a.bf16 ? launch<false, 3>(a, parts, st) : launch<true, 3>(a, parts, st);
         case 4: return a.bf16 ? launch<false, 4>(a, parts, st) : launch<true, 4>(a, parts, st);
+        case 6: return a.bf16 ? launch<false, 6>(a, parts, st) : launch<true, 6>(a, parts, st);
         default: return a.bf16 ? launch<false, 8>(a, parts, st) : launch<true, 8>(a, parts, st);
     }
 }
