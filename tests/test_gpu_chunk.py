@@ -183,6 +183,117 @@ def test_strided_rows_of_a_fused_projection(ops, oracle, dtype):
     assert torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,start,heads,kv_heads,window,prefix", [
+    ([3, 1, 2, 0], [300, 129, 640, 5], 4, 2, 0, None), ([2] * 5, [128, 127, 255, 1, 0], 2, 2, 0, None),
+    ([3, 1, 2], [700, 400, 128], 2, 2, 64, [10, 0, 200]), ([1, 1], [600, 130], 8, 1, 1, None), ([4], [900], 6, 3, 130, [129]),
+    ([40] + [1] * 9, [200] + [37 * i for i in range(9)], 2, 2, 0, None),  # one request of many rows among single ones
+    ([9, 30, 7], [250, 100, 0], 2, 2, 40, [3, 100, 0]), ([16, 16], [300, 140], 1, 1, 0, None), ([6], [250], 2, 2, 0, None),
+])
+def test_few_rows(ops, oracle, dtype, n, start, heads, kv_heads, window, prefix):
+    """The form for few rows a request: tiles of 1 to 8 rows, several of them where a request has more."""
+    Case(dtype, n, start, heads=heads, kv_heads=kv_heads, seed=sum(n) + heads).check(ops, oracle, window=window, prefix=prefix)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_few_rows_and_what_they_do_not_see(ops, oracle, dtype):
+    """As test_what_a_row_does_not_see..., in the form for few rows: tokens in front of a key or value that is not
+    finite are untouched, those behind it take it in."""
+    for bad in (math.nan, math.inf):
+        c = Case(dtype, [4, 1], [100, 7], seed=22)
+        clean = c.run(ops)[0]
+        c.v[2, 1, 17] = bad
+        got = c.run(ops)[0]
+        assert torch.equal(got[:2], clean[:2]) and torch.equal(got[4:], clean[4:])
+        assert not torch.isfinite(got[2:4, 1, 17]).any() and torch.isfinite(got[2:4, 1, :17]).all()
+        c = Case(dtype, [4, 1], [100, 7], seed=22)
+        c.k[2, 1] = math.nan
+        got = c.run(ops)[0]
+        assert torch.equal(got[:2], clean[:2]) and torch.isnan(got[2:4, 1]).all() and torch.equal(got[:, 0], clean[:, 0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [[2, 3], [140, 20]])
+@pytest.mark.parametrize("factor", [-1.0, 0.0])
+def test_scales_below_and_at_zero(ops, oracle, dtype, n, factor):
+    c = Case(dtype, n, [50, 129], seed=23)
+    c.scale *= factor
+    c.check(ops, oracle)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_that_grow_along_the_cache(ops, oracle, dtype):
+    """Keys that grow from page to page, so that the maxima are raised over and over, and keys that shrink."""
+    for order in (1, -1):
+        c = Case(dtype, [200], [900], seed=24)
+        grow = torch.linspace(0.1, 8.0, 900)[::order] if order == 1 else torch.linspace(0.1, 8.0, 900).flip(0)
+        for r in range(900):
+            c.pool[c.lut[0, r // 128], 0, c.layer, r % 128] *= grow[r].to(dtype)
+        c.check(ops, oracle)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_requests(ops, oracle, dtype):
+    rng = np.random.default_rng(5)
+    for most, B in ((4, 300), (60, 70)):  # the forms for few rows and for many
+        n = rng.integers(0, most, B).tolist()
+        Case(dtype, n, rng.integers(0, 200, B).tolist(), heads=1, kv_heads=1, layers=1, layer=0, seed=B).check(ops, oracle)
+
+
+def test_a_table_far_wider_than_its_requests(ops, oracle):
+    """Most entries name the null page; the operands of all heads at once would pass a gigabyte, so that the heads
+    are taken in several passes."""
+    Case(torch.float32, [150, 30], [260, 0], heads=6, kv_heads=3, seed=25, lut_pad=2500).check(ops, oracle)
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import importlib, torch
+ops = importlib.import_module("unlimited-ocr-max_b200.ops")
+i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+for n, heads in ((200, 2), (2, 2)):
+    pool = torch.randn(4, 2, 1, 128, heads, 128, device="cuda")
+    q, k, v = (torch.randn(n, heads, 128, device="cuda") for _ in range(3))
+    lut, off, start, out = i([[0, 1, 2]]), i([0, n]), i([40]), torch.zeros_like(q)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.paged_chunk_attention(q, k, v, pool, 0, lut, off, start, 0.1, out=out)
+    assert not out.any()
+    g.replay()
+    want = ops.paged_chunk_attention(q, k, v, pool, 0, lut, off, start, 0.1)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_refusals(ops):
+    c = Case(torch.float32, [5], [10], seed=26)
+    q, k, v, pool, layer, lut, off, start, scale = _flat(c)
+    call = lambda **m: ops.paged_chunk_attention(*({"q": q, "k": k, "v": v, "pool": pool, "layer": layer, "lut": lut, "off": off,  # noqa: E731
+                                                   "start": start, "scale": scale} | m).values())
+    for bad, kind in (({"q": q.bfloat16()}, TypeError), ({"k": k[:, :1]}, ValueError), ({"v": v[:3]}, ValueError), ({"lut": lut.long()}, TypeError),
+                      ({"off": off[:1]}, ValueError), ({"start": start.long()}, TypeError), ({"layer": 2}, ValueError),
+                      ({"pool": pool[:, :, :, :64]}, ValueError), ({"pool": pool.transpose(3, 4)}, ValueError), ({"pool": pool.half()}, TypeError),
+                      ({"q": q[0]}, ValueError), ({"scale": math.inf}, ValueError), ({"k": pool[0, 0, 0, :5]}, ValueError)):
+        with pytest.raises(kind):
+            call(**bad)
+    with pytest.raises(ValueError, match="window"):
+        ops.paged_chunk_attention(q, k, v, pool, layer, lut, off, start, scale, window=-1)
+    with pytest.raises(ValueError, match="overlaps q"):
+        ops.paged_chunk_attention(q, k, v, pool, layer, lut, off, start, scale, out=q)
+    with pytest.raises(ValueError, match="out must be"):
+        ops.paged_chunk_attention(q, k, v, pool, layer, lut, off, start, scale, out=torch.empty_like(q).transpose(0, 1))
+
+
 def _flat(c):
     i32 = lambda a: torch.from_numpy(np.asarray(a, np.int32)).to(DEV)  # noqa: E731
     return [c.q.to(DEV), c.k.to(DEV), c.v.to(DEV), c.pool.to(DEV), c.layer, i32(c.lut), i32(c.offsets), i32(c.start),
