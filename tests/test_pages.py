@@ -34,6 +34,10 @@ def _chunk(lib, **v):
     ({"q_ld": 514}, 1, "row strides"), ({"k_ld": 128}, 1, "row strides"), ({"dtype": 1, "v_ld": 260}, 1, "row strides"),
     ({"scale": float("nan")}, 1, "scale"), ({"scale": float("inf")}, 1, "scale"), ({}, 1, "null pointer"),
     ({"T": 0}, 0, ""), ({"B": 0}, 0, ""),
+    ({"B": 8193}, 4, "8193 requests"), ({"B": 8192, "cols": 1 << 18}, 4, "tables of 8192"),
+    ({"B": 64, "cols": 1 << 22, "heads": 1024, "kv": 1024, "q_ld": 1 << 17, "k_ld": 1 << 17, "v_ld": 1 << 17}, 4, "too much"),
+    ({"B": 64, "cols": 1 << 19, "heads": 1024, "kv": 1024, "q_ld": 1 << 17, "k_ld": 1 << 17, "v_ld": 1 << 17}, 1, "null pointer"),
+    ({"T": 1 << 28, "cols": 1 << 22}, 4, "too much"), ({"window": 1 << 31}, 1, "window"), ({"cols": (1 << 22) + 1}, 1, "bad pool"),
 ])
 def test_chunk_attention_refusals(uocr, change, code, word):
     rc, err = _chunk(uocr.load(), **change)
