@@ -816,6 +816,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs 
         } else if (threadIdx.x == 32 * (kTeamWarps + 1)) {
             fence_proxy_async_smem();  // the ring was find_run's scratch
             pdl_wait_prior_grid();
+            fence_proxy_async_global();  // the operands were stored through the generic proxy
             copy_role<kF32>(a, s, ring, im, g);
         }
     }
