@@ -312,11 +312,13 @@ _CHUNK_WS: dict[tuple, int] = {}
 
 def _on_device(t: torch.Tensor, call) -> None:
     """``call(stream)`` with ``t``'s device current, on its current stream."""
-    if torch.cuda.current_device() == t.device.index:
-        check(call(_stream(t)))
+    index = t.device.index
+    # the raw handle: the wrapped stream object costs 2 us, as much as a launch's share of a decode step
+    if torch.cuda.current_device() == index:
+        check(call(torch._C._cuda_getCurrentRawStream(index)))
     else:
-        with torch.cuda.device(t.device):
-            check(call(_stream(t)))
+        with torch.cuda.device(index):
+            check(call(torch._C._cuda_getCurrentRawStream(index)))
 
 
 def paged_chunk_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, kv_pool: torch.Tensor, layer: int,
@@ -371,26 +373,26 @@ def paged_chunk_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Ten
     k_new, k_ld = _rows(k_new)
     v_new, v_ld = _rows(v_new)
     if out is None:
-        out = torch.empty((T, heads, 128), dtype=dt, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != dt or out.shape != (T, heads, 128) or not out.is_contiguous():
         raise ValueError(f"{op}: out must be a contiguous {dt} tensor of shape {(T, heads, 128)}")
     size = dt.itemsize
-    at = {"q": q.data_ptr(), "k_new": k_new.data_ptr(), "v_new": v_new.data_ptr(), "the pool": kv_pool.data_ptr()}
-    pool_at, out_at = at["the pool"], out.data_ptr()
+    q_at, k_at, v_at, pool_at, out_at = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), kv_pool.data_ptr(), out.data_ptr()
     pool_end, out_end = pool_at + kv_pool.numel() * size, out_at + T * heads * 128 * size
-    for name, ld, width in (("q", q_ld, heads), ("k_new", k_ld, kv_heads), ("v_new", v_ld, kv_heads)):
-        a, z = at[name], at[name] + ((T - 1) * ld + width * 128) * size
-        if T and a < out_end and out_at < z:
-            raise ValueError(f"{op}: out overlaps {name}")
-        if T and a < pool_end and pool_at < z:
-            raise ValueError(f"{op}: {name} overlaps the pool")
-    if T and pool_at < out_end and out_at < pool_end:
-        raise ValueError(f"{op}: out overlaps the pool")
+    if T:
+        for name, at, ld, width in (("q", q_at, q_ld, heads), ("k_new", k_at, k_ld, kv_heads), ("v_new", v_at, v_ld, kv_heads)):
+            end = at + ((T - 1) * ld + width * 128) * size
+            if at < out_end and out_at < end:
+                raise ValueError(f"{op}: out overlaps {name}")
+            if at < pool_end and pool_at < end:
+                raise ValueError(f"{op}: {name} overlaps the pool")
+        if pool_at < out_end and out_at < pool_end:
+            raise ValueError(f"{op}: out overlaps the pool")
     kind = 1 if dt == torch.bfloat16 else 0
-    scale, window, lib = float(scale), int(window), load()
+    lib = load()
 
     def call(stream):
-        key = (T, heads, kv_heads, kind, cols, B, kv_pool.device)
+        key = (T, heads, kv_heads, kind, cols, B, kv_pool.device.index)
         need = _CHUNK_WS.get(key)
         if need is None:
             if len(_CHUNK_WS) > 4096:
@@ -398,8 +400,8 @@ def paged_chunk_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Ten
             need = _CHUNK_WS[key] = lib.uocr_paged_chunk_workspace_bytes(T, heads, kv_heads, kind, cols, B)
         ws = torch.empty(need, dtype=torch.uint8, device=kv_pool.device)
         return lib.uocr_paged_chunk_attention(
-            at["q"], q_ld, at["k_new"], k_ld, at["v_new"], v_ld, T, heads, kv_heads, dim, kind, pool_at, pages, layers, layer,
-            lut.data_ptr(), cols, row_offsets.data_ptr(), start.data_ptr(), B, scale, window,
+            q_at, q_ld, k_at, k_ld, v_at, v_ld, T, heads, kv_heads, dim, kind, pool_at, pages, layers, layer, lut.data_ptr(),
+            cols, row_offsets.data_ptr(), start.data_ptr(), B, float(scale), int(window),
             None if prefix is None else prefix.data_ptr(), out_at, ws.data_ptr(), need, stream)
 
     _on_device(kv_pool, call)
