@@ -240,6 +240,47 @@ def test_many_requests(ops, oracle, dtype):
         Case(dtype, n, rng.integers(0, 200, B).tolist(), heads=1, kv_heads=1, layers=1, layer=0, seed=B).check(ops, oracle)
 
 
+def test_as_many_requests_as_a_call_takes(ops, oracle):
+    rng = np.random.default_rng(6)
+    n = rng.integers(0, 2, 8192).tolist()
+    Case(torch.bfloat16, n, rng.integers(0, 12, 8192).tolist(), heads=1, kv_heads=1, layers=1, layer=0, seed=9).check(ops, oracle)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [[2, 3], [140, 20]])
+def test_the_widest_window(ops, oracle, dtype, n):
+    Case(dtype, n, [300, 0], seed=27).check(ops, oracle, window=2 ** 31 - 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [2, 200])
+def test_pages_beyond_32_bits_of_offset(ops, dtype, n):
+    """The same cache in a small pool and, page by page, at the end of one of more than 2^32 elements."""
+    c = Case(dtype, [n], [300], heads=2, kv_heads=1, layers=1, layer=0, seed=28)
+    args = _flat(c)
+    want = ops.paged_chunk_attention(*args)
+    used, pages, layers, layer = c.lut.shape[1], 530, 256, 255
+    assert pages * 2 * layers * 128 * 128 > 2 ** 32
+    pool = torch.empty((pages, 2, layers, 128, 1, 128), dtype=dtype, device=DEV)
+    far = [pages - 2 - i for i in range(used)]
+    for i, p in enumerate(far):
+        pool[p, :, layer] = c.pool[c.lut[0, i], :, 0].to(DEV)
+        pool[p, :, layer - 1] = 7
+    lut = torch.tensor([far], dtype=torch.int32, device=DEV)
+    got = ops.paged_chunk_attention(*args[:3], pool, layer, lut, *args[6:])
+    assert torch.equal(got, want)
+    for i, p in enumerate(far):
+        assert torch.equal(pool[p, :, layer].view(torch.uint8), args[3][c.lut[0, i], :, 0].view(torch.uint8))
+        assert bool((pool[p, :, layer - 1] == 7).all())
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    pool[0].zero_(), pool[1].zero_()
+    ops.copy_pages(pool, i32([far[0]]), i32([0]))
+    assert torch.equal(pool[0].view(torch.uint8), pool[far[0]].view(torch.uint8))
+    ops.compact_rows(pool, i32([far[:1]]), i32([[1]]), i32([[3, 100]]), i32([2]))
+    assert torch.equal(pool[1, :, :, :2].view(torch.uint8), pool[far[0]][:, :, [3, 100]].view(torch.uint8))
+    assert bool((pool[1, :, :, 2:] == 0).all())
+
+
 def test_a_table_far_wider_than_its_requests(ops, oracle):
     """Most entries name the null page; the operands of all heads at once would pass a gigabyte, so that the heads
     are taken in several passes."""
