@@ -142,11 +142,20 @@ UOCR_API int uocr_paged_decode_attention(const float* q, const float* k_new, con
  * rows r <= p, all of them (window 0) or those with r > p - window or r < prefix[b] (window >= 1; prefix
  * null: 0). Rows below start[b] are read from the pool (page ids past the pool read its last page), the
  * new rows from k_new and v_new; new rows with a page id past the pool are attended but not stored, new
- * rows beyond the lookup table are in no request. Rows of out in no request are left as they were. What a row does not see
- * does not reach it, whatever it holds (NaN and infinities included).
- * Sums and softmax in fp32. The workspace (uocr_paged_chunk_workspace_bytes(...) bytes on the current
- * device, 0 for sizes that the call refuses; 256-byte aligned, no initial contents) belongs to the call until it has finished. The
- * result is deterministic (a fixed split and order on one kind of GPU). B <= 8192. */
+ * rows beyond the lookup table are in no request. Rows of out in no request are left as they were. What a row
+ * does not see does not reach it, whatever it holds (NaN and infinities included). A page row that the call
+ * stores is read or stored for no other request of the call.
+ * Sums and softmax in fp32. Two forms, by T x heads / kv_heads against B: up to 16 (fp32; bf16 8) rows of
+ * (token, query head) a request and KV head on average are computed on the fp32 units, more on the tensor cores: fp32
+ * there as three products of fp16 halves, q and keys to 2^-22 of themselves (or 2^-29 of their
+ * row's largest element), values to 2^-38 of the largest finite one of their page and head; bf16 weights rounded to bf16. A
+ * visible fp32 key with an element that is not finite makes the row NaN there. A wait inside the
+ * kernel that runs out (200 ms) ends it with NaN in the rows concerned.
+ * The workspace (uocr_paged_chunk_workspace_bytes(...) bytes on the current device, 0 for sizes that the call
+ * refuses; 256-byte aligned, no initial contents) belongs to the call until it has finished. On the tensor cores it holds
+ * 128 KB (bf16 64 KB) per page of the tables and KV head, up to 1 GiB or one head's share, so tables should be no wider
+ * than their requests are long. The result is deterministic (a fixed split and order on one kind of GPU).
+ * B <= 8192. */
 UOCR_API size_t uocr_paged_chunk_workspace_bytes(int64_t T, int64_t heads, int64_t kv_heads, int dtype,
                                int64_t lut_cols, int64_t B);
 UOCR_API int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, int64_t k_ld, const void* v_new,
@@ -165,8 +174,9 @@ UOCR_API int uocr_copy_pages(void* kv_pool, int64_t pages, int64_t layers, int64
 /* Rows of B requests compacted, in every layer, k and v: logical row i of request b in dst_lut
  * [B][dst_cols] takes its logical row keep[b * max_keep + i] in src_lut [B][src_cols], for
  * i < min(keep_len[b], max_keep). keep[b] ascends strictly, so that dst_lut may hold the same pages at
- * the same places as src_lut (in place); other pages of dst_lut occur in no request's src_lut. A row that
- * lies beyond its table, or whose page id is outside the pool, is skipped. No counterpart in the
+ * the same places as src_lut (in place); other pages of dst_lut occur in no request's src_lut, and a page in which
+ * rows change is in no other request's tables (requests that share a page: to fresh pages, or one by one). A row
+ * that lies beyond its table, or whose page id is outside the pool, is skipped. No counterpart in the
  * reference. */
 UOCR_API int uocr_compact_rows(void* kv_pool, int64_t pages, int64_t layers, int64_t row_bytes, const int32_t* src_lut,
                       int64_t src_cols, const int32_t* dst_lut, int64_t dst_cols, const int32_t* keep,

@@ -337,9 +337,12 @@ def paged_chunk_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Ten
     only those with ``r > p - window`` or ``r < prefix[b]`` (int32 ``[B]``; None: 0). ``out [T, heads, 128]``
     (contiguous, overlapping no input) is returned; its rows in no request keep what they held. All index
     tensors are on the device, and nothing synchronises; the workspace is the call's own, so calls may run
-    on several streams and be captured. The result is deterministic. ``T * heads / kv_heads`` against the
-    number of requests decides the form: up to 8 rows a request and KV head are computed straight from the
-    cache, more on the tensor cores (fp32 values then to 2^-38 of the largest finite one of their page).
+    on several streams and be captured. The result is deterministic. No page row that the call stores is in
+    another request's table. ``T * heads / kv_heads`` against the number of requests decides the form: up
+    to 16 (bf16: 8) rows a request and KV head are computed straight from the cache, more on the tensor
+    cores. There fp32 values are taken to 2^-38 of the largest finite one of their page, a visible fp32 key that
+    is not finite makes the row NaN, and the workspace grows with ``B * cols``: 128 KB (bf16: 64 KB) a page
+    and KV head, up to 1 GiB or one head's share.
     """
     op = "paged_chunk_attention"
     tensors = [q, k_new, v_new, kv_pool, lut, row_offsets, start]
@@ -430,8 +433,9 @@ def compact_rows(kv_pool: torch.Tensor, src_lut: torch.Tensor, dst_lut: torch.Te
     """Logical row ``i`` of request ``b`` in ``dst_lut [B, dst_cols]`` takes its logical row ``keep[b, i]`` in
     ``src_lut [B, src_cols]``, for ``i < keep_len[b]``, in every layer of ``kv_pool`` (fp32 or bf16), k and v.
     All are int32 on the device; ``keep[b]`` ascends strictly. ``dst_lut`` may hold the same pages at the
-    same places as ``src_lut`` (in place); its other pages occur in no request's ``src_lut``. Rows beyond
-    the tables, or with a page id outside the pool, are skipped."""
+    same places as ``src_lut`` (in place); its other pages occur in no request's ``src_lut``, and a page in
+    which rows change is in no other request's tables. Rows beyond the tables, or with a page id outside the
+    pool, are skipped."""
     op = "compact_rows"
     _need_cuda(op, kv_pool, src_lut, dst_lut, keep, keep_len)
     pages, layers, _, row_bytes = _pool_dims(op, kv_pool)
