@@ -800,7 +800,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
 }
 
 template <bool kF32>
-__global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(ChunkArgs a, Images im, ChunkParts parts) {
+__global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ Images im, const __grid_constant__ ChunkParts parts) {
     extern __shared__ unsigned char raw[];
     __shared__ Shared s;
     unsigned char* ring = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);

@@ -148,7 +148,7 @@ UOCR_DEV void store_new_keys(const ChunkArgs& a, const Place& p, int row0, int l
 }
 
 template <bool kF32, int NQ>
-__global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(ChunkArgs a, ChunkParts parts) {
+__global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ ChunkParts parts) {
     using W = Words<kF32>;
     extern __shared__ char raw[];
     Shared<NQ>& s = *reinterpret_cast<Shared<NQ>*>(raw);
