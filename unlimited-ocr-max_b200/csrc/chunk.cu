@@ -218,7 +218,7 @@ UOCR_DEV void query_operand(const ChunkArgs& a, const Images& im, int f, int hea
         x[i] = make_uint4(0, 0, 0, 0);
         if (row < rows)
             x[i] = ldg_nc_v4(static_cast<const char*>(a.q) +
-                             ((r.lo + R / g) * a.q_ld + (size_t)((a.head0 + head) * g + R % g) * kDim) * kElt +
+                             ((r.lo + token_of(a, R)) * a.q_ld + (size_t)((a.head0 + head) * g + R - token_of(a, R) * g) * kDim) * kElt +
                              (kF32 ? lane : lane & 15) * 16);
     }
 #pragma unroll
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = a.heads / a.kv_heads;
     const Request r = request_at(a, b);
     if (r.n == 0) return;
-    const Tile first = tile_at(a, r, 0, g, kTile);
+    const Tile first = tile_at(a, r, 0, kTile);
     const int last = r.start + r.n - 1, r0 = page * kPageRows;
     if (r0 > last || (page < first.tail_page && r0 >= r.prefix)) return;  // no token of the request sees it
     const uint32_t id = __ldg(a.lut + (size_t)b * a.lut_cols + page);
@@ -633,7 +633,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
         __syncwarp();
         const int R = now.qt * kTile + row, rows = now.r.n * g - now.qt * kTile;  // valid rows of the tile
         const bool live = (warp & 3) * 32 < rows;                                 // this warp has some
-        const int pos = now.r.start + R / g;
+        const int pos = now.r.start + token_of(a, R);
         m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[i] = 0;
@@ -754,7 +754,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
         const int slot = now.j == 0 ? 1 : 0;
         float* part = parts.slots + ((size_t)blockIdx.x * 2 + slot) * slot_floats(kTile);
         if (whole && row < rows) {
-            const size_t at = ((size_t)(now.r.lo + R / g) * a.heads + (a.head0 + now.head) * g + R % g) * kDim + half * 64;
+            const size_t at = ((size_t)(now.r.lo + pos - now.r.start) * a.heads + (a.head0 + now.head) * g + R - (pos - now.r.start) * g) * kDim + half * 64;
             auto two = [&](int i) {
                 uint32_t y0, y1;
                 unpair(mul2(acc[i], f2), y0, y1);
@@ -889,7 +889,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(ChunkArgs a, ChunkParts
     }
     const float inv = 1.f / l;
     const int R = r0 + row;
-    const size_t at = ((size_t)(lo + R / g) * a.heads + head * g + R % g) * kDim + c0;
+    const size_t at = ((size_t)(lo + token_of(a, R)) * a.heads + head * g + R - token_of(a, R) * g) * kDim + c0;
     if constexpr (kF32) {
         float4* out = reinterpret_cast<float4*>(static_cast<float*>(a.out) + at);
         out[0] = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
@@ -977,6 +977,10 @@ size_t chunk_workspace_bytes(const ChunkArgs& a, int sms) {
 
 cudaError_t launch_chunk_attention(const ChunkArgs& args, void* ws, int sms, cudaStream_t st) {
     ChunkArgs a = args;
+    const int g = a.heads / a.kv_heads;
+    a.group_shift = 32;
+    while (g >> (a.group_shift - 31)) ++a.group_shift;
+    a.group_mul = ((1ull << a.group_shift) + g - 1) / g;
     if (a.B <= 0 || a.T <= 0) return cudaSuccess;
     char* w = static_cast<char*>(ws);
     ChunkParts parts{reinterpret_cast<float*>(w + ((size_t)sms * kInfoInts * 4 + 255) / 256 * 256), reinterpret_cast<int*>(w), sms,

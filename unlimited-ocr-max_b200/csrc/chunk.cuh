@@ -42,6 +42,11 @@ UOCR_DEV Request request_at(const ChunkArgs& a, int b) {
     return r;
 }
 
+// n / g for 0 <= n < 2^31 and g = heads / kv_heads: group_mul = 2^s / g rounded up, off by less than 1, so that the quotient is
+// off by less than n / 2^s < 1 / g with s = group_shift > 31 + log2(g). (A division by a variable is 20 instructions, and
+// the walks' code is fetched anew for every tile.)
+UOCR_DEV int token_of(const ChunkArgs& a, int n) { return (int)((unsigned long long)(uint32_t)n * a.group_mul >> a.group_shift); }
+
 // A query tile is `tile` (token, query head of the KV head) rows of a request. Its pages: columns [0, head_pages) and [tail_page, ...) of its lookup row, `count` in all.
 struct Tile {
     int first_pos, last_pos;  // logical rows of its first and last token
@@ -49,11 +54,11 @@ struct Tile {
     UOCR_DEV int page(int j) const { return j < head_pages ? j : j - head_pages + tail_page; }
 };
 
-UOCR_DEV Tile tile_at(const ChunkArgs& a, const Request& r, int qt, int g, int tile) {
+UOCR_DEV Tile tile_at(const ChunkArgs& a, const Request& r, int qt, int tile) {
     Tile t;
     const int r0 = qt * tile;
-    t.first_pos = r.start + r0 / g;
-    t.last_pos = r.start + min(r.n - 1, (r0 + tile - 1) / g);
+    t.first_pos = r.start + token_of(a, r0);
+    t.last_pos = r.start + min(r.n - 1, token_of(a, r0 + tile - 1));
     t.head_pages = t.tail_page = 0;
     if (a.window > 0) {
         t.tail_page = max(0, t.first_pos - a.window + 1) / kPageRows;
@@ -78,8 +83,8 @@ struct Walk {
     Request r;
     Tile t;
     // at x of the segment's tile and head; false: the run ends in front of its pages
-    UOCR_DEV bool enter(const ChunkArgs& a, int g, int tile, int lead, int x) {
-        t = tile_at(a, r, qt, g, tile);
+    UOCR_DEV bool enter(const ChunkArgs& a, int tile, int lead, int x) {
+        t = tile_at(a, r, qt, tile);
         const int end = min(x + left, t.count + lead);
         j = max(x - lead, 0);
         n = max(end - lead, 0) - j;
@@ -92,7 +97,7 @@ struct Walk {
         b = s.b, qt = s.qt, head = s.head;
         r = request_at(a, b);
         tiles = (r.n * g + tile - 1) / tile;
-        return enter(a, g, tile, lead, s.x);
+        return enter(a, tile, lead, s.x);
     }
     UOCR_DEV bool next(const ChunkArgs& a, int g, int tile, int lead) {
         if (left <= 0) return false;
@@ -107,7 +112,7 @@ struct Walk {
                 tiles = (r.n * g + tile - 1) / tile;
             }
         }
-        return enter(a, g, tile, lead, 0);
+        return enter(a, tile, lead, 0);
     }
     UOCR_DEV bool whole() const { return j == 0 && n == t.count; }
 };
@@ -123,13 +128,15 @@ UOCR_DEV T warp_scan(T v, int lane) {  // inclusive
 }
 
 // All threads: this CTA's run of units. scratch: B long longs of shared memory.
-__device__ __noinline__ void find_run(const ChunkArgs& a, Run& run, long long* scratch, int g, int tile, int lead) {
+UOCR_DEV void find_run(const ChunkArgs& a, Run& run, long long* scratch, int g, int tile, int lead) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll 1  // run once: short code is fetched sooner
     for (int b = warp; b < a.B; b += blockDim.x / 32) {
         const Request r = request_at(a, b);
         const int tiles = (r.n * g + tile - 1) / tile;
         long long sum = 0;
-        for (int qt = lane; qt < tiles; qt += 32) sum += tile_at(a, r, qt, g, tile).count + lead;
+#pragma unroll 1
+        for (int qt = lane; qt < tiles; qt += 32) sum += tile_at(a, r, qt, tile).count + lead;
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) scratch[b] = sum * a.pass_heads;
@@ -137,16 +144,22 @@ __device__ __noinline__ void find_run(const ChunkArgs& a, Run& run, long long* s
     __syncthreads();
     if (warp == 0) {
         long long total = 0;
+#pragma unroll 1
         for (int b = lane; b < a.B; b += 32) total += scratch[b];
 #pragma unroll
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
         const long long ctas = min((long long)gridDim.x, total);
         long long u0 = 0, u1 = 0;
-        if ((long long)blockIdx.x < ctas) u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
+        if ((long long)blockIdx.x < ctas) {  // runs of two lengths, the longer ones first
+            const long long each = total / ctas, rest = total - each * ctas;
+            u0 = each * blockIdx.x + min((long long)blockIdx.x, rest);
+            u1 = u0 + each + (blockIdx.x < rest ? 1 : 0);
+        }
         if (lane == 0) run.left = (int)(u1 - u0);
         if (u1 > u0) {
             int b = 0;
             long long before = 0;  // units in front of request b
+#pragma unroll 1
             for (int b0 = 0; b0 < a.B; b0 += 32) {
                 const long long mine = b0 + lane < a.B ? scratch[b0 + lane] : 0;
                 const long long upto = before + warp_scan(mine, lane);
@@ -161,14 +174,15 @@ __device__ __noinline__ void find_run(const ChunkArgs& a, Run& run, long long* s
             }
             const Request r = request_at(a, b);
             const int tiles = (r.n * g + tile - 1) / tile;
+#pragma unroll 1
             for (int q0 = 0; q0 < tiles; q0 += 32) {
-                const int count = q0 + lane < tiles ? tile_at(a, r, q0 + lane, g, tile).count + lead : 0;
+                const int count = q0 + lane < tiles ? tile_at(a, r, q0 + lane, tile).count + lead : 0;
                 const long long upto = before + warp_scan((long long)count * a.pass_heads, lane);
                 const uint32_t hit = __ballot_sync(0xffffffffu, upto > u0);
                 if (hit) {
                     if (lane == __ffs(hit) - 1) {
                         const long long in = u0 - (upto - (long long)count * a.pass_heads);
-                        run.b = b, run.qt = q0 + lane, run.head = (int)(in / count), run.x = (int)(in % count);
+                        run.b = b, run.qt = q0 + lane, run.head = (int)(in / count), run.x = (int)(in - (long long)run.head * count);
                     }
                     break;
                 }

@@ -76,8 +76,8 @@ UOCR_DEV Place place_of(const ChunkArgs& a, const Walk& w, int j, uint32_t id, i
     p.k_new = static_cast<const char*>(a.k) + (w.r.lo - p.cached) * (a.k_ld * kElt) + column;
     p.v_new = static_cast<const char*>(a.v) + (w.r.lo - p.cached) * (a.v_ld * kElt) + column;
     // new rows whose first query head lies in this tile
-    p.own0 = p.cached + (w.qt * tile + g - 1) / g;
-    p.own1 = id < (uint32_t)a.pages ? p.cached + min(w.r.n, (w.qt * tile + tile + g - 1) / g) : p.own0;
+    p.own0 = p.cached + token_of(a, w.qt * tile + g - 1);
+    p.own1 = id < (uint32_t)a.pages ? p.cached + min(w.r.n, token_of(a, w.qt * tile + tile + g - 1)) : p.own0;
     return p;
 }
 
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(const __grid_co
             const int R = w.qt * NQ + e / (kDim / 4);
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (R < w.r.n * g) {
-                const size_t at = (w.r.lo + R / g) * a.q_ld + (size_t)(w.head * g + R % g) * kDim + (e % (kDim / 4)) * 4;
+                const size_t at = (w.r.lo + token_of(a, R)) * a.q_ld + (size_t)(w.head * g + R - token_of(a, R) * g) * kDim + (e % (kDim / 4)) * 4;
                 if constexpr (kF32) {
                     v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at);
                 } else {
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(const __grid_co
             for (int j = 0; j < NQ; ++j) {
                 bool seen = true;
                 if (!all) {
-                    const int pos = start + (qt * NQ + j) / g, r = c0 + row0 + mine;
+                    const int pos = start + token_of(a, qt * NQ + j), r = c0 + row0 + mine;
                     seen = r <= pos && (a.window <= 0 || r > pos - a.window || r < prefix);
                     if (!seen) sc[j] = -INFINITY;
                 }
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(const __grid_co
             if (whole) {
                 const float inv = 1.f / L;
                 const int R = qt * NQ + j;
-                const size_t at = ((size_t)(lo + R / g) * a.heads + head * g + R % g) * kDim + d;
+                const size_t at = ((size_t)(lo + token_of(a, R)) * a.heads + head * g + R - token_of(a, R) * g) * kDim + d;
                 if constexpr (kF32) *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(o.x * inv, o.y * inv);
                 else *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at) = pack_bf16(o.x * inv, o.y * inv);
             } else {

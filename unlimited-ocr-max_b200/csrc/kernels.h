@@ -58,7 +58,9 @@ struct ChunkArgs {
     const int32_t* prefix;              // [B] or null
     int T, B, heads, kv_heads, pages, layers, layer, lut_cols, window, bf16;
     float scale;
-    int head0, pass_heads;              // the KV heads of one pass over the call (set by the launcher)
+    // Set by the launcher: the KV heads of one pass over the call; n / (heads / kv_heads) as n * group_mul >> group_shift
+    int head0, pass_heads, group_shift;
+    unsigned long long group_mul;
 };
 constexpr int kChunkMaxRequests = 8192;
 size_t chunk_workspace_bytes(const ChunkArgs& a, int sms);
