@@ -155,7 +155,7 @@ UOCR_API int uocr_paged_decode_attention(const float* q, const float* k_new, con
  * refuses; 256-byte aligned, no initial contents) belongs to the call until it has finished. On the tensor cores it holds
  * 128 KB (bf16 64 KB) per page of the tables and KV head, up to 1 GiB or one head's share, so tables should be no wider
  * than their requests are long. The result is deterministic (a fixed split and order on one kind of GPU).
- * B <= 8192. */
+ * B <= 8192, and (T x heads / kv_heads / 128 + B) x kv_heads x (lut_cols + 4) <= 2^30. */
 UOCR_API size_t uocr_paged_chunk_workspace_bytes(int64_t T, int64_t heads, int64_t kv_heads, int dtype,
                                int64_t lut_cols, int64_t B);
 UOCR_API int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, int64_t k_ld, const void* v_new,

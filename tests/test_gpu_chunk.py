@@ -422,6 +422,21 @@ def test_pages_and_lengths_outside_the_pool_stay_inside_it(ops, oracle):
     assert torch.equal(got[4:7], fresh[4:7]) and got.shape == want.shape
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_offsets_that_do_not_ascend_stay_inside(ops, dtype):
+    """Requests that lie over one another: some result, nothing outside out and the requests' pages, and a call
+    after it is right."""
+    c = Case(dtype, [300, 2, 40], [10, 300, 0], seed=62)
+    args = _flat(c)
+    want = ops.paged_chunk_attention(*args)
+    for off in ([0, 342, 0, 342], [342, 0, 300, 5], [-7, 10 ** 9, 3, 2 ** 31 - 1]):
+        bad = _flat(c)
+        bad[6] = torch.tensor(off, dtype=torch.int32, device=DEV)
+        ops.paged_chunk_attention(*bad)
+        torch.cuda.synchronize()
+    assert torch.equal(ops.paged_chunk_attention(*_flat(c)), want)
+
+
 def test_chunks_of_any_size_make_the_same_cache(ops):
     """A prompt fed in pieces: the pool is the same bit for bit, the outputs within the bound of the
     split's other order of summation (twice the derived one, S about 10 here: 2^-12)."""

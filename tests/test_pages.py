@@ -36,7 +36,7 @@ def _chunk(lib, **v):
     ({"T": 0}, 0, ""), ({"B": 0}, 0, ""),
     ({"B": 8193}, 4, "8193 requests"), ({"B": 8192, "cols": 1 << 18}, 4, "tables of 8192"),
     ({"B": 64, "cols": 1 << 22, "heads": 1024, "kv": 1024, "q_ld": 1 << 17, "k_ld": 1 << 17, "v_ld": 1 << 17}, 4, "too much"),
-    ({"B": 64, "cols": 1 << 19, "heads": 1024, "kv": 1024, "q_ld": 1 << 17, "k_ld": 1 << 17, "v_ld": 1 << 17}, 1, "null pointer"),
+    ({"B": 64, "cols": 1 << 13, "heads": 1024, "kv": 1024, "q_ld": 1 << 17, "k_ld": 1 << 17, "v_ld": 1 << 17}, 1, "null pointer"),
     ({"T": 1 << 28, "cols": 1 << 22}, 4, "too much"), ({"window": 1 << 31}, 1, "window"), ({"cols": (1 << 22) + 1}, 1, "bad pool"),
 ])
 def test_chunk_attention_refusals(uocr, change, code, word):

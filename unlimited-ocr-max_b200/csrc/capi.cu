@@ -347,9 +347,9 @@ int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, i
     if (B * lut_cols > (int64_t(1) << 30))
         return fail(UOCR_EUNSUPPORTED, "paged_chunk_attention: tables of %lld x %lld pages (this build: <= 2^30)", (long long)B,
                     (long long)lut_cols);
-    // A CTA counts its (query tile, head, page) units in 31 bits, and 148 share them. The form for few rows has at most three
-    // tiles a request: a factor of four is kept free.
-    if ((T * (heads / kv_heads) / 128 + B) * kv_heads > (int64_t(1) << 36) / (lut_cols + T / 128 + 4))
+    // The (query tile, head, page) units of a call, with what a tile counts beside its pages, are counted in 32 bits. The form
+    // for few rows has at most three tiles a request: a factor of four is kept free.
+    if ((T * (heads / kv_heads) / 128 + B) * kv_heads > (int64_t(1) << 30) / (lut_cols + 4))
         return fail(UOCR_EUNSUPPORTED, "paged_chunk_attention: T %lld over %lld pages a request is too much for one call",
                     (long long)T, (long long)lut_cols);
     if (window < 0 || window > INT32_MAX)

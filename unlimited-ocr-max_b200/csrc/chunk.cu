@@ -815,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_attention_kernel(const __gr
     }
     if (warp == kTeamWarps) tmem_alloc(&s.tmem, 512);
     tc_fence_before();
-    find_run(a, s.run, reinterpret_cast<long long*>(ring), g, kTile, kLead);
+    find_run(a, s.run, reinterpret_cast<uint32_t*>(ring), g, kTile, kLead);
     tc_fence_after();
     pdl_launch_dependents();
     if (warp < kTeamWarps) {

@@ -105,10 +105,13 @@ struct Walk {
             head = 0;
             if (++qt >= tiles) {
                 qt = 0;
-                do {  // left > 0: another request with rows follows
-                    ++b;
+                do {  // left > 0: another request with rows follows (unless offsets that do not ascend overflowed the count)
+                    if (++b >= a.B) {
+                        left = 0;
+                        return false;
+                    }
                     r = request_at(a, b);
-                } while (r.n == 0 && b < a.B - 1);
+                } while (r.n == 0);
                 tiles = (r.n * g + tile - 1) / tile;
             }
         }
@@ -127,14 +130,16 @@ UOCR_DEV T warp_scan(T v, int lane) {  // inclusive
     return v;
 }
 
-// All threads: this CTA's run of units. scratch: B long longs of shared memory.
-UOCR_DEV void find_run(const ChunkArgs& a, Run& run, long long* scratch, int g, int tile, int lead) {
+// All threads: this CTA's run of units. scratch: B words of shared memory. A call has less than 2^32 units, counted with the
+// tiles' leads: the entry point sees to it. (Offsets that do not ascend may reach that many: the run then is some run,
+// within the call's requests, tiles and heads.)
+UOCR_DEV void find_run(const ChunkArgs& a, Run& run, uint32_t* scratch, int g, int tile, int lead) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll 1  // run once: short code is fetched sooner
     for (int b = warp; b < a.B; b += blockDim.x / 32) {
         const Request r = request_at(a, b);
         const int tiles = (r.n * g + tile - 1) / tile;
-        long long sum = 0;
+        uint32_t sum = 0;
 #pragma unroll 1
         for (int qt = lane; qt < tiles; qt += 32) sum += tile_at(a, r, qt, tile).count + lead;
 #pragma unroll
@@ -143,26 +148,27 @@ UOCR_DEV void find_run(const ChunkArgs& a, Run& run, long long* scratch, int g, 
     }
     __syncthreads();
     if (warp == 0) {
-        long long total = 0;
+        uint32_t total = 0;
 #pragma unroll 1
         for (int b = lane; b < a.B; b += 32) total += scratch[b];
 #pragma unroll
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        const long long ctas = min((long long)gridDim.x, total);
-        long long u0 = 0, u1 = 0;
-        if ((long long)blockIdx.x < ctas) {  // runs of two lengths, the longer ones first
-            const long long each = total / ctas, rest = total - each * ctas;
-            u0 = each * blockIdx.x + min((long long)blockIdx.x, rest);
+        const uint32_t ctas = min(gridDim.x, total);
+        uint32_t u0 = 0, u1 = 0;
+        if (blockIdx.x < ctas) {  // runs of two lengths, the longer ones first
+            const uint32_t each = total / ctas, rest = total - each * ctas;
+            u0 = each * blockIdx.x + min(blockIdx.x, rest);
             u1 = u0 + each + (blockIdx.x < rest ? 1 : 0);
         }
-        if (lane == 0) run.left = (int)(u1 - u0);
+        if (lane == 0) run.left = 0;
+        __syncwarp();
         if (u1 > u0) {
             int b = 0;
-            long long before = 0;  // units in front of request b
+            uint32_t before = 0;  // units in front of request b
 #pragma unroll 1
             for (int b0 = 0; b0 < a.B; b0 += 32) {
-                const long long mine = b0 + lane < a.B ? scratch[b0 + lane] : 0;
-                const long long upto = before + warp_scan(mine, lane);
+                const uint32_t mine = b0 + lane < a.B ? scratch[b0 + lane] : 0;
+                const uint32_t upto = before + warp_scan(mine, lane);
                 const uint32_t hit = __ballot_sync(0xffffffffu, upto > u0);
                 if (hit) {
                     const int f = __ffs(hit) - 1;
@@ -176,13 +182,13 @@ UOCR_DEV void find_run(const ChunkArgs& a, Run& run, long long* scratch, int g, 
             const int tiles = (r.n * g + tile - 1) / tile;
 #pragma unroll 1
             for (int q0 = 0; q0 < tiles; q0 += 32) {
-                const int count = q0 + lane < tiles ? tile_at(a, r, q0 + lane, tile).count + lead : 0;
-                const long long upto = before + warp_scan((long long)count * a.pass_heads, lane);
+                const uint32_t count = q0 + lane < tiles ? tile_at(a, r, q0 + lane, tile).count + lead : 0;
+                const uint32_t upto = before + warp_scan(count * a.pass_heads, lane);
                 const uint32_t hit = __ballot_sync(0xffffffffu, upto > u0);
                 if (hit) {
                     if (lane == __ffs(hit) - 1) {
-                        const long long in = u0 - (upto - (long long)count * a.pass_heads);
-                        run.b = b, run.qt = q0 + lane, run.head = (int)(in / count), run.x = (int)(in - (long long)run.head * count);
+                        const uint32_t in = u0 - (upto - count * a.pass_heads);
+                        run.left = (int)(u1 - u0), run.b = b, run.qt = q0 + lane, run.head = (int)min(in / count, a.pass_heads - 1u), run.x = (int)(in % count);
                     }
                     break;
                 }

@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(const __grid_co
     Shared<NQ>& s = *reinterpret_cast<Shared<NQ>*>(raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     const int g = a.heads / a.kv_heads, row0 = warp * 16;
-    find_run(a, s.run, reinterpret_cast<long long*>(raw + sizeof(Shared<NQ>)), g, NQ, kLead);
+    find_run(a, s.run, reinterpret_cast<uint32_t*>(raw + sizeof(Shared<NQ>)), g, NQ, kLead);
     pdl_launch_dependents();
     Walk& w = s.walk[warp];
     bool more = w.begin(a, s.run, g, NQ, kLead);
@@ -365,9 +365,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(const __grid_co
 
 template <bool kF32, int NQ>
 cudaError_t launch(const ChunkArgs& a, const ChunkParts& parts, cudaStream_t st) {
-    const size_t smem = sizeof(Shared<NQ>) + (size_t)a.B * sizeof(long long);
+    const size_t smem = sizeof(Shared<NQ>) + (size_t)a.B * sizeof(uint32_t);
     auto kernel = chunk_rows_kernel<kF32, NQ>;
-    cudaError_t err = ensure_smem_optin(reinterpret_cast<const void*>(kernel), sizeof(Shared<NQ>) + kChunkMaxRequests * sizeof(long long));
+    cudaError_t err = ensure_smem_optin(reinterpret_cast<const void*>(kernel), sizeof(Shared<NQ>) + kChunkMaxRequests * sizeof(uint32_t));
     if (err != cudaSuccess) return err;
     kernel<<<parts.ctas, kThreads, smem, st>>>(a, parts);
     err = cudaGetLastError();
