@@ -403,7 +403,8 @@ __device__ void copy_role(const ChunkArgs& a, Shared& s, unsigned char* ring, co
         return true;
     };
     auto run = [&] {
-        for (bool more = w.begin(a, s.run, g, kTile, kLead); more; more = w.next(a, g, kTile, kLead)) {
+        w = s.run.first;
+        for (bool more = s.run.some; more; more = w.next(a, g, kTile, kLead)) {
             const int n = w.n;
             for (int jj = 0; jj <= n; ++jj) {
                 if (jj < n && !copy(false, jj)) return false;
@@ -471,7 +472,8 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
     auto run = [&] {
         auto next = [&](bool first) {
             __syncwarp();
-            const bool more = first ? w.begin(a, s.run, g, kTile, kLead) : w.next(a, g, kTile, kLead);
+            if (first) w = s.run.first;
+            const bool more = first ? s.run.some : w.next(a, g, kTile, kLead);
             __syncwarp();
             return __any_sync(0xffffffffu, more);
         };
@@ -623,7 +625,8 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
 
     Walk& w = s.walk[warp];
     Walk& now = s.now[warp];  // the segment at work
-    bool more = w.begin(a, s.run, g, kTile, kLead);
+    w = s.run.first;
+    bool more = s.run.some;
     __syncwarp();
     int state[2] = {0, 0}, place[4] = {0, 0, 0, 0};
     uint32_t unit0 = 0;

@@ -68,13 +68,9 @@ UOCR_DEV Tile tile_at(const ChunkArgs& a, const Request& r, int qt, int tile) {
     return t;
 }
 
-// A CTA's run of the call's work: its length, and where it begins (heads are counted from the pass's first). Work is
-// counted in pages; a tile and head counts `lead` more in front of its pages, for what a CTA does once for it
-// (its queries, its results), so that a run of many short tiles takes no longer than one of a few long ones.
-struct Run {
-    int left, b, qt, head, x;
-};
-
+// A CTA's run of the call's work. Work is counted in pages; a tile and head counts `lead` more in front of its pages, for what
+// a CTA does once for it (its queries, its results), so that a run of many short tiles takes no longer than one of a few long
+// ones.
 // The walk over a CTA's units, a segment (pages of one tile and head) at a time; every warp walks by
 // itself.
 struct Walk {
@@ -90,14 +86,6 @@ struct Walk {
         n = max(end - lead, 0) - j;
         left -= end - x;
         return n > 0;
-    }
-    UOCR_DEV bool begin(const ChunkArgs& a, const Run& s, int g, int tile, int lead) {
-        left = s.left;
-        if (left <= 0) return false;
-        b = s.b, qt = s.qt, head = s.head;
-        r = request_at(a, b);
-        tiles = (r.n * g + tile - 1) / tile;
-        return enter(a, tile, lead, s.x);
     }
     UOCR_DEV bool next(const ChunkArgs& a, int g, int tile, int lead) {
         if (left <= 0) return false;
@@ -118,6 +106,12 @@ struct Walk {
         return enter(a, tile, lead, 0);
     }
     UOCR_DEV bool whole() const { return j == 0 && n == t.count; }
+};
+
+// A CTA's run: its first segment, if it has one (heads are counted from the pass's first).
+struct Run {
+    Walk first;
+    int some;
 };
 
 template <typename T>
@@ -160,7 +154,7 @@ UOCR_DEV void find_run(const ChunkArgs& a, Run& run, uint32_t* scratch, int g, i
             u0 = each * blockIdx.x + min(blockIdx.x, rest);
             u1 = u0 + each + (blockIdx.x < rest ? 1 : 0);
         }
-        if (lane == 0) run.left = 0;
+        if (lane == 0) run.some = 0;
         __syncwarp();
         if (u1 > u0) {
             int b = 0;
@@ -188,7 +182,11 @@ UOCR_DEV void find_run(const ChunkArgs& a, Run& run, uint32_t* scratch, int g, i
                 if (hit) {
                     if (lane == __ffs(hit) - 1) {
                         const uint32_t in = u0 - (upto - count * a.pass_heads);
-                        run.left = (int)(u1 - u0), run.b = b, run.qt = q0 + lane, run.head = (int)min(in / count, a.pass_heads - 1u), run.x = (int)(in % count);
+                        Walk w;
+                        w.left = (int)(u1 - u0), w.b = b, w.qt = q0 + lane, w.head = (int)min(in / count, a.pass_heads - 1u);
+                        w.r = r, w.tiles = tiles;
+                        run.some = w.enter(a, tile, lead, (int)(in % count));
+                        run.first = w;
                     }
                     break;
                 }

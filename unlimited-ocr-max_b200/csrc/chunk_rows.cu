@@ -157,7 +157,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(const __grid_co
     find_run(a, s.run, reinterpret_cast<uint32_t*>(raw + sizeof(Shared<NQ>)), g, NQ, kLead);
     pdl_launch_dependents();
     Walk& w = s.walk[warp];
-    bool more = w.begin(a, s.run, g, NQ, kLead);
+    w = s.run.first;
+    bool more = s.run.some;
     __syncwarp();
     int state[2] = {0, 0}, where[4] = {0, 0, 0, 0};
     const float factor = a.scale * kLog2e;
