@@ -959,9 +959,9 @@ cudaError_t launch_chunk_join(const ChunkArgs& a, const ChunkParts& p, cudaStrea
 }
 
 // Rows of a query tile: 1 to 8 where a request has few (token, head) rows of a KV head on average (chunk_rows.cu: bound
-// by the cache's bytes), else 128 (tensor cores). Measured at 8 requests of 8000 rows, 10 heads: fp32, 16 rows 316 us
-// against 359, 24 rows 464 against 359; bf16 (16 heads), 8 rows 244 us against 292, 9 rows 469 against 292. The tile's
-// rows cost time too (fp32, 2 to 8 rows: 109 to 166 us): a whole average is taken for every request's
+// by the cache's bytes), else 128 (tensor cores). Measured at 8 requests of 8000 rows, 10 heads: fp32, 16 rows 274 us
+// against 353, 24 rows 411 against 353; bf16 (16 heads), 8 rows 217 us against 287, 9 rows 430 against 287. The tile's
+// rows cost time too (fp32, 2 to 8 rows: 107 to 145 us): a whole average is taken for every request's
 // number of rows, with another one they differ and twice the average less one is provided for, since a second tile
 // reads the cache again.
 static int tile_rows(const ChunkArgs& a) {

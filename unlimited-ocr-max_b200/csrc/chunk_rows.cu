@@ -13,10 +13,10 @@
 // The weights of a row are held by two lanes and read back by all: (p, p) as one 8-byte word feeds a packed fp32 product
 // without a move. bf16 rows are widened where they are used, exactly; nothing is rounded before the result.
 //
-// Measured (B200, fp32, 10 heads): 8 requests over 8000 rows, 656 MB: 1 row each 108 us (6.1 TB/s), 4 rows 113, 8 rows
-// 166 (the fp32 units bound it: every element takes part in 8 products). 1 to 5 drafted tokens over contexts of 997 to
-// 8000 rows, 368 MB: 78 us, 4.7 TB/s (the request of 5 has two tiles of 3 and is read twice). Short calls are bound by
-// latency: one request of 640 rows 12.4 us with the joining launch, 8 requests of 77 to 639 rows (29 MB) 16.5. A unit's
+// Measured (B200, fp32, 10 heads): 8 requests over 8000 rows, 656 MB: 1 row each 105 us (6.2 TB/s), 4 rows 110, 8 rows
+// 145 (the fp32 units bound it: every element takes part in 8 products). 1 to 5 drafted tokens over contexts of 997 to
+// 8000 rows, 368 MB: 74 us, 5.0 TB/s (the request of 5 has two tiles of 3 and is read twice). Short calls are bound by
+// latency: one request of 640 rows 11.4 us with the joining launch, 8 requests of 77 to 639 rows (29 MB) 14.7. A unit's
 // chain is table, keys, scores, values; smaller units would shorten it for one short request only, and cost the long
 // ones their streams.
 #include <type_traits>
