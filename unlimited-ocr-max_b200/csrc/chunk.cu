@@ -49,7 +49,7 @@ namespace uocr {
 namespace {
 
 constexpr int kTile = 128;      // (token, head) rows of a query tile
-constexpr int kLead = 3;        // what a tile costs beside its pages
+constexpr int kLead = 3;        // what a tile costs beside its pages (2 to 4 measure alike)
 constexpr int kTeamWarps = 8;   // softmax; then a warpgroup: the issuing warp, the copying warp and two idle ones
 constexpr int kThreads = 32 * (kTeamWarps + 4);
 constexpr int kLaunchRegs = 168, kTeamRegs = 216, kOtherRegs = 72;  // a thread
@@ -960,8 +960,8 @@ cudaError_t launch_chunk_join(const ChunkArgs& a, const ChunkParts& p, cudaStrea
 
 // Rows of a query tile: 1 to 8 where a request has few (token, head) rows of a KV head on average (chunk_rows.cu: bound
 // by the cache's bytes), else 128 (tensor cores). Measured at 8 requests of 8000 rows, 10 heads: fp32, 16 rows 274 us
-// against 353, 24 rows 411 against 353; bf16 (16 heads), 8 rows 217 us against 287, 9 rows 430 against 287. The tile's
-// rows cost time too (fp32, 2 to 8 rows: 107 to 145 us): a whole average is taken for every request's
+// against 353; bf16 (16 heads), 8 rows 217 us against 287; beyond the rule, a little earlier: fp32, 24 rows 464 us against 359;
+// bf16, 9 rows 469 against 292. The tile's rows cost time too (fp32, 2 to 8 rows: 107 to 145 us): a whole average is taken for every request's
 // number of rows, with another one they differ and twice the average less one is provided for, since a second tile
 // reads the cache again.
 static int tile_rows(const ChunkArgs& a) {
