@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
     const int row0 = warp * 16 + (kF32 ? 0 : lane >> 4), byte = (kF32 ? lane : lane & 15) * 16;
     const int cached = r.start - r0, known = min(kPageRows, last + 1 - r0);
     PageMeta& meta = im.meta[index];
-    for (int v = 0; v < 2; ++v) {
+    for (int v = 0; v < 2; ++v) {  // rows pass L2 by (read and stored once), where the operands should stay: 8 x 512 fp32 79.4 -> 78.3 us
         char* pool = static_cast<char*>(a.pool) +
                      ((((size_t)min(id, (uint32_t)(a.pages - 1)) * 2 + v) * a.layers + a.layer) * kPageRows) * row_bytes +
                      (size_t)head * (kDim * kElt) + byte;
@@ -282,13 +282,13 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
         for (int i = 0; i < kWords; ++i) {
             const int row = row0 + i * kPer;
             x[i] = make_uint4(0, 0, 0, 0);
-            if (row < known) x[i] = ldg_nc_v4(row < cached ? pool + row * row_bytes : fresh + row * ld);
+            if (row < known) x[i] = __ldcs(reinterpret_cast<const uint4*>(row < cached ? pool + row * row_bytes : fresh + row * ld));
         }
         if (known > cached && id < (uint32_t)a.pages) {
 #pragma unroll
             for (int i = 0; i < kWords; ++i) {
                 const int row = row0 + i * kPer;
-                if (row >= cached && row < known) *reinterpret_cast<uint4*>(pool + row * row_bytes) = x[i];
+                if (row >= cached && row < known) __stcs(reinterpret_cast<uint4*>(pool + row * row_bytes), x[i]);
             }
         }
         float up = 1.f;
