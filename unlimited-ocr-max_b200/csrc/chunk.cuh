@@ -129,24 +129,31 @@ UOCR_DEV T warp_scan(T v, int lane) {  // inclusive
 // within the call's requests, tiles and heads.)
 UOCR_DEV void find_run(const ChunkArgs& a, Run& run, uint32_t* scratch, int g, int tile, int lead) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll 1  // run once: short code is fetched sooner
-    for (int b = warp; b < a.B; b += blockDim.x / 32) {
-        const Request r = request_at(a, b);
-        const int tiles = (r.n * g + tile - 1) / tile;
-        uint32_t sum = 0;
+    // A warp's requests, one in each lane, then one after the other with the lanes on its tiles. (The loops stay rolled: run
+    // once, short code is fetched sooner.)
+    const int warps = blockDim.x / 32;
 #pragma unroll 1
-        for (int qt = lane; qt < tiles; qt += 32) sum += tile_at(a, r, qt, tile).count + lead;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) scratch[b] = sum * a.pass_heads;
+    for (int b0 = warp; b0 < a.B; b0 += 32 * warps) {
+        const Request mine = request_at(a, min(b0 + lane * warps, a.B - 1));
+#pragma unroll 1
+        for (int i = 0, b = b0; i < 32 && b < a.B; ++i, b += warps) {
+            Request r;
+            r.lo = 0, r.n = __shfl_sync(0xffffffffu, mine.n, i), r.start = __shfl_sync(0xffffffffu, mine.start, i);
+            r.prefix = __shfl_sync(0xffffffffu, mine.prefix, i);
+            const int tiles = (r.n * g + tile - 1) / tile;
+            uint32_t sum = 0;
+#pragma unroll 1
+            for (int qt = lane; qt < tiles; qt += 32) sum += tile_at(a, r, qt, tile).count + lead;
+            sum = __reduce_add_sync(0xffffffffu, sum);
+            if (lane == 0) scratch[b] = sum * a.pass_heads;
+        }
     }
     __syncthreads();
     if (warp == 0) {
         uint32_t total = 0;
 #pragma unroll 1
         for (int b = lane; b < a.B; b += 32) total += scratch[b];
-#pragma unroll
-        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        total = __reduce_add_sync(0xffffffffu, total);
         const uint32_t ctas = min(gridDim.x, total);
         uint32_t u0 = 0, u1 = 0;
         if (blockIdx.x < ctas) {  // runs of two lengths, the longer ones first
