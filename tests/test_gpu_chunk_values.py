@@ -1,0 +1,113 @@
+"""GPU: the chunk attention (``ops.paged_chunk_attention``) with values, weights and keys of unlike and extreme
+sizes, in both of its forms.
+
+Tolerances, per output element: the bound of ``test_gpu_chunk.py``, 2^-19 A + 2^-17 S A with A = sum p |v| and
+S = scale * max sum |q k| over the visible rows, bf16 2^-8 (A + |out|) more for the weights' and the result's
+rounding; and what an element is held to beside its row's largest: with R = sum p * (the largest |v| of the row),
+a value to 2^-29 of its row's largest element, a weight to 2^-39 of the largest of its page, 128 of them over values
+that are within 2^10 of one another: 128 * 2^-39 * 2^10 + 2^-29 < 2^-21, of R.
+"""
+
+from __future__ import annotations
+
+import importlib
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_chunk import Case, _bound
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.float32, torch.bfloat16]
+FEW, MANY = [4, 2], [150, 40]  # rows of each request: the form for few rows, and the tensor cores
+HEADS = {"heads": 60, "kv_heads": 60, "layers": 1, "layer": 0}  # enough of them that a CTA's run has several pages
+
+
+@pytest.fixture(scope="module")
+def ops():
+    return importlib.import_module("unlimited-ocr-max_b200.ops")
+
+
+def _np(t):
+    return t.float().numpy()
+
+
+def _formula(c, window=0, prefix=None):
+    """The formula in float64: out, A, S and R of each row (zeros for rows in no request)."""
+    q, k, v, pool = (t.double().to(DEV) for t in (c.q, c.k, c.v, c.pool[:, :, c.layer]))
+    T, heads, _ = q.shape
+    ref, mag, largest = (torch.zeros_like(q) for _ in range(3))
+    smag = torch.zeros((T, heads), dtype=torch.float64, device=DEV)
+    for b, (n, s0) in enumerate(zip(c.n, c.start)):
+        if not n:
+            continue
+        lo, rows = int(c.offsets[b]), torch.arange(s0 + n, device=DEV)
+        lut = torch.from_numpy(c.lut[b]).long().to(DEV)
+        K, V = (pool[lut, i].flatten(0, 1)[: s0 + n].clone() for i in (0, 1))
+        K[s0:], V[s0:] = k[lo: lo + n], v[lo: lo + n]
+        K, V = (t.repeat_interleave(heads // t.shape[1], 1).permute(1, 0, 2) for t in (K, V))
+        p = rows[s0:, None]
+        seen = rows <= p
+        if window:
+            seen &= (rows > p - window) | (rows < (0 if prefix is None else int(prefix[b])))
+        x = q[lo: lo + n].permute(1, 0, 2)
+        K, V = K.nan_to_num(0.0, 0.0, 0.0), V.nan_to_num(0.0, 0.0, 0.0)  # hidden rows of the pool
+        w = torch.softmax((x @ K.mT * c.scale).masked_fill(~seen, -math.inf), -1)
+        out = lambda t: t.permute(1, 0, 2)  # noqa: E731
+        ref[lo: lo + n], mag[lo: lo + n] = out(w @ V), out(w @ V.abs())
+        largest[lo: lo + n] = out(w @ V.abs().amax(-1, keepdim=True))
+        smag[lo: lo + n] = (x.abs() @ K.abs().mT * abs(c.scale)).masked_fill(~seen, 0).amax(-1).T
+    return tuple(t.cpu().numpy() for t in (ref, mag, smag, largest))
+
+
+def _check(c, ops, **more):
+    """Against the formula, with the rows' largest elements in the bound."""
+    got = _np(c.run(ops, **more)[0]).astype(np.float64)
+    ref, mag, smag, largest = _formula(c, **more)
+    live = slice(int(c.offsets[0]), int(c.offsets[-1]))
+    tol = (_bound(c.dtype, ref, mag, smag) + 2.0 ** -21 * largest)[live]
+    far = np.abs(got - ref)[live]
+    assert (far <= tol).all(), (int((~(far <= tol)).sum()), np.argwhere(~(far <= tol))[:4].tolist(), float(np.nanmax(far / tol)))
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [FEW, MANY])
+@pytest.mark.parametrize("span", [9, 12, 30, 60])
+def test_rows_of_values_of_unlike_sizes(ops, oracle, dtype, n, span):
+    c = Case(dtype, n, [200, 300], seed=33, **HEADS)
+    rng = np.random.default_rng(span)
+    for t in (c.v, c.pool[:, 1]):
+        t *= torch.from_numpy(2.0 ** rng.integers(-span, span + 1, (*t.shape[:-1], 1)).astype(np.float32)).to(dtype)
+    _check(c, ops)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [FEW, MANY])
+def test_rows_of_zeros_among_small_and_large_ones(ops, oracle, dtype, n):
+    c = Case(dtype, n, [256, 130], seed=34, **HEADS)
+    rows = torch.arange(128)
+    for p in range(c.pool.shape[0]):
+        c.pool[p, 1][:, rows % 3 == 0] *= 0
+        c.pool[p, 1][:, rows % 3 == 1] *= 2.0 ** -70
+    _check(c, ops)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [FEW, MANY])
+@pytest.mark.parametrize("bits", [30, 45, 60])
+@pytest.mark.parametrize("first", [True, False])
+def test_small_weights_of_large_values(ops, oracle, dtype, n, bits, first):
+    """A page whose weights are 2^-bits of the others' and whose values 2^(bits + 10) times theirs: it makes up the
+    result, whether the walk meets it first or last."""
+    c = Case(dtype, n, [256, 256], seed=41, **HEADS)
+    c.q += 1  # a common direction, along which the page's keys differ
+    for b in (0, 1):
+        page = c.lut[b, 0 if first else 1]
+        c.pool[page, 0, c.layer] -= bits * math.log(2) / (c.scale * 128)
+        c.pool[page, 1, c.layer] *= 2.0 ** (bits + 10)
+    got = _check(c, ops)
+    assert np.abs(got).max() > 2.0 ** 6

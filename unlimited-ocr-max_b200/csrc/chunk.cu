@@ -29,8 +29,8 @@
 //
 // fp32: a product of fp32 rows is three products of fp16 halves, hi x hi + hi x lo + lo x hi, where
 // x = hi + lo to 2^-22 of x: a row of k (all of a page's rows where they are of like size), a query row and a page's v
-// are scaled by a power of two that brings their largest element to [2^14, 2^15), and the weights by 2^7 above their
-// headroom, so the halves keep their bits over fp16's exponent range. The small products go into the accumulator
+// are scaled by a power of two that brings their largest element to [2^14, 2^15), and a row's weights on a page to at most
+// 2^14, so the halves keep their bits over fp16's exponent range. The small products go into the accumulator
 // first: the tensor core's additions truncate, and only the last 8 then round at the result's full size. bf16: one
 // product; the weights are rounded to bf16, as the tensor core takes both operands in one type.
 // Values that are not finite are kept out of the V operand (0 x inf would reach rows that do not see
@@ -510,12 +510,13 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
 
 // ---- the softmax warps ------------------------------------------------------------------------
 // Two threads per row of the query tile (its TMEM lane): columns and dimensions [64 half, 64 half + 64) each. A row's
-// weights are 2^(score - m); m is at most 7 below the row's maximum so far, and where a page exceeds that the row's
-// warps raise m and scale what they have. bf16: the tensor core adds the products of 16 pages in TMEM, which then come
-// into the threads' registers; fp32: of one page, for its own additions truncate (the threads' round to nearest:
-// 8.6e-7 off at 8192 rows, 1.2e-6 with two pages to a sum and no faster). The fp32 weights are 2^7 larger: at most
-// 2^14, and their halves resolve 2^-25.
-constexpr float kHeadroom = 7.f, kLift = 7.f;
+// sums are of 2^(score - m) and of that times values; m is at most 7 below the row's maximum so far, and where a page
+// exceeds that the row's warps raise m and scale what they have. bf16: the weights in the operand are 2^(score - m), and the
+// tensor core adds the products of 16 pages in TMEM, which then come into the threads' registers. fp32: of one page, for
+// its own additions truncate (the threads' round to nearest: 8.6e-7 off at 8192 rows, 1.2e-6 with two pages to a sum and
+// no faster); the weights' fp16 halves resolve 2^-25, so they are 2^(score - the page's maximum + 14), 2^-39 of the page's
+// largest, and the page's sum takes 2^(its maximum - m - 14): weights of 2^-60 beside values of 2^70 count in full.
+constexpr float kHeadroom = 7.f, kLift = 14.f;
 // Row `row` of the values of page t (this head's 128 columns).
 template <bool kF32>
 UOCR_DEV const char* value_row(const ChunkArgs& a, const Walk& w, int t, int row) {
@@ -697,7 +698,8 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
             }
             s.xmax[u & 1][half][row] = top;
             named_bar_sync(pair_bar, 64);
-            const float mn = fmaxf(m, fmaxf(top, s.xmax[u & 1][half ^ 1][row]));
+            const float page_max = fmaxf(top, s.xmax[u & 1][half ^ 1][row]);
+            const float mn = fmaxf(m, page_max);
             float keep = 1.f;
             const bool raised = __any_sync(0xffffffffu, mn > m + kHeadroom);  // the same in both warps of the rows
             if (raised) {
@@ -705,11 +707,14 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
                 l *= keep;
                 m = mn;
             }
+            // the operand's weights are 2^(score - ref), times 2^14 in fp32; one of 1 there counts `unit` in the sums
+            const float ref = kF32 ? page_max : m;
+            const float unit = !kF32 ? 1.f : ref == -INFINITY ? 0.f : exp2_fast(ref - m - kLift);
             const float old_scale = sum_scale;
-            sum_scale = page.y;
+            sum_scale = page.y * unit;
             const bool fresh = j % kSumPages<kF32> == 0;  // a new sum in TMEM
             if (run) {
-                const float base = (kF32 ? kLift : 0.f) - (m == -INFINITY ? 0.f : m);
+                const float base = (kF32 ? kLift : 0.f) - (ref == -INFINITY ? 0.f : ref);
                 const uint64_t q2 = pair(factor, factor), s2 = pair(base, base);
                 uint64_t sum2[2] = {0, 0};
 #pragma unroll
@@ -735,7 +740,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
                 }
                 uint32_t u0, u1;
                 unpair(add2(sum2[0], sum2[1]), u0, u1);
-                l += __uint_as_float(u0) + __uint_as_float(u1);
+                l += (__uint_as_float(u0) + __uint_as_float(u1)) * unit;
                 tmem_wait_st();
                 tc_fence_before();
             }
