@@ -147,9 +147,10 @@ UOCR_API int uocr_paged_decode_attention(const float* q, const float* k_new, con
  * stores is read or stored for no other request of the call.
  * Sums and softmax in fp32. Two forms, by T x heads / kv_heads against B: up to 16 (fp32; bf16 8) rows of
  * (token, query head) a request and KV head on average are computed on the fp32 units, more on the tensor cores: fp32
- * there as three products of fp16 halves, q and keys to 2^-22 of themselves (or 2^-29 of their
- * row's largest element), values to 2^-38 of the largest finite one of their page and head, weights to 2^-39 of the
- * largest that the row has on their page; bf16 weights rounded to bf16. A
+ * there as three products of fp16 halves, q, keys and values to 2^-22 of themselves (or 2^-29 of their
+ * row's largest finite element), weights to 2^-39 of the largest that the row has on their page (where its values' rows are of
+ * unlike size: the largest product of a weight and a row's size); bf16 weights rounded to bf16. Within this, hidden
+ * rows may decide how a visible one rounds. A
  * visible fp32 key with an element that is not finite makes the row NaN there. A wait inside the
  * kernel that runs out (200 ms) ends it with NaN in the rows concerned.
  * The workspace (uocr_paged_chunk_workspace_bytes(...) bytes on the current device, 0 for sizes that the call

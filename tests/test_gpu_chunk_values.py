@@ -111,3 +111,31 @@ def test_small_weights_of_large_values(ops, oracle, dtype, n, bits, first):
         c.pool[page, 1, c.layer] *= 2.0 ** (bits + 10)
     got = _check(c, ops)
     assert np.abs(got).max() > 2.0 ** 6
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [FEW, MANY])
+@pytest.mark.parametrize("large", [1e12, 1e13, 1e30])
+@pytest.mark.parametrize("whole_row", [False, True])
+def test_a_large_value_of_a_later_token(ops, oracle, dtype, n, large, whole_row):
+    """Tokens in front of it do not see it."""
+    c = Case(dtype, n, [100, 60], seed=31, **HEADS)
+    clean = _np(c.run(ops)[0])
+    at = n[0] - 2  # the last row but one of the first request
+    c.v[at, 1, slice(None) if whole_row else 17] = large
+    got = _check(c, ops)
+    # rows that do not see it: within the bound of the formula on both sides, and of the clean call
+    tol = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -12
+    assert (np.abs(got[:at] - clean[:at]) <= tol).all() and (got[n[0]:] == clean[n[0]:]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [FEW, MANY])
+@pytest.mark.parametrize("large", [1e13, 1e30])
+def test_large_values_outside_the_window(ops, oracle, dtype, n, large):
+    """Rows that no token, or only the first tokens, see, on the pages of rows that all see."""
+    c = Case(dtype, n, [300, 129], seed=32, **HEADS)
+    for r in range(140, 180):  # behind the prefix, in front of the window of all tokens or of the later ones
+        c.pool[c.lut[0, r // 128], 1, c.layer, r % 128] *= large
+    _check(c, ops, window=130, prefix=[139, 0])
+    _check(c, ops, window=120, prefix=[139, 0])

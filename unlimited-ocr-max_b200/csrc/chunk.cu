@@ -28,8 +28,8 @@
 // 3. chunk_join_kernel.
 //
 // fp32: a product of fp32 rows is three products of fp16 halves, hi x hi + hi x lo + lo x hi, where
-// x = hi + lo to 2^-22 of x: a row of k (all of a page's rows where they are of like size), a query row and a page's v
-// are scaled by a power of two that brings their largest element to [2^14, 2^15), and a row's weights on a page to at most
+// x = hi + lo to 2^-22 of x: a query row, and a row of k or v (all of a page's rows where they are of like size), are
+// scaled by a power of two that brings their largest element to [2^14, 2^15), and a row's weights on a page to at most
 // 2^14, so the halves keep their bits over fp16's exponent range. The small products go into the accumulator
 // first: the tensor core's additions truncate, and only the last 8 then round at the result's full size. bf16: one
 // product; the weights are rounded to bf16, as the tensor core takes both operands in one type.
@@ -66,11 +66,12 @@ constexpr uint32_t kTeamBar = 1, kPairBar = 2;  // all softmax warps; the two wa
 // TMEM columns
 constexpr uint32_t kColS = 0, kColPv = 256, kColQ = 384;
 
-// Beside a page's operands: 1 / scale of each row of k, and of all of them where they share one (else 0); 1 / scale of
-// v, and which rows of v are not finite. bf16 has the last of these only.
+// Beside a page's operands: 1 / scale of each row of k, and of all of them where they share one (else 0); the binary
+// logarithm of 1 / scale of each row of v, and 1 / scale of all of them where they share one (else 0); and which rows
+// of v are not finite. bf16 has the last of these only.
 struct alignas(16) PageMeta {
-    float keys[kPageRows];
-    float all_keys, values;
+    float keys[kPageRows], values_log2[kPageRows];
+    float all_keys, all_values;
     float pad[2];
     uint32_t bad[4];
 };
@@ -98,7 +99,7 @@ struct Shared {
     volatile int abort;
     Run run;
     Walk walk[kThreads / 32], now[kTeamWarps];
-    float xmax[2][2][kTile], xsum[2][kTile];
+    float xmax[2][2][kTile], xsum[2][kTile], xref[2][kTile];
 };
 
 // Has the phase of `parity` completed? (No suspension, unlike try_wait.)
@@ -187,6 +188,7 @@ UOCR_DEV void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
 // the values are smaller than 2^14 after scaling, which costs them bits they do not have)
 UOCR_DEV float scale_up(uint32_t bits) { return __uint_as_float((268u - max(bits >> 23, 15u)) << 23); }
 UOCR_DEV float scale_down(uint32_t bits) { return __uint_as_float((max(bits >> 23, 15u) - 14u) << 23); }
+UOCR_DEV float scale_down_log2(uint32_t bits) { return (float)((int)max(bits >> 23, 15u) - 141); }
 
 // ---- the first launch: rows into operands ------------------------------------------------------
 UOCR_DEV bool odd_f32(uint32_t e) { return (e & 0x7F800000u) == 0x7F800000u; }
@@ -291,80 +293,67 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
                 if (row >= cached && row < known) __stcs(reinterpret_cast<uint4*>(pool + row * row_bytes), x[i]);
             }
         }
-        float up = 1.f;
-        uint32_t my_top = 0, page_top = 0;  // fp32, k: lane i has the largest magnitude of row i
-        if (v) {
-            // values that are not finite leave the operand; fp32: one scale for the page, whose rows are summed over
-            uint32_t top = 0, bad = 0;
-#pragma unroll
-            for (int i = 0; i < kWords; ++i)
-                top = kF32 ? max(top, top_of(x[i])) : top | odd_bf16(x[i].x) | odd_bf16(x[i].y) | odd_bf16(x[i].z) | odd_bf16(x[i].w);
-            if (kF32) top = __reduce_max_sync(0xffffffffu, top);
-            if (kF32 ? top >= 0x7F800000u : __any_sync(0xffffffffu, top != 0)) {  // rare
-                top = 0;
-#pragma unroll
-                for (int i = 0; i < kWords; ++i) {
-                    bool row_bad = false;
-                    auto drop = [&](uint32_t& e) {
-                        if (kF32) {
-                            if (odd_f32(e)) e = 0, row_bad = true;
-                        } else {
-                            const uint32_t o = odd_bf16(e);
-                            if (o & 0x00008000u) e &= 0xFFFF0000u;
-                            if (o & 0x80000000u) e &= 0x0000FFFFu;
-                            row_bad |= o != 0;
-                        }
-                    };
-                    drop(x[i].x), drop(x[i].y), drop(x[i].z), drop(x[i].w);
-                    const uint32_t who = __ballot_sync(0xffffffffu, row_bad);
-                    if (kF32) bad |= (who ? 1u : 0u) << i;
-                    else bad |= ((who & 0xFFFFu ? 1u : 0u) | (who >> 16 ? 2u : 0u)) << (2 * i);
-                    if (kF32) top = max(top, top_of(x[i]));
-                }
-                if (kF32) top = __reduce_max_sync(0xffffffffu, top);
-            }
-            __syncthreads();  // tops may still be read
-            if (lane == 0) tops[warp] = top, bads[warp] = bad;
-            __syncthreads();
-            if (kF32) {
-                top = __reduce_max_sync(0xffffffffu, tops[lane & 7]);
-                up = scale_up(top);
-                if (threadIdx.x == 0) meta.values = scale_down(top);
-            }
-            if (threadIdx.x < 4) meta.bad[threadIdx.x] = bads[2 * threadIdx.x] | bads[2 * threadIdx.x + 1] << 16;
-        } else if (kF32) {
+        uint32_t my_top = 0;  // fp32: lane i has the largest magnitude of row i
+        if constexpr (kF32) {
+            uint32_t bad = 0;
 #pragma unroll
             for (int i = 0; i < kWords; ++i) {
                 uint32_t top = __reduce_max_sync(0xffffffffu, top_of(x[i]));
-                if (top >= 0x7F800000u) {  // rare: the row's scores become NaN; it sets no scale
+                if (top >= 0x7F800000u) {  // rare. Elements that are not finite set no scale; of v they leave the operand, with k the row's scores become NaN
                     uint32_t m = 0;
                     auto mark = [&](uint32_t& e) {
-                        if (odd_f32(e)) e = 0x7FFFFFFFu;
+                        if (odd_f32(e)) e = v ? 0 : 0x7FFFFFFFu;
                         else m = max(m, e & 0x7FFFFFFFu);
                     };
                     mark(x[i].x), mark(x[i].y), mark(x[i].z), mark(x[i].w);
                     top = __reduce_max_sync(0xffffffffu, m);
+                    bad |= 1u << i;
                 }
                 if (lane == i) my_top = top;
             }
-            page_top = __reduce_max_sync(0xffffffffu, my_top);
-            if (lane == 0) tops[warp] = page_top;
+            uint32_t page_top = __reduce_max_sync(0xffffffffu, my_top);
+            __syncthreads();  // tops may still be read
+            if (lane == 0) tops[warp] = page_top, bads[warp] = bad;
             __syncthreads();
             page_top = __reduce_max_sync(0xffffffffu, tops[lane & 7]);
-            // A row within 2^10 of the page's largest takes the page's scale (its halves still hold 2^-29 of it);
-            // others have their own.
+            // A row within 2^10 of the page's largest can take the page's scale (its halves still hold 2^-29 of it). A key
+            // that is not has its own. Values are summed over the rows: one scale for all of them, or each its
+            // own, for the largest may be one that a token does not see.
             const bool near = my_top == 0 || (my_top >> 23) + 10 >= page_top >> 23;
-            if (near) my_top = page_top;
             const bool all = __syncthreads_and(near || lane >= 16);
-            if (lane < 16) meta.keys[warp * 16 + lane] = scale_down(my_top);
-            if (threadIdx.x == 0) meta.all_keys = all ? scale_down(page_top) : 0.f;
+            if (v ? all : near) my_top = page_top;
+            if (lane < 16) (v ? meta.values_log2 : meta.keys)[warp * 16 + lane] = v ? scale_down_log2(my_top) : scale_down(my_top);
+            if (threadIdx.x == 0) (v ? meta.all_values : meta.all_keys) = all ? scale_down(page_top) : 0.f;
+        } else if (v) {
+            // values that are not finite leave the operand
+            uint32_t odd = 0, bad = 0;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) odd |= odd_bf16(x[i].x) | odd_bf16(x[i].y) | odd_bf16(x[i].z) | odd_bf16(x[i].w);
+            if (__any_sync(0xffffffffu, odd != 0)) {  // rare
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    bool row_bad = false;
+                    auto drop = [&](uint32_t& e) {
+                        const uint32_t o = odd_bf16(e);
+                        if (o & 0x00008000u) e &= 0xFFFF0000u;
+                        if (o & 0x80000000u) e &= 0x0000FFFFu;
+                        row_bad |= o != 0;
+                    };
+                    drop(x[i].x), drop(x[i].y), drop(x[i].z), drop(x[i].w);
+                    const uint32_t who = __ballot_sync(0xffffffffu, row_bad);
+                    bad |= ((who & 0xFFFFu ? 1u : 0u) | (who >> 16 ? 2u : 0u)) << (2 * i);
+                }
+            }
+            if (lane == 0) bads[warp] = bad;
+            __syncthreads();
         }
+        if (v && threadIdx.x < 4) meta.bad[threadIdx.x] = bads[2 * threadIdx.x] | bads[2 * threadIdx.x + 1] << 16;
         unsigned char* out = im.operands + (index * 2 + v) * kOperandBytes<kF32>;
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
             const int row = row0 + i * kPer;
             if constexpr (kF32) {
-                if (!v) up = scale_up(__shfl_sync(0xffffffffu, my_top, i));
+                const float up = scale_up(__shfl_sync(0xffffffffu, my_top, i));
                 uint2 hi, lo;
                 split2(__uint_as_float(x[i].x) * up, __uint_as_float(x[i].y) * up, hi.x, lo.x);
                 split2(__uint_as_float(x[i].z) * up, __uint_as_float(x[i].w) * up, hi.y, lo.y);
@@ -663,7 +652,8 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
             const PageMeta& pm = s.meta[u & 7];
             const float2 page = kF32 ? *reinterpret_cast<const float2*>(&pm.all_keys) : make_float2(1.f, 1.f);
             const uint4 bad = *reinterpret_cast<const uint4*>(pm.bad);
-            const float all_keys = page.x, factor = kF32 && all_keys != 0.f ? fmaxf(qscale * all_keys, 1e-37f) : qscale;
+            const float all_keys = page.x;
+            float factor = kF32 && all_keys != 0.f ? fmaxf(qscale * all_keys, 1e-37f) : qscale;
             uint32_t x[64];
             float top = -INFINITY;
             if (run) {
@@ -696,9 +686,12 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
                 }
                 top = fmaxf(top, top2) * factor;
             }
-            s.xmax[u & 1][half][row] = top;
+            // NaN: a warp that has given up; its partner then does too, so that both go the same way below
+            s.xmax[u & 1][half][row] = alive ? fmaxf(top, -INFINITY) : NAN;
             named_bar_sync(pair_bar, 64);
-            const float page_max = fmaxf(top, s.xmax[u & 1][half ^ 1][row]);
+            const float other = s.xmax[u & 1][half ^ 1][row];
+            alive = alive && other == other;
+            const float page_max = fmaxf(top, other);
             const float mn = fmaxf(m, page_max);
             float keep = 1.f;
             const bool raised = __any_sync(0xffffffffu, mn > m + kHeadroom);  // the same in both warps of the rows
@@ -708,10 +701,33 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
                 m = mn;
             }
             // the operand's weights are 2^(score - ref), times 2^14 in fp32; one of 1 there counts `unit` in the sums
-            const float ref = kF32 ? page_max : m;
+            float ref = kF32 ? page_max : m;
             const float unit = !kF32 ? 1.f : ref == -INFINITY ? 0.f : exp2_fast(ref - m - kLift);
             const float old_scale = sum_scale;
             sum_scale = page.y * unit;
+            const bool unlike = kF32 && alive && page.y == 0.f;
+            if (unlike) {
+                // A scale for each row of v: its weight takes 1 / scale, and the operand's weights are relative to the largest
+                // of these products, of the rows that this one sees. l takes the weights alone.
+                float most = -INFINITY, sum = 0.f;
+                if (run) {
+                    const float shift = kLift - (ref == -INFINITY ? 0.f : ref);
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        const float score = __uint_as_float(x[i]) * factor;
+                        sum += exp2_fast(score + shift);
+                        const float w = score + pm.values_log2[half * 64 + i];
+                        most = fmaxf(most, w);
+                        x[i] = __float_as_uint(w);
+                    }
+                    l = fmaf(sum, unit, l);
+                }
+                s.xref[half][row] = most;
+                named_bar_sync(pair_bar, 64);
+                ref = fmaxf(most, s.xref[half ^ 1][row]);
+                factor = 1.f;
+                sum_scale = ref == -INFINITY ? 0.f : exp2_fast(ref - m - kLift);
+            }
             const bool fresh = j % kSumPages<kF32> == 0;  // a new sum in TMEM
             if (run) {
                 const float base = (kF32 ? kLift : 0.f) - (ref == -INFINITY ? 0.f : ref);
@@ -740,7 +756,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
                 }
                 uint32_t u0, u1;
                 unpair(add2(sum2[0], sum2[1]), u0, u1);
-                l += (__uint_as_float(u0) + __uint_as_float(u1)) * unit;
+                if (!unlike) l += (__uint_as_float(u0) + __uint_as_float(u1)) * unit;
                 tmem_wait_st();
                 tc_fence_before();
             }
