@@ -17,7 +17,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_chunk import Case, _bound
+from test_gpu_chunk import Case, _bound, _round
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -64,11 +64,11 @@ def _formula(c, window=0, prefix=None):
 
 
 def _check(c, ops, **more):
-    """Against the formula, with the rows' largest elements in the bound."""
+    """Against the formula, with the rows' largest elements in the bound (and without its absolute part)."""
     got = _np(c.run(ops, **more)[0]).astype(np.float64)
     ref, mag, smag, largest = _formula(c, **more)
     live = slice(int(c.offsets[0]), int(c.offsets[-1]))
-    tol = (_bound(c.dtype, ref, mag, smag) + 2.0 ** -21 * largest)[live]
+    tol = (_bound(c.dtype, ref, mag, smag) - 1e-30 + 2.0 ** -21 * largest)[live]
     far = np.abs(got - ref)[live]
     assert (far <= tol).all(), (int((~(far <= tol)).sum()), np.argwhere(~(far <= tol))[:4].tolist(), float(np.nanmax(far / tol)))
     return got
@@ -139,3 +139,32 @@ def test_large_values_outside_the_window(ops, oracle, dtype, n, large):
         c.pool[c.lut[0, r // 128], 1, c.layer, r % 128] *= large
     _check(c, ops, window=130, prefix=[139, 0])
     _check(c, ops, window=120, prefix=[139, 0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,start", [(FEW, [400, 900]), (MANY, [400, 900])])
+@pytest.mark.parametrize("size", [2.0 ** 64, 2.0 ** 66, 2.0 ** 112, 2.0 ** 120, 3e38])
+@pytest.mark.parametrize("where", ["all", "first page", "last page"])
+def test_values_up_to_the_largest_of_the_type(ops, oracle, dtype, n, start, size, where):
+    """A mean of finite values is finite: sums of weights times values stay inside the type's range."""
+    c = Case(dtype, n, start, seed=42, **HEADS)
+    large = lambda t: _round((0.75 + 0.25 * torch.rand(t.shape)).numpy() * size, dtype)  # noqa: E731
+    for b in (0, 1):
+        for i in range(start[b] // 128):
+            if where == "all" or i == (0 if where == "first page" else start[b] // 128 - 1):
+                c.pool[c.lut[b, i], 1] = large(c.pool[0, 1])
+    if where == "all":
+        c.v = large(c.v)
+    got = _check(c, ops)
+    assert np.isfinite(got[: sum(n)]).all() and np.abs(got).max() > size * 2.0 ** -6
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [FEW, MANY])
+@pytest.mark.parametrize("size", [1e-20, 1e-30, 1e-34])
+def test_small_values(ops, dtype, n, size):
+    """Results keep their bits down to 2^-126: sums of weights of at most 2^-10 times values are 2^-124 here."""
+    c = Case(dtype, n, [400, 300], seed=45, **HEADS)
+    c.v *= size
+    c.pool[:, 1] *= size
+    _check(c, ops)

@@ -67,12 +67,13 @@ constexpr uint32_t kTeamBar = 1, kPairBar = 2;  // all softmax warps; the two wa
 constexpr uint32_t kColS = 0, kColPv = 256, kColQ = 384;
 
 // Beside a page's operands: 1 / scale of each row of k, and of all of them where they share one (else 0); the binary
-// logarithm of 1 / scale of each row of v, and 1 / scale of all of them where they share one (else 0); and which rows
-// of v are not finite. bf16 has the last of these only.
+// logarithms of 1 / scale of each row of v and of all of them (kUnlike: 0, they do not share one); are there large finite
+// values, of 2^50 or more, bf16 2^65 (kLarge), or rows of v that are not finite (kBad), and which. bf16 has the last two only.
+constexpr uint32_t kUnlike = 1, kLarge = 2, kBad = 4;
 struct alignas(16) PageMeta {
     float keys[kPageRows], values_log2[kPageRows];
-    float all_keys, all_values;
-    float pad[2];
+    float all_keys, all_values_log2;
+    uint32_t values_are, pad;
     uint32_t bad[4];
 };
 
@@ -192,6 +193,7 @@ UOCR_DEV float scale_down_log2(uint32_t bits) { return (float)((int)max(bits >> 
 
 // ---- the first launch: rows into operands ------------------------------------------------------
 UOCR_DEV bool odd_f32(uint32_t e) { return (e & 0x7F800000u) == 0x7F800000u; }
+UOCR_DEV uint32_t large_bf16(uint32_t e) { return e & e << 1 & 0x40004000u; }  // per half: 2^65 or more, odd ones among them
 UOCR_DEV uint32_t odd_bf16(uint32_t e) { return ((e & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }  // per half, its top bit
 UOCR_DEV uint32_t top_of(const uint4& x) {
     return max(max(x.x & 0x7FFFFFFFu, x.y & 0x7FFFFFFFu), max(x.z & 0x7FFFFFFFu, x.w & 0x7FFFFFFFu));
@@ -293,6 +295,11 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
                 if (row >= cached && row < known) __stcs(reinterpret_cast<uint4*>(pool + row * row_bytes), x[i]);
             }
         }
+        auto any_bad = [&] {
+            uint32_t any = 0;
+            for (int i = 0; i < 8; ++i) any |= bads[i];
+            return any ? kBad : 0u;
+        };
         uint32_t my_top = 0;  // fp32: lane i has the largest magnitude of row i
         if constexpr (kF32) {
             uint32_t bad = 0;
@@ -323,13 +330,24 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
             const bool all = __syncthreads_and(near || lane >= 16);
             if (v ? all : near) my_top = page_top;
             if (lane < 16) (v ? meta.values_log2 : meta.keys)[warp * 16 + lane] = v ? scale_down_log2(my_top) : scale_down(my_top);
-            if (threadIdx.x == 0) (v ? meta.all_values : meta.all_keys) = all ? scale_down(page_top) : 0.f;
+            if (threadIdx.x == 0) {
+                if (v) {
+                    meta.all_values_log2 = all ? scale_down_log2(page_top) : 0.f;
+                    meta.values_are = (all ? 0 : kUnlike) | (page_top >> 23 >= 127 + 50 ? kLarge : 0) | any_bad();
+                } else {
+                    meta.all_keys = all ? scale_down(page_top) : 0.f;
+                }
+            }
         } else if (v) {
             // values that are not finite leave the operand
-            uint32_t odd = 0, bad = 0;
+            uint32_t large = 0, bad = 0;
+            auto look = [&] {
+                large = 0;
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) odd |= odd_bf16(x[i].x) | odd_bf16(x[i].y) | odd_bf16(x[i].z) | odd_bf16(x[i].w);
-            if (__any_sync(0xffffffffu, odd != 0)) {  // rare
+                for (int i = 0; i < kWords; ++i) large |= large_bf16(x[i].x) | large_bf16(x[i].y) | large_bf16(x[i].z) | large_bf16(x[i].w);
+            };
+            look();
+            if (__any_sync(0xffffffffu, large != 0)) {  // rare
 #pragma unroll
                 for (int i = 0; i < kWords; ++i) {
                     bool row_bad = false;
@@ -343,9 +361,11 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
                     const uint32_t who = __ballot_sync(0xffffffffu, row_bad);
                     bad |= ((who & 0xFFFFu ? 1u : 0u) | (who >> 16 ? 2u : 0u)) << (2 * i);
                 }
+                look();
             }
             if (lane == 0) bads[warp] = bad;
-            __syncthreads();
+            large = __syncthreads_or(large != 0);
+            if (threadIdx.x == 0) meta.values_are = (large ? kLarge : 0) | any_bad();
         }
         if (v && threadIdx.x < 4) meta.bad[threadIdx.x] = bads[2 * threadIdx.x] | bads[2 * threadIdx.x + 1] << 16;
         unsigned char* out = im.operands + (index * 2 + v) * kOperandBytes<kF32>;
@@ -505,7 +525,12 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
 // its own additions truncate (the threads' round to nearest: 8.6e-7 off at 8192 rows, 1.2e-6 with two pages to a sum and
 // no faster); the weights' fp16 halves resolve 2^-25, so they are 2^(score - the page's maximum + 14), 2^-39 of the page's
 // largest, and the page's sum takes 2^(its maximum - m - 14): weights of 2^-60 beside values of 2^70 count in full.
+// m is `room` above the maximum. From a page on that holds large values it is so by the logarithm of the tile's rows and the
+// headroom, so that the sums stay below the values, up to the type's largest ones. Up to there it is 28 below in fp32, where the
+// scale of a page's sum is 2^-28 of its values (so values down to the type's smallest normal ones keep their bits).
 constexpr float kHeadroom = 7.f, kLift = 14.f;
+template <bool kF32>
+constexpr float kRoom = kF32 ? -28.f : 0.f;
 // Row `row` of the values of page t (this head's 128 columns).
 template <bool kF32>
 UOCR_DEV const char* value_row(const ChunkArgs& a, const Walk& w, int t, int row) {
@@ -635,6 +660,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
         const int n = now.n, first_pos = now.t.first_pos, last_pos = now.t.last_pos, prefix = now.r.prefix;
         const int head_pages = now.t.head_pages - now.j, tail_page = now.t.tail_page - head_pages;  // page of the segment's j
         float sum_scale = 1.f;  // of the sum in TMEM
+        float room = kRoom<kF32>;
         for (int j = 0;; ++j) {
             if (j == n) {  // the next segment's queries, while the last products run
                 if (more) load_query(w);
@@ -650,8 +676,8 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
                              (a.window <= 0 || c0 > last_pos - a.window || c0 + kPageRows <= prefix);
             // keys of one scale: it goes into the factor; else 1 / scale of each one's key (a branch, rarely taken)
             const PageMeta& pm = s.meta[u & 7];
-            const float2 page = kF32 ? *reinterpret_cast<const float2*>(&pm.all_keys) : make_float2(1.f, 1.f);
-            const uint4 bad = *reinterpret_cast<const uint4*>(pm.bad);
+            const float4 page = kF32 ? *reinterpret_cast<const float4*>(&pm.all_keys) : make_float4(1.f, 0.f, 0.f, 0.f);
+            const uint32_t values_are = kF32 ? __float_as_uint(page.z) : pm.values_are;
             const float all_keys = page.x;
             float factor = kF32 && all_keys != 0.f ? fmaxf(qscale * all_keys, 1e-37f) : qscale;
             uint32_t x[64];
@@ -692,20 +718,27 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
             const float other = s.xmax[u & 1][half ^ 1][row];
             alive = alive && other == other;
             const float page_max = fmaxf(top, other);
-            const float mn = fmaxf(m, page_max);
-            float keep = 1.f;
+            float mn = m, keep = 1.f;
+            if ((values_are & kLarge) && room == kRoom<kF32>) {
+                asm volatile("");  // a branch, rarely taken
+                room = kHeadroom + 7.f + (32 - __clz(now.t.count - 1));
+                mn = m + (room - kRoom<kF32>);
+            }
+            mn = fmaxf(mn, page_max + room);
             const bool raised = __any_sync(0xffffffffu, mn > m + kHeadroom);  // the same in both warps of the rows
             if (raised) {
                 keep = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
                 l *= keep;
                 m = mn;
             }
-            // the operand's weights are 2^(score - ref), times 2^14 in fp32; one of 1 there counts `unit` in the sums
+            // the operand's weights are 2^(score - ref), times 2^14 in fp32; one of 1 there counts `unit` in l, and a product
+            // with the values' operand `sum_scale` in the sums
             float ref = kF32 ? page_max : m;
-            const float unit = !kF32 ? 1.f : ref == -INFINITY ? 0.f : exp2_fast(ref - m - kLift);
+            auto counts = [&](float log2) { return ref == -INFINITY ? 0.f : exp2_fast(ref - m + (log2 - kLift)); };
+            const float unit = kF32 ? counts(0.f) : 1.f;
             const float old_scale = sum_scale;
-            sum_scale = page.y * unit;
-            const bool unlike = kF32 && alive && page.y == 0.f;
+            if (kF32) sum_scale = counts(page.y);
+            const bool unlike = kF32 && alive && (values_are & kUnlike);
             if (unlike) {
                 // A scale for each row of v: its weight takes 1 / scale, and the operand's weights are relative to the largest
                 // of these products, of the rows that this one sees. l takes the weights alone.
@@ -726,7 +759,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
                 named_bar_sync(pair_bar, 64);
                 ref = fmaxf(most, s.xref[half ^ 1][row]);
                 factor = 1.f;
-                sum_scale = ref == -INFINITY ? 0.f : exp2_fast(ref - m - kLift);
+                sum_scale = counts(0.f);
             }
             const bool fresh = j % kSumPages<kF32> == 0;  // a new sum in TMEM
             if (run) {
@@ -764,7 +797,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
             if (j > 0 && (fresh || raised)) take_sum(u - 1, old_scale, keep, fresh, live);
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.p_full[u & 1]);
-            if (bad.x | bad.y | bad.z | bad.w) add_bad(now, u, c0 / kPageRows, pos);
+            if (values_are & kBad) add_bad(now, u, c0 / kPageRows, pos);
         }
         take_sum(unit0 + n - 1, sum_scale, 1.f, true, live);
         unit0 += n;

@@ -198,6 +198,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(const __grid_co
         const int rows = min(NQ, w.r.n * g - qt * NQ);
         const bool whole = w.whole(), begins = w.j == 0, ends = w.j + w.n == w.t.count;
         const int first_pos = w.t.first_pos, last_pos = w.t.last_pos;
+        // weights are 1 / (a power of two not below the rows of the tile's pages) at most: sums stay below the values
+        const float most = __uint_as_float((127 - 7 - (32 - __clz(w.t.count - 1))) << 23);
         for (int u = 0; u < n; ++u) {
             uint32_t id = 0;
             if (u + 1 < n) id = page_id(u + 1);
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(const __grid_co
                     if (!seen) sc[j] = -INFINITY;
                 }
                 const float mn = fmaxf(m[j], warp_max(sc[j]));
-                const float p = exp2_fast(sc[j] - (mn == -INFINITY ? 0.f : mn));
+                const float p = exp2_fast(sc[j] - (mn == -INFINITY ? 0.f : mn)) * most;
                 const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m[j] - mn);
                 m[j] = mn;
                 l[j] = l[j] * alpha + p;
