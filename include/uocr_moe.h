@@ -448,6 +448,12 @@ UOCR_API int uocr_moe_device_status(const void* workspace, uocr_stream_t stream)
  * calls after the status read are correct. 0 turns it off. Not thread-safe; for tests only. */
 UOCR_API int uocr_moe_test_wait_extra(int extra);
 
+/* Test hook (no counterpart in the reference): in the chunk attentions launched from now on (tensor-core form) the softmax
+ * warps of the bit mask `warps` (8 of a CTA: warp w has query rows 32 (w % 4) on and half w / 4 of the columns) act as if
+ * their last wait of each query tile had run out; used to check that this leaves NaN and that the next call is
+ * correct. 0 turns it off. Not thread-safe; for tests only. */
+UOCR_API int uocr_chunk_test_expire(int warps);
+
 #ifdef __cplusplus
 }
 #endif

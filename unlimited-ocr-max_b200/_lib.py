@@ -113,6 +113,7 @@ SIGNATURES: dict[str, tuple] = {
     "uocr_ipc_import": (I32, [P, ctypes.c_uint64, ctypes.POINTER(ctypes.c_void_p)]),
     "uocr_ipc_close": (I32, [P, ctypes.c_uint64]),
     "uocr_moe_test_wait_extra": (I32, [I32]),
+    "uocr_chunk_test_expire": (I32, [I32]),
 }
 
 _lock = threading.Lock()

@@ -52,6 +52,7 @@ namespace uocr {
 unsigned long long* g_decode_trace = nullptr;
 size_t g_decode_trace_bytes = 0;
 int g_decode_wait_extra = 0;
+int g_chunk_expire = 0;
 
 // Read a workspace's status word after `stream` finished; if it is set, clear it together with the
 // control words a failed call may have left behind (decode: DecodeCtl; prefill and exchange
@@ -1018,6 +1019,12 @@ int uocr_moe_device_status(const void* workspace, uocr_stream_t stream) {
     if (!workspace) return fail(UOCR_EINVAL, "device_status: null workspace");
     uint32_t code = 0;
     return uocr::read_clear_status(workspace, S(stream), &code);
+}
+
+int uocr_chunk_test_expire(int warps) {
+    if (warps < 0 || warps > 255) return fail(UOCR_EINVAL, "test_expire: %d outside 0..255", warps);
+    uocr::g_chunk_expire = warps;
+    return ok();
 }
 
 int uocr_moe_test_wait_extra(int extra) {

@@ -423,8 +423,8 @@ __device__ void copy_role(const ChunkArgs& a, Shared& s, unsigned char* ring, co
         }
         return true;
     };
-    if (run()) return;
-    s.abort = 1;  // a wait gave up: the copies in flight land before this CTA's memory is given back
+    if (!run()) s.abort = 1;  // a wait gave up
+    // The copies in flight land before this CTA's memory is given back (the issuing warp has seen them all, unless it gave up)
     for (uint32_t k = 0; k < kStages<kF32> && k < issued; ++k) {
         if (stage == 0) stage = kStages<kF32>, phase ^= 1;
         mbar_wait(&s.full[--stage], phase, nullptr);
@@ -799,6 +799,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
             if (lane == 0) mbar_arrive(&s.p_full[u & 1]);
             if (values_are & kBad) add_bad(now, u, c0 / kPageRows, pos);
         }
+        if (a.expire >> warp & 1) s.abort = 1, alive = false;
         take_sum(unit0 + n - 1, sum_scale, 1.f, true, live);
         unit0 += n;
         // to out, or column by column to the workspace
@@ -1035,6 +1036,7 @@ size_t chunk_workspace_bytes(const ChunkArgs& a, int sms) {
 cudaError_t launch_chunk_attention(const ChunkArgs& args, void* ws, int sms, cudaStream_t st) {
     ChunkArgs a = args;
     const int g = a.heads / a.kv_heads;
+    a.expire = g_chunk_expire;
     a.group_shift = 32;
     while (g >> (a.group_shift - 31)) ++a.group_shift;
     a.group_mul = ((1ull << a.group_shift) + g - 1) / g;

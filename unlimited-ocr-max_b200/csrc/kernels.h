@@ -60,6 +60,7 @@ struct ChunkArgs {
     float scale;
     // Set by the launcher: the KV heads of one pass over the call; n / (heads / kv_heads) as n * group_mul >> group_shift
     int head0, pass_heads, group_shift;
+    int expire;  // test hook: softmax warps (bits) whose last wait of a tile runs out
     unsigned long long group_mul;
 };
 constexpr int kChunkMaxRequests = 8192;
@@ -170,6 +171,7 @@ extern size_t g_decode_trace_bytes;
 // test hook: operand groups per slot the next decode launches' down phase waits for on top of the
 // real ones (capi.cu)
 extern int g_decode_wait_extra;
+extern int g_chunk_expire;
 cudaError_t launch_decode_layer(const DecodeArgs& a, cudaStream_t st);
 
 // prefill.cu
