@@ -46,3 +46,26 @@ def test_calls_after_an_expired_wait_are_correct(ops, hook, dtype, warps):
         assert hook.uocr_chunk_test_expire(0) == 0
         got, after = c.run(ops)
         assert torch.equal(got, want) and torch.equal(after.view(torch.uint8), pool.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("warps", [1 << 0, 1 << 1, 1 << 6, 255])
+def test_an_expired_wait_leaves_nan_and_nothing_wrong(ops, hook, dtype, warps):
+    """A row's columns belong to two warps: where one of them gives up, or works on what one that gave up has left, all 128 are NaN.
+    The other rows are right, and rows in no request are left."""
+    c = _case(dtype)
+    want, pool = c.run(ops)
+    assert hook.uocr_chunk_test_expire(warps) == 0
+    got, after = c.run(ops)
+    assert hook.uocr_chunk_test_expire(0) == 0
+    assert torch.equal(after.view(torch.uint8), pool.view(torch.uint8))
+    assert torch.equal(got[:3], want[:3]) and torch.equal(got[-5:], want[-5:])
+    lost = torch.isnan(got[3:-5])
+    assert torch.equal(lost.any(-1), lost.all(-1))
+    assert torch.equal(got[3:-5][~lost], want[3:-5][~lost])
+    for w in range(8):
+        if warps >> w & 1:  # rows 32 (w % 4) .. of each tile of 128
+            for at, n in ((0, 300), (300, 40)):
+                for r in range(at, at + n):
+                    if (r - at) % 128 // 32 == w % 4:
+                        assert lost[r].all()

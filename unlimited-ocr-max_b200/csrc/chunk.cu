@@ -803,11 +803,13 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
         take_sum(unit0 + n - 1, sum_scale, 1.f, true, live);
         unit0 += n;
         // to out, or column by column to the workspace
-        s.xsum[half][row] = l;
+        // A warp that gave up set s.abort in front of the arrivals that let others go on, so that whoever worked on what it left sees it
+        // here. NaN in one half's l makes the row NaN in both, here or by way of the parts' l.
+        s.xsum[half][row] = alive && !s.abort ? l : NAN;
         named_bar_sync(pair_bar, 64);
         const float total = s.xsum[0][row] + s.xsum[1][row];
         const bool whole = now.whole();
-        const float f = !alive ? NAN : whole ? 1.f / total : 1.f;
+        const float f = whole ? 1.f / total : 1.f;
         const uint64_t f2 = pair(f, f);
         const int slot = now.j == 0 ? 1 : 0;
         float* part = parts.slots + ((size_t)blockIdx.x * 2 + slot) * slot_floats(kTile);
