@@ -480,11 +480,7 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
     };
     auto run = [&] {
         auto next = [&](bool first) {
-            __syncwarp();
-            if (first) w = s.run.first;
-            const bool more = first ? s.run.some : w.next(a, g, kTile, kLead);
-            __syncwarp();
-            return __any_sync(0xffffffffu, more);
+            return __any_sync(0xffffffffu, first ? warp_first(w, s.run) : warp_next(w, a, g, kTile, kLead));
         };
         for (bool more = next(true); more; more = next(false), ++seg) {
             const int n = __reduce_max_sync(0xffffffffu, w.n);
@@ -640,14 +636,13 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
 
     Walk& w = s.walk[warp];
     Walk& now = s.now[warp];  // the segment at work
-    w = s.run.first;
-    bool more = s.run.some;
-    __syncwarp();
+    bool more = warp_first(w, s.run);
     int state[2] = {0, 0}, place[4] = {0, 0, 0, 0};
     uint32_t unit0 = 0;
     if (more) load_query(w);
     while (more) {
-        now = w;
+        __syncwarp();
+        if (lane == 0) now = w;
         __syncwarp();
         const int R = now.qt * kTile + row, rows = now.r.n * g - now.qt * kTile;  // valid rows of the tile
         const bool live = (warp & 3) * 32 < rows;                                 // this warp has some
@@ -655,8 +650,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
         m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < 64; ++i) acc[i] = 0;
-        more = w.next(a, g, kTile, kLead);  // w is one ahead from here on
-        __syncwarp();
+        more = warp_next(w, a, g, kTile, kLead);  // w is one ahead from here on
         const int n = now.n, first_pos = now.t.first_pos, last_pos = now.t.last_pos, prefix = now.r.prefix;
         const int head_pages = now.t.head_pages - now.j, tail_page = now.t.tail_page - head_pages;  // page of the segment's j
         float sum_scale = 1.f;  // of the sum in TMEM

@@ -158,9 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(const __grid_co
     find_run(a, s.run, reinterpret_cast<uint32_t*>(raw + sizeof(Shared<NQ>)), g, NQ, kLead);
     pdl_launch_dependents();
     Walk& w = s.walk[warp];
-    w = s.run.first;
-    bool more = s.run.some;
-    __syncwarp();
+    bool more = warp_first(w, s.run);
     int state[2] = {0, 0}, where[4] = {0, 0, 0, 0};
     const float factor = a.scale * kLog2e;
     // a segment's queries: thread (row, 4 columns)
@@ -310,9 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_rows_kernel(const __grid_co
             pl = next;
         }
         // the next segment's first keys and queries are on their way while this one is joined
-        __syncwarp();
-        more = w.next(a, g, NQ, kLead);
-        __syncwarp();
+        more = warp_next(w, a, g, NQ, kLead);
         if (more) {
             pl = place_of<kF32>(a, w, 0, page_id(0), g, NQ);
             load_keys<kF32>(a, pl, row0, lane, x);
