@@ -147,3 +147,17 @@ def test_every_page_of_every_tile_once(walk, n, start, g, kv, window, prefix, ti
             want += [(b, qt, h, j) for h in range(kv) for j in range(count.value)]
     assert [(b, qt, h, j + i) for _, b, qt, h, j, k in segments for i in range(k)] == want
     assert [s[0] for s in segments] == sorted(s[0] for s in segments)
+
+
+def test_requests_stay_inside_whatever_the_lengths_say(walk):
+    low, high = -2 ** 31, 2 ** 31 - 1
+    odd = [low, low + 1, -7, -1, 0, 1, 5, 99, 100, 101, 640, high - 1, high]
+    out = (ctypes.c_int * 4)()
+    for a in odd:
+        for b in odd:
+            for s in odd:
+                walk.request(100, 1, 5, _i32([a, b]), _i32([s]), _i32([b]), 0, out)
+                lo, n, start, prefix = out
+                assert 0 <= lo <= lo + n <= 100 and 0 <= start <= start + n <= 640 and prefix >= 0, (a, b, s, out[:])
+                if 0 <= a <= b <= 100 and 0 <= s <= 640:
+                    assert (lo, n, start) == (a, min(b - a, 640 - s), s)

@@ -17,7 +17,8 @@ UOCR_DEV Request request_at(const ChunkArgs& a, int b) {
     Request r;
     r.lo = min(max(__ldg(a.offsets + b), 0), a.T);
     r.start = min(max(__ldg(a.start + b), 0), a.lut_cols * kPageRows);
-    r.n = max(min(min(__ldg(a.offsets + b + 1), a.T) - r.lo, a.lut_cols * kPageRows - r.start), 0);
+    const int hi = min(max(__ldg(a.offsets + b + 1), 0), a.T);  // (from 0 on: a difference with INT_MIN would wrap)
+    r.n = max(min(hi - r.lo, a.lut_cols * kPageRows - r.start), 0);
     r.prefix = a.prefix ? max(__ldg(a.prefix + b), 0) : 0;
     return r;
 }
