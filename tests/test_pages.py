@@ -201,3 +201,16 @@ def test_a_full_pool_changes_nothing(pool, kvp):
         kvp.PagePool(0, 1, 1, device="cpu")
     with pytest.raises(TypeError):
         kvp.PagePool(1, 1, 1, dtype=torch.float16, device="cpu")
+
+
+@pytest.mark.parametrize("sizes", [(0, 4, 2, 0, 3, 2), (4, 4, 2, 0, 3, 0), (4, 5, 2, 0, 3, 2), (4, 0, 2, 0, 3, 2), (4, 4, 2, 7, 3, 2), (4, 4, 2, 0, 0, 2),
+                                   (4, 2048, 2, 0, 3, 2), (1 << 40, 4, 2, 0, 3, 2), (4, 4, 2, 0, 3, 8193), (4, 4, 2, 0, (1 << 22) + 1, 2),
+                                   (4, 4, 2, 0, 1 << 18, 8192), (4, 1024, 1024, 0, 1 << 22, 64), (1 << 28, 4, 2, 0, 1 << 22, 2)])
+def test_no_workspace_for_sizes_that_the_call_refuses(uocr, sizes):
+    lib = uocr.load()
+    T, heads, kv, dtype, cols, B = sizes
+    if T and B:
+        rc, _ = _chunk(lib, T=T, heads=heads, kv=kv, dtype=dtype, cols=cols, B=B, q_ld=1 << 18, k_ld=1 << 18, v_ld=1 << 18)
+        assert rc in (1, 4) and "null pointer" not in lib.uocr_last_error().decode()
+    assert lib.uocr_paged_chunk_workspace_bytes(T, heads, kv, dtype, cols, B) == 0
+    assert lib.uocr_paged_chunk_workspace_bytes(4, 4, 2, 0, 3, 2) > 0

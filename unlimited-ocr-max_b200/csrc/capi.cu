@@ -311,10 +311,16 @@ int uocr_paged_decode_attention(const float* q, const float* k_new, const float*
                        "paged_decode_attention: launch");
 }
 
+// The (query tile, head, page) units of a call, with what a tile counts beside its pages, are counted in 32 bits. The form
+// for few rows has at most three tiles a request: a factor of four is kept free.
+static bool chunk_units_ok(int64_t T, int64_t heads, int64_t kv_heads, int64_t lut_cols, int64_t B) {
+    return (T * (heads / kv_heads) / 128 + B) * kv_heads <= (int64_t(1) << 30) / (lut_cols + 4);
+}
+
 size_t uocr_paged_chunk_workspace_bytes(int64_t T, int64_t heads, int64_t kv_heads, int dtype, int64_t lut_cols, int64_t B) {
     if (T < 1 || B < 1 || B > uocr::kChunkMaxRequests || heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 1024 ||
         T > (int64_t(1) << 30) / (heads / kv_heads) || lut_cols < 1 || lut_cols > (1 << 22) || B * lut_cols > (int64_t(1) << 30) ||
-        (dtype != UOCR_DTYPE_F32 && dtype != UOCR_DTYPE_BF16))
+        (dtype != UOCR_DTYPE_F32 && dtype != UOCR_DTYPE_BF16) || !chunk_units_ok(T, heads, kv_heads, lut_cols, B))
         return 0;
     uocr::ChunkArgs a{};
     a.T = (int)T; a.B = (int)B; a.heads = (int)heads; a.kv_heads = (int)kv_heads; a.lut_cols = (int)lut_cols;
@@ -348,9 +354,7 @@ int uocr_paged_chunk_attention(const void* q, int64_t q_ld, const void* k_new, i
     if (B * lut_cols > (int64_t(1) << 30))
         return fail(UOCR_EUNSUPPORTED, "paged_chunk_attention: tables of %lld x %lld pages (this build: <= 2^30)", (long long)B,
                     (long long)lut_cols);
-    // The (query tile, head, page) units of a call, with what a tile counts beside its pages, are counted in 32 bits. The form
-    // for few rows has at most three tiles a request: a factor of four is kept free.
-    if ((T * (heads / kv_heads) / 128 + B) * kv_heads > (int64_t(1) << 30) / (lut_cols + 4))
+    if (!chunk_units_ok(T, heads, kv_heads, lut_cols, B))
         return fail(UOCR_EUNSUPPORTED, "paged_chunk_attention: T %lld over %lld pages a request is too much for one call",
                     (long long)T, (long long)lut_cols);
     if (window < 0 || window > INT32_MAX)
