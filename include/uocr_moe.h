@@ -150,8 +150,7 @@ UOCR_API int uocr_paged_decode_attention(const float* q, const float* k_new, con
  * there as three products of fp16 halves, q, keys and values to 2^-22 of themselves (or 2^-29 of their
  * row's largest finite element), weights to 2^-39 of the largest that the row has on their page (where its values' rows are of
  * unlike size: the largest product of a weight and a row's size); bf16 weights rounded to bf16. Within this, hidden
- * rows may decide how a visible one rounds. A
- * visible fp32 key with an element that is not finite makes the row NaN there. A wait inside the
+ * rows may decide how a visible one rounds. A wait inside the
  * kernel that runs out (200 ms) ends it with NaN in the rows concerned.
  * The workspace (uocr_paged_chunk_workspace_bytes(...) bytes on the current device, 0 for sizes that the call
  * refuses; 256-byte aligned, no initial contents) belongs to the call until it has finished. On the tensor cores it holds

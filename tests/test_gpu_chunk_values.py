@@ -168,3 +168,55 @@ def test_small_values(ops, dtype, n, size):
     c.v *= size
     c.pool[:, 1] *= size
     _check(c, ops)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [FEW, MANY])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+@pytest.mark.parametrize("factor", [1.0, -1.0])
+def test_keys_with_infinite_elements(ops, oracle, dtype, n, bad, factor):
+    """A row whose score is -inf has the weight 0, one whose score is +inf or NaN makes the row of out NaN: as the
+    formula, whichever elements of the key are infinite, in cached and in new rows."""
+    c = Case(dtype, n, [200, 130], seed=43)
+    c.scale *= factor
+    cached = [(0, 5, 3), (0, 150, 100), (1, 129, 0)]  # request, row, element
+    for b, r, d in cached:
+        c.pool[c.lut[b, r // 128], 0, c.layer, r % 128, 1, d] = bad
+    c.k[1, 0, 64] = bad  # a new row; its second element of the other sign
+    c.k[1, 0, 65] = -bad
+    got = _np(c.run(ops)[0]).astype(np.float64)
+    q, k, v, pool = (_np(t).astype(np.float64) for t in (c.q, c.k, c.v, c.pool))
+    finite_nan = [0, 0]
+    for b in range(2):
+        for i in range(n[b]):
+            t, rows = int(c.offsets[b]) + i, c.start[b] + i + 1
+            for h in range(2):
+                K = np.stack([pool[c.lut[b, r // 128], 0, c.layer, r % 128, h] if r < c.start[b] else k[c.offsets[b] + r - c.start[b], h]
+                              for r in range(rows)])
+                V = np.stack([pool[c.lut[b, r // 128], 1, c.layer, r % 128, h] if r < c.start[b] else v[c.offsets[b] + r - c.start[b], h]
+                              for r in range(rows)])
+                with np.errstate(invalid="ignore"):
+                    s = (K * q[t, h]).sum(1) * c.scale
+                if np.isnan(s).any() or (s == math.inf).any():
+                    assert np.isnan(got[t, h]).all()
+                    finite_nan[1] += 1
+                    continue
+                seen = np.isfinite(s)
+                p = np.exp(s[seen] - s[seen].max())
+                p /= p.sum()
+                ref, mag = p @ V[seen], p @ np.abs(V[seen])
+                smag = (np.abs(K[seen]) @ np.abs(q[t, h])).max() * abs(c.scale)
+                tol = _bound(dtype, ref, mag, np.float64(smag)) + 2.0 ** -21 * (p @ np.abs(V[seen]).max(1))
+                assert (np.abs(got[t, h] - ref) <= tol).all()
+                finite_nan[0] += 1
+    assert min(finite_nan) > 0
+
+
+@pytest.mark.parametrize("n", [FEW, MANY])
+def test_a_scale_of_zero_and_an_infinite_key(ops, n):
+    """0 times an infinite score is not a number."""
+    c = Case(torch.float32, n, [200, 130], seed=44)
+    c.pool[c.lut[0, 0], 0, c.layer, 7, 1, 9] = math.inf
+    c.scale = 0.0
+    got = _np(c.run(ops)[0])
+    assert np.isnan(got[: n[0], 1]).all() and np.isfinite(got[: n[0], 0]).all() and np.isfinite(got[n[0]: sum(n)]).all()

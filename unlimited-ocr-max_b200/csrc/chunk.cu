@@ -68,13 +68,13 @@ constexpr uint32_t kColS = 0, kColPv = 256, kColQ = 384;
 
 // Beside a page's operands: 1 / scale of each row of k, and of all of them where they share one (else 0); the binary
 // logarithms of 1 / scale of each row of v and of all of them (kUnlike: 0, they do not share one); are there large finite
-// values, of 2^50 or more, bf16 2^65 (kLarge), or rows of v that are not finite (kBad), and which. bf16 has the last two only.
+// values, of 2^50 or more, bf16 2^65 (kLarge), or rows of v or k that are not finite (kBad), and which. bf16 has what is of v's last two only.
 constexpr uint32_t kUnlike = 1, kLarge = 2, kBad = 4;
 struct alignas(16) PageMeta {
     float keys[kPageRows], values_log2[kPageRows];
     float all_keys, all_values_log2;
-    uint32_t values_are, pad;
-    uint32_t bad[4];
+    uint32_t values_are, keys_are;
+    uint32_t bad[4], bad_keys[4];
 };
 
 // The operands of a pass, made by the first launch. Keys and values: page p of request b and head h (of the pass)
@@ -306,10 +306,10 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
 #pragma unroll
             for (int i = 0; i < kWords; ++i) {
                 uint32_t top = __reduce_max_sync(0xffffffffu, top_of(x[i]));
-                if (top >= 0x7F800000u) {  // rare. Elements that are not finite set no scale; of v they leave the operand, with k the row's scores become NaN
+                if (top >= 0x7F800000u) {  // rare. Elements that are not finite leave the operand and set no scale
                     uint32_t m = 0;
                     auto mark = [&](uint32_t& e) {
-                        if (odd_f32(e)) e = v ? 0 : 0x7FFFFFFFu;
+                        if (odd_f32(e)) e = 0;
                         else m = max(m, e & 0x7FFFFFFFu);
                     };
                     mark(x[i].x), mark(x[i].y), mark(x[i].z), mark(x[i].w);
@@ -336,6 +336,7 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
                     meta.values_are = (all ? 0 : kUnlike) | (page_top >> 23 >= 127 + 50 ? kLarge : 0) | any_bad();
                 } else {
                     meta.all_keys = all ? scale_down(page_top) : 0.f;
+                    meta.keys_are = any_bad();
                 }
             }
         } else if (v) {
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
             large = __syncthreads_or(large != 0);
             if (threadIdx.x == 0) meta.values_are = (large ? kLarge : 0) | any_bad();
         }
-        if (v && threadIdx.x < 4) meta.bad[threadIdx.x] = bads[2 * threadIdx.x] | bads[2 * threadIdx.x + 1] << 16;
+        if ((kF32 || v) && threadIdx.x < 4) (v ? meta.bad : meta.bad_keys)[threadIdx.x] = bads[2 * threadIdx.x] | bads[2 * threadIdx.x + 1] << 16;
         unsigned char* out = im.operands + (index * 2 + v) * kOperandBytes<kF32>;
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
@@ -527,15 +528,15 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
 constexpr float kHeadroom = 7.f, kLift = 14.f;
 template <bool kF32>
 constexpr float kRoom = kF32 ? -28.f : 0.f;
-// Row `row` of the values of page t (this head's 128 columns).
+// Row `row` of the keys (v 0) or values (1) of page t (this head's 128 columns).
 template <bool kF32>
-UOCR_DEV const char* value_row(const ChunkArgs& a, const Walk& w, int t, int row) {
+UOCR_DEV const char* cache_row(const ChunkArgs& a, const Walk& w, int t, int row, int v) {
     constexpr int kElt = kF32 ? 4 : 2;
     const int r = t * kPageRows + row, column = (a.head0 + w.head) * kDim;
-    if (r >= w.r.start) return static_cast<const char*>(a.v) + ((size_t)(w.r.lo + r - w.r.start) * a.v_ld + column) * kElt;
+    if (r >= w.r.start) return static_cast<const char*>(v ? a.v : a.k) + ((size_t)(w.r.lo + r - w.r.start) * (v ? a.v_ld : a.k_ld) + column) * kElt;
     const uint32_t id = min(__ldg(a.lut + (size_t)w.b * a.lut_cols + t), (uint32_t)(a.pages - 1));
     return static_cast<const char*>(a.pool) +
-           (((((size_t)id * 2 + 1) * a.layers + a.layer) * kPageRows + row) * ((size_t)a.kv_heads * kDim) + column) * kElt;
+           (((((size_t)id * 2 + v) * a.layers + a.layer) * kPageRows + row) * ((size_t)a.kv_heads * kDim) + column) * kElt;
 }
 
 // Which of 32 columns from c0 on a row sees: c <= hi and (c >= lo or c < pre), all relative to the page.
@@ -610,6 +611,27 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
         if (ends && lane == 0) mbar_arrive(&s.pv_free);
     };
 
+    // fp32: the scores of this half's keys of page t that have elements that are not finite, kept out of the operand: those
+    // elements alone make the score, an infinity or NaN, whatever it is scaled by later. In the place of the tensor core's scores.
+    auto fix_scores = [&](const Walk& w, uint32_t u, int t, int R, uint32_t sa) {
+        const bool valid = R < w.r.n * g;
+        const float* q = static_cast<const float*>(a.q) + (valid ? (size_t)(w.r.lo + token_of(a, R)) * a.q_ld : 0) +
+                         (size_t)((a.head0 + w.head) * g + (valid ? R - token_of(a, R) * g : 0)) * kDim;
+#pragma unroll 1
+        for (int c = 0; c < 64; ++c) {
+            const int key = half * 64 + c;
+            if (!(s.meta[u & 7].bad_keys[key >> 5] >> (key & 31) & 1)) continue;
+            const float* k = reinterpret_cast<const float*>(cache_row<true>(a, w, t, key, 0));
+            float sum = 0.f;
+#pragma unroll 1
+            for (int d = 0; valid && d < kDim; ++d)
+                if (odd_f32(__float_as_uint(k[d]))) sum = fmaf(q[d], k[d], sum);
+            __syncwarp();
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(sa + c), "r"(__float_as_uint(sum * a.scale)) : "memory");
+        }
+        tmem_wait_st();
+    };
+
     // The values of page t that are not finite and were kept out of its operand
     auto add_bad = [&](const Walk& w, uint32_t u, int t, int pos) __attribute__((always_inline)) {
         for (int q = 0; q < kPageRows; ++q) {
@@ -617,7 +639,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
             const int r = t * kPageRows + q;
             const bool seen = r <= pos && (a.window <= 0 || r > pos - a.window || r < w.r.prefix);
             if (!seen) continue;
-            const char* p = value_row<kF32>(a, w, t, q) + half * (kF32 ? 256 : 128);
+            const char* p = cache_row<kF32>(a, w, t, q, 1) + half * (kF32 ? 256 : 128);
             auto odd = [](float v) { return odd_f32(__float_as_uint(v)) ? v : 0.f; };
 #pragma unroll
             for (int d = 0; d < 32; ++d) {
@@ -677,6 +699,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
             uint32_t x[64];
             float top = -INFINITY;
             if (run) {
+                if (kF32 && __float_as_uint(page.w)) fix_scores(now, u, c0 / kPageRows, R, sa);
                 tmem_ld64(sa, x);
                 if (kF32 && all_keys == 0.f) {
                     asm volatile("");
