@@ -145,9 +145,11 @@ UOCR_API int uocr_paged_decode_attention(const float* q, const float* k_new, con
  * rows beyond the lookup table are in no request. Rows of out in no request are left as they were. What a row
  * does not see does not reach it, whatever it holds (NaN and infinities included). A page row that the call
  * stores is read or stored for no other request of the call.
- * Sums and softmax in fp32, the sums below the values (no overflow in front of the division). Two forms, by T x heads / kv_heads against B: up to 16 (fp32; bf16 8) rows of
- * (token, query head) a request and KV head on average are computed on the fp32 units, more on the tensor cores: fp32
- * there as three products of fp16 halves, q, keys and values to 2^-22 of themselves (or 2^-29 of their
+ * Sums and softmax in fp32, the sums below the values (no overflow in front of the division). Two forms, by
+ * T x heads / kv_heads against B: up to 16 (fp32; bf16 8) rows of (token, query head) a request and KV head on average are
+ * computed on the fp32 units, more on the tensor cores. All requests of a call take one form, and rows in no request and empty
+ * requests count: single tokens and long chunks, or a batch with many padded rows, are faster as calls of their own. fp32
+ * is computed on the tensor cores as three products of fp16 halves, q, keys and values to 2^-22 of themselves (or 2^-29 of their
  * row's largest finite element), weights to 2^-39 of the largest that the row has on their page (where its values' rows are of
  * unlike size: the largest product of a weight and a row's size); bf16 weights rounded to bf16. Within this, hidden
  * rows may decide how a visible one rounds. A wait inside the

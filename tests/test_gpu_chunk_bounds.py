@@ -110,3 +110,43 @@ def test_offsets_of_any_kind_write_inside_only(ops, dtype, n):
         got = ops.paged_chunk_attention(*_flat(c))
         assert torch.equal(got, want) and bool(torch.isfinite(got).all())
     assert pages > 1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [[1], [3], [150]])
+def test_tables_rows_and_pools_of_other_layouts(ops, dtype, n):
+    """Tables of uint32, transposed or cut from wider ones; broadcast keys and values; rows of one token with a stride of their own;
+    a pool inside a larger tensor."""
+    c = Case(dtype, n, [300], heads=4, kv_heads=2, seed=94, lut_pad=1)
+    args = _flat(c)
+    want = ops.paged_chunk_attention(*args)
+    stored = args[3].clone()
+
+    def same(**change):
+        a = _flat(c)
+        for i, v in change.items():
+            a[int(i[1:])] = v
+        got = ops.paged_chunk_attention(*a)
+        assert torch.equal(got, want) and torch.equal(_bits(a[3]), _bits(stored))
+
+    lut = args[5]
+    same(_5=lut.to(torch.int64).to(torch.uint32))
+    same(_5=lut.t().contiguous().t())
+    same(_5=torch.cat([lut, lut], 1)[:, : lut.shape[1]])
+    same(_5=torch.cat([lut, lut], 1).to(torch.int64).to(torch.uint32)[:, : lut.shape[1]])
+    same(_6=torch.stack([args[6], args[6]], 1)[:, 0], _7=torch.stack([args[7], args[7]], 1)[:, 1])
+    same(_0=torch.cat([args[0], args[0]], 1)[:, :4], _2=torch.cat([args[2], args[2], args[2]], 1)[:, 2:4])
+    big = torch.zeros(c.pool.numel() + 64, dtype=dtype, device=DEV)
+    pool = big[64:].view(c.pool.shape)
+    pool.copy_(c.pool)
+    same(_3=pool)
+    assert bool((big[:64] == 0).all())
+    a = _flat(c)
+    one = a[1][:1, :1].expand(len(c.k), 2, 128)  # one key for all rows and heads
+    a[1] = one
+    b = _flat(c)
+    b[1] = one.contiguous()
+    assert torch.equal(ops.paged_chunk_attention(*a), ops.paged_chunk_attention(*b)) and torch.equal(_bits(a[3]), _bits(b[3]))
+    with pytest.raises(ValueError, match="16-byte"):
+        at = torch.zeros(c.pool.numel() + 1, dtype=dtype, device=DEV)[1:].view(c.pool.shape)
+        ops.paged_chunk_attention(*args[:3], at, *args[4:])

@@ -19,7 +19,8 @@
 // Three launches, each begun while the one in front of it ends:
 // 1. chunk_operands_kernel turns every visible page's k and v and every query tile into the tensor core's operands, in
 //    the workspace, and stores the new rows in the pool. Each row is converted once, however many query tiles read
-//    it (8192 fp32 tokens of 10 heads: 1.05 ms against 1.72 where every tile's CTA converted them for itself).
+//    it (8192 fp32 tokens of 10 heads: 1.05 ms in a first version, 1.72 with every tile's CTA converting them for itself;
+//    0.46 ms now).
 // 2. chunk_attention_kernel: one warp copies operands into a ring in shared memory (bulk copies), one issues
 //    tcgen05.mma, 8 warps do the softmax, two threads per query row. The query operand and the weights P are read by
 //    the tensor core from TMEM, so shared memory carries each key and value once:
@@ -32,15 +33,19 @@
 // scaled by a power of two that brings their largest element to [2^14, 2^15), and a row's weights on a page to at most
 // 2^14, so the halves keep their bits over fp16's exponent range. The small products go into the accumulator
 // first: the tensor core's additions truncate, and only the last 8 then round at the result's full size. bf16: one
-// product; the weights are rounded to bf16, as the tensor core takes both operands in one type.
+// product; the weights are rounded to bf16, as the tensor core takes both operands in one type (0.0022 of the result off
+// against 64 bits, of which rounding the result itself is 0.0017; halves of the weights would cost a second product).
 // Values that are not finite are kept out of the V operand (0 x inf would reach rows that do not see
-// them) and added to the rows that do see them.
+// them) and added to the rows that do see them; elements of fp32 keys that are not finite are kept out of the K operand, and
+// make the rows' scores by themselves. A hidden row has the weight 0, and its size takes no part either: where a page's rows of
+// values are not within 2^10 of one another, each has a scale of its own, which goes into its weight (8192 tokens with
+// such pages throughout: 541 us against 459).
 //
 // Measured (B200). fp32, 8192 tokens of 10 heads: operands 64 us (HBM, 5.2 TB/s), attention 380 us (1.38 PFLOP/s of fp16
 // products, 0.82 of a cuBLAS bf16 burst; a page takes 3900 cycles, of which the tensor core works 3.1 k: the rest is the softmax
 // warps' exponentials, rounding and waits), joining 5 us; long loops of calls run into the power limit
-// (500 us a call). bf16, requests of 2048 and 767 tokens over 6000 and 2249
-// rows, 32 heads over 8: operands 27 us, attention 333 us (3000 cycles a page, the tensor core 1024: the
+// (530 us a call). bf16, requests of 2048 and 767 tokens over 6000 and 2249
+// rows, 32 heads over 8: operands 27 us, attention 337 us (3000 cycles a page, the tensor core 1024: the
 // softmax warps bound it, 1024 for the exponentials alone). Taken and dropped: four threads a row (spills; 4700 cycles),
 // k and v of a page converted by CTAs of their own (no faster), exponentials and rounding alternated (no change).
 #include "chunk.cuh"
@@ -68,7 +73,8 @@ constexpr uint32_t kColS = 0, kColPv = 256, kColQ = 384;
 
 // Beside a page's operands: 1 / scale of each row of k, and of all of them where they share one (else 0); the binary
 // logarithms of 1 / scale of each row of v and of all of them (kUnlike: 0, they do not share one); are there large finite
-// values, of 2^50 or more, bf16 2^65 (kLarge), or rows of v or k that are not finite (kBad), and which. bf16 has what is of v's last two only.
+// values, of 2^50 or more, bf16 2^65 (kLarge), or rows of v or k that are not finite (kBad), and which. Of these bf16 has
+// values_are and bad only.
 constexpr uint32_t kUnlike = 1, kLarge = 2, kBad = 4;
 struct alignas(16) PageMeta {
     float keys[kPageRows], values_log2[kPageRows];
@@ -1032,12 +1038,14 @@ cudaError_t launch_chunk_join(const ChunkArgs& a, const ChunkParts& p, cudaStrea
     return launch_dependent(a.bf16 ? chunk_join_kernel<false> : chunk_join_kernel<true>, grid, 256, 0, st, a, p);
 }
 
-// Rows of a query tile: 1 to 8 where a request has few (token, head) rows of a KV head on average (chunk_rows.cu: bound
-// by the cache's bytes), else 128 (tensor cores). Measured at 8 requests of 8000 rows, 10 heads: fp32, 16 rows 274 us
-// against 353; bf16 (16 heads), 8 rows 217 us against 287; beyond the rule, a little earlier: fp32, 24 rows 464 us against 359;
-// bf16, 9 rows 469 against 292. The tile's rows cost time too (fp32, 2 to 8 rows: 107 to 145 us): a whole average is taken for every request's
-// number of rows, with another one they differ and twice the average less one is provided for, since a second tile
-// reads the cache again.
+// Rows of a query tile: 1 to 8 where a request has few (token, head) rows of a KV head on average (chunk_rows.cu: bound by
+// the cache's bytes), else 128 (tensor cores). One form for the whole call, by T (rows in no request among them) and B
+// (empty requests among them), as the lengths are on the device: 63 single tokens over 639 rows and a chunk of 512 over
+// 7700 take 1149 us in one call, 82 + 105 in two; 7 single tokens over 8000 rows beside that chunk 401, 109 + 105 in two.
+// Measured at 8 requests of 8000 rows, 10 heads: fp32, 16 rows 274 us against 353; bf16 (16 heads), 8 rows 217 us against
+// 287; beyond the rule, a little earlier: fp32, 24 rows 464 us against 359; bf16, 9 rows 469 against 292. The tile's rows
+// cost time too (fp32, 2 to 8 rows: 107 to 145 us): a whole average is taken for every request's number of rows, with
+// another one they differ and twice the average less one is provided for, since a second tile reads the cache again.
 static int tile_rows(const ChunkArgs& a) {
     const long long rows = (long long)a.T * (a.heads / a.kv_heads);
     if (rows > (a.bf16 ? 8ll : 16ll) * a.B) return kTile;

@@ -16,7 +16,7 @@
 // Measured (B200, fp32, 10 heads): 8 requests over 8000 rows, 656 MB: 1 row each 105 us (6.2 TB/s), 4 rows 110, 8 rows
 // 145 (the fp32 units bound it: every element takes part in 8 products). 1 to 5 drafted tokens over contexts of 997 to
 // 8000 rows, 368 MB: 74 us, 5.0 TB/s (the request of 5 has two tiles of 3 and is read twice). Short calls are bound by
-// latency: one request of 640 rows 10.8 us with the joining launch, 8 requests of 77 to 639 rows (29 MB) 14.6; 256
+// latency: one request of 640 rows 11.0 us with the joining launch, 8 requests of 77 to 639 rows (29 MB) 14.5; 256
 // requests of 100 rows (265 MB) 74 us, 3.6 TB/s: tiles of one page, 4 us each for the chain table, keys, scores, values,
 // join (the next tile found a tile ahead: 71 us, but 11.5 for the one request, and not kept). Smaller units would
 // shorten it for one short request only, and cost the long ones their streams.

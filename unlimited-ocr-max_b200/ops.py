@@ -340,8 +340,10 @@ def paged_chunk_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Ten
     on several streams and be captured. The result is deterministic. No page row that the call stores is in
     another request's table. ``T * heads / kv_heads`` against the number of requests decides the form: up
     to 16 (bf16: 8) rows a request and KV head are computed straight from the cache, more on the tensor
-    cores. There fp32 rows are taken to 2^-29 of their largest element, and the workspace grows with ``B * cols``: 128 KB (bf16: 64 KB) a page
-    and KV head, up to 1 GiB or one head's share.
+    cores. All requests of a call take one form: single tokens and long chunks are faster as calls of their
+    own, and so are batches without padded rows. On the tensor cores fp32 rows are taken to 2^-29 of their
+    largest element, bf16 weights are rounded to bf16, and the workspace grows with ``B * cols``: 128 KB
+    (bf16: 64 KB) a page and KV head, up to 1 GiB or one head's share.
     """
     op = "paged_chunk_attention"
     tensors = [q, k_new, v_new, kv_pool, lut, row_offsets, start]
