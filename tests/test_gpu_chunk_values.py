@@ -220,3 +220,22 @@ def test_a_scale_of_zero_and_an_infinite_key(ops, n):
     c.scale = 0.0
     got = _np(c.run(ops)[0])
     assert np.isnan(got[: n[0], 1]).all() and np.isfinite(got[: n[0], 0]).all() and np.isfinite(got[n[0]: sum(n)]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [FEW, MANY])
+@pytest.mark.parametrize("where", ["page", "window"])
+def test_small_values_beside_large_ones_that_are_not_seen(ops, dtype, n, where):
+    """Rows of 1e30 on the pages of rows of 1e-30: of later tokens, or outside the window."""
+    c = Case(dtype, n, [300, 129], seed=46, **HEADS)
+    c.v *= 1e-30
+    c.pool[:, 1] *= 1e-30
+    if where == "page":
+        c.v[n[0] - 1] = 1e30
+        c.v[sum(n) - 1] = 1e30
+        _check(c, ops)
+    else:
+        for r in range(140, 180):
+            c.pool[c.lut[0, r // 128], 1, c.layer, r % 128] *= 1e20
+            c.pool[c.lut[0, r // 128], 1, c.layer, r % 128] *= 1e20
+        _check(c, ops, window=120, prefix=[139, 0])

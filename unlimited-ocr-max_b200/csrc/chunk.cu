@@ -72,9 +72,8 @@ constexpr uint32_t kTeamBar = 1, kPairBar = 2;  // all softmax warps; the two wa
 constexpr uint32_t kColS = 0, kColPv = 256, kColQ = 384;
 
 // Beside a page's operands: 1 / scale of each row of k, and of all of them where they share one (else 0); the binary
-// logarithms of 1 / scale of each row of v and of all of them (kUnlike: 0, they do not share one); are there large finite
-// values, of 2^50 or more, bf16 2^65 (kLarge), or rows of v or k that are not finite (kBad), and which. Of these bf16 has
-// values_are and bad only.
+// logarithms of 1 / scale of each row of v and of all of them (kUnlike: they do not share one); are there rows of v or k that
+// are not finite (kBad), and which. bf16 has values_are and bad only, and there: are there finite values of 2^65 or more (kLarge)?
 constexpr uint32_t kUnlike = 1, kLarge = 2, kBad = 4;
 struct alignas(16) PageMeta {
     float keys[kPageRows], values_log2[kPageRows];
@@ -339,7 +338,7 @@ __global__ void __launch_bounds__(256, 2) chunk_operands_kernel(ChunkArgs a, Ima
             if (threadIdx.x == 0) {
                 if (v) {
                     meta.all_values_log2 = all ? scale_down_log2(page_top) : 0.f;
-                    meta.values_are = (all ? 0 : kUnlike) | (page_top >> 23 >= 127 + 50 ? kLarge : 0) | any_bad();
+                    meta.values_are = (all ? 0 : kUnlike) | any_bad();
                 } else {
                     meta.all_keys = all ? scale_down(page_top) : 0.f;
                     meta.keys_are = any_bad();
@@ -528,10 +527,13 @@ __device__ void mma_role(const ChunkArgs& a, Shared& s, unsigned char* ring, int
 // its own additions truncate (the threads' round to nearest: 8.6e-7 off at 8192 rows, 1.2e-6 with two pages to a sum and
 // no faster); the weights' fp16 halves resolve 2^-25, so they are 2^(score - the page's maximum + 14), 2^-39 of the page's
 // largest, and the page's sum takes 2^(its maximum - m - 14): weights of 2^-60 beside values of 2^70 count in full.
-// m is `room` above the maximum. From a page on that holds large values it is so by the logarithm of the tile's rows and the
-// headroom, so that the sums stay below the values, up to the type's largest ones. Up to there it is 28 below in fp32, where the
-// scale of a page's sum is 2^-28 of its values (so values down to the type's smallest normal ones keep their bits).
-constexpr float kHeadroom = 7.f, kLift = 14.f;
+// m is `room` above the maximum. From a page on on which a row sees large values it is so by the logarithm of the tile's rows and
+// the headroom, so that the sums stay below the values, up to the type's largest ones. Up to there it is 28 below in fp32, where the
+// scale of a page's sum is 2^-28 of its values (so values down to the type's smallest normal ones keep their bits). Large:
+// in bf16 the page has some of 2^65 or more; in fp32 the largest product of a weight and a value of the page reaches 2^50 or so, the
+// weight 1 being the largest so far (a page's sum is below 2^86 until then, 2^22 of them in range). The row's own products: what it
+// does not see does not decide.
+constexpr float kHeadroom = 7.f, kLift = 14.f, kLarge32 = 64.f;
 template <bool kF32>
 constexpr float kRoom = kF32 ? -28.f : 0.f;
 // Row `row` of the keys (v 0) or values (1) of page t (this head's 128 columns).
@@ -741,49 +743,47 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
             const float other = s.xmax[u & 1][half ^ 1][row];
             alive = alive && other == other;
             const float page_max = fmaxf(top, other);
-            float mn = m, keep = 1.f;
-            if ((values_are & kLarge) && room == kRoom<kF32>) {
+            // The operand's weights are 2^(score - ref), in fp32 times 2^14; products with the values' operand count 2^ref_log2 more.
+            float ref = page_max, ref_log2 = page.y, unlike_sum = 0.f;
+            const bool unlike = kF32 && alive && (values_are & kUnlike);
+            if (unlike) {
+                // A scale for each row of v: its weight takes 1 / scale, and the operand's weights are relative to the largest
+                // of these products, of the rows that this one sees. l takes the weights alone.
+                float most = -INFINITY;
+                if (run) {
+                    const float shift = kLift - (page_max == -INFINITY ? 0.f : page_max);
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        const float score = __uint_as_float(x[i]) * factor;
+                        unlike_sum += exp2_fast(score + shift);
+                        const float w = score + pm.values_log2[half * 64 + i];
+                        most = fmaxf(most, w);
+                        x[i] = __float_as_uint(w);
+                    }
+                }
+                s.xref[half][row] = most;
+                named_bar_sync(pair_bar, 64);
+                ref = fmaxf(most, s.xref[half ^ 1][row]);
+                ref_log2 = 0.f;
+                factor = 1.f;
+            }
+            float mn = fmaxf(m, page_max + room), keep = 1.f;
+            if (room == kRoom<kF32> && (kF32 ? ref + ref_log2 > mn + kLarge32 : (values_are & kLarge) && page_max != -INFINITY)) {
                 asm volatile("");  // a branch, rarely taken
                 room = kHeadroom + 7.f + (32 - __clz(now.t.count - 1));
-                mn = m + (room - kRoom<kF32>);
+                mn += room - kRoom<kF32>;
             }
-            mn = fmaxf(mn, page_max + room);
             const bool raised = __any_sync(0xffffffffu, mn > m + kHeadroom);  // the same in both warps of the rows
             if (raised) {
                 keep = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
                 l *= keep;
                 m = mn;
             }
-            // the operand's weights are 2^(score - ref), times 2^14 in fp32; one of 1 there counts `unit` in l, and a product
-            // with the values' operand `sum_scale` in the sums
-            float ref = kF32 ? page_max : m;
-            auto counts = [&](float log2) { return ref == -INFINITY ? 0.f : exp2_fast(ref - m + (log2 - kLift)); };
-            const float unit = kF32 ? counts(0.f) : 1.f;
+            // a weight of 1 in the operand counts `unit` in l, and a product `sum_scale` in the sums
+            if (!kF32) ref = m;
+            const float unit = !kF32 ? 1.f : page_max == -INFINITY ? 0.f : exp2_fast(page_max - m - kLift);
             const float old_scale = sum_scale;
-            if (kF32) sum_scale = counts(page.y);
-            const bool unlike = kF32 && alive && (values_are & kUnlike);
-            if (unlike) {
-                // A scale for each row of v: its weight takes 1 / scale, and the operand's weights are relative to the largest
-                // of these products, of the rows that this one sees. l takes the weights alone.
-                float most = -INFINITY, sum = 0.f;
-                if (run) {
-                    const float shift = kLift - (ref == -INFINITY ? 0.f : ref);
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) {
-                        const float score = __uint_as_float(x[i]) * factor;
-                        sum += exp2_fast(score + shift);
-                        const float w = score + pm.values_log2[half * 64 + i];
-                        most = fmaxf(most, w);
-                        x[i] = __float_as_uint(w);
-                    }
-                    l = fmaf(sum, unit, l);
-                }
-                s.xref[half][row] = most;
-                named_bar_sync(pair_bar, 64);
-                ref = fmaxf(most, s.xref[half ^ 1][row]);
-                factor = 1.f;
-                sum_scale = counts(0.f);
-            }
+            if (kF32) sum_scale = ref == -INFINITY ? 0.f : exp2_fast(ref - m + (ref_log2 - kLift));
             const bool fresh = j % kSumPages<kF32> == 0;  // a new sum in TMEM
             if (run) {
                 const float base = (kF32 ? kLift : 0.f) - (ref == -INFINITY ? 0.f : ref);
@@ -812,7 +812,7 @@ __device__ void team_role(const ChunkArgs& a, Shared& s, const Images& im, const
                 }
                 uint32_t u0, u1;
                 unpair(add2(sum2[0], sum2[1]), u0, u1);
-                if (!unlike) l += (__uint_as_float(u0) + __uint_as_float(u1)) * unit;
+                l += (unlike ? unlike_sum : __uint_as_float(u0) + __uint_as_float(u1)) * unit;
                 tmem_wait_st();
                 tc_fence_before();
             }
